@@ -60,7 +60,13 @@ enum {
 };
 
 /* bits of the device status word */
-enum { OC_STATUS_TIMEOUT = 1, OC_STATUS_BAD_PAGE = 2, OC_STATUS_BAD_SEQLEN = 4 };
+enum {
+  OC_STATUS_TIMEOUT = 1,
+  OC_STATUS_BAD_PAGE = 2,
+  OC_STATUS_BAD_SEQLEN = 4,
+  OC_STATUS_POSITION = 8, /* a position, length or sequence outside its tables */
+  OC_STATUS_PAGES = 16    /* oc_reserve_pages: too few free pages or table columns */
+};
 
 /* gate selector of oc_fused_attention_paged */
 enum { OC_GATE_ZETA = 0, OC_GATE_CAUCHY_SCHWARZ = 2 };
@@ -350,6 +356,144 @@ int oc_fused_attention_v2_noalloc(const void* q, int q_dtype, int64_t q_head_str
                                   int num_heads, int64_t seq_len, int head_dim, double zeta_max,
                                   int num_splits, int num_sms, void* out, int out_dtype, int64_t out_head_stride,
                                   uint8_t* mask_out, uint32_t* retained, uint32_t* status, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Serving from a paged cache: rotary embedding with append, exact attention
+ * of one new token and of packed prompts, and page bookkeeping.
+ *
+ * A paged cache is a tensor (num_blocks, kv_heads, block_size, head_dim) and
+ * a block table (num_seqs, max_blocks) int32 of page ids, -1 where a sequence
+ * holds no page.  Strides are in elements; the last dimension is contiguous.
+ * Arguments are passed as a struct, which the caller zero-initialises.
+ * ------------------------------------------------------------------------ */
+
+/* oc_rotary_append_paged: rotary embedding of q (tokens, q_heads, head_dim)
+ * into q_out and of k into k_out and / or the cache, and the append of k and
+ * v to the cache.  Token t sits at positions[t] of sequence seq_ids[t]
+ * (seq_ids NULL: sequence t; a negative id: no append).  Columns [0,
+ * rotary_dim) turn, in pairs (i, i + rotary_dim / 2), or (2i, 2i + 1) with
+ * OC_ROTARY_INTERLEAVED, by the angle whose cosine and sine are cos_tab /
+ * sin_tab (table_rows, rotary_dim / 2) float32; OC_ROTARY_INVERSE turns back.
+ * rotary_dim 0: no rotation.  q, k (with v), k_out and the caches are each
+ * optional.  Caches are of dtype, or OC_F8E4M3 holding round(k / k_scale),
+ * saturated.  A position outside the tables or the block table, and a page
+ * outside [0, num_blocks), sets OC_STATUS_POSITION / OC_STATUS_BAD_PAGE and
+ * skips the token's append. */
+enum { OC_ROTARY_INTERLEAVED = 1, OC_ROTARY_INVERSE = 2 };
+typedef struct {
+  const void *q, *k, *v;
+  void *q_out, *k_out;
+  int64_t q_tok_stride, q_head_stride, k_tok_stride, k_head_stride, v_tok_stride, v_head_stride;
+  int64_t qo_tok_stride, qo_head_stride, ko_tok_stride, ko_head_stride;
+  int64_t tokens;
+  const void* positions; /* int32, or int64 with positions_64 */
+  const int32_t* seq_ids;
+  const float *cos_tab, *sin_tab;
+  int64_t table_rows;
+  void *k_cache, *v_cache;
+  int64_t kc_block_stride, kc_head_stride, kc_tok_stride, vc_block_stride, vc_head_stride, vc_tok_stride;
+  const int32_t* block_tables;
+  int64_t block_table_stride, num_blocks;
+  uint32_t* status;
+  float k_scale, v_scale;
+  int q_heads, kv_heads, head_dim, rotary_dim, dtype, cache_dtype, positions_64, flags, block_size, max_blocks,
+      num_seqs, num_sms;
+} oc_rotary_args;
+int oc_rotary_append_paged(const oc_rotary_args* args, void* stream);
+
+/* oc_paged_decode_attention: o = softmax(s) V for the newest token of each
+ * sequence, q (num_seqs, kv_heads * group, head_dim), over the first
+ * seq_lens[i] tokens of its pages (the query sits at seq_lens[i] - 1):
+ *   x = scale * k_scale * q.k_j;  x = softcap * tanh(x / softcap) if softcap > 0;
+ *   s_j = x + slopes[h] * (j - (seq_lens[i] - 1));
+ * with window > 0 only the last window keys are seen.  A sequence of length 0
+ * gives 0 and lse -inf.  Keys and values of other slots of a page are never
+ * used, whatever they hold.  lse (num_seqs, heads) float32, natural
+ * logarithm, is optional.  Caches are of dtype, or both OC_F8E4M3.
+ * workspace: oc_paged_decode_workspace_bytes() of the same arguments. */
+typedef struct {
+  const void *q, *k_cache, *v_cache;
+  void* out;
+  float* lse;
+  const float* slopes;
+  const int32_t *block_tables, *seq_lens;
+  int64_t q_seq_stride, q_head_stride, out_seq_stride, out_head_stride;
+  int64_t kc_block_stride, kc_head_stride, kc_tok_stride, vc_block_stride, vc_head_stride, vc_tok_stride;
+  int64_t block_table_stride, num_blocks;
+  uint32_t* status;
+  void* workspace;
+  size_t workspace_bytes;
+  float scale, softcap, k_scale, v_scale;
+  int num_seqs, kv_heads, group, head_dim, dtype, cache_dtype, block_size, max_blocks, window, num_sms;
+} oc_paged_decode_args;
+size_t oc_paged_decode_workspace_bytes(const oc_paged_decode_args* args);
+int oc_paged_decode_attention(const oc_paged_decode_args* args, void* stream);
+
+/* oc_prompt_attention: attention of packed documents over themselves (cu_q
+ * NULL: one document, all queries over all keys).  Document d holds queries [cu_q[d], cu_q[d + 1]) and keys [cu_k[d],
+ * cu_k[d + 1]); its query i sits at position i + (keys - queries).  A query
+ * at p sees key j of its document if j < prefix_lens[d] (when given), or if
+ * (j <= p or not causal) and (window == 0 or j > p - window).  Scores as in
+ * oc_paged_decode_attention, with the bias - slopes[h] * |p - j|.  A query
+ * that sees nothing, and a row outside every document, gives 0 and lse -inf.
+ * lse (tokens, heads) float32 is optional.  OC_F16, OC_BF16: head_dim a
+ * multiple of 8 up to 128; OC_F32: head_dim up to 256. */
+typedef struct {
+  const void *q, *k, *v;
+  void* out;
+  float* lse;
+  const float* slopes;
+  const int32_t *cu_q, *cu_k, *prefix_lens;
+  int64_t q_tok_stride, q_head_stride, k_tok_stride, k_head_stride, v_tok_stride, v_head_stride;
+  int64_t out_tok_stride, out_head_stride, lse_tok_stride;
+  int64_t tokens, key_tokens;
+  uint32_t* status;
+  float scale, softcap;
+  int docs, kv_heads, group, head_dim, dtype, causal, window, num_sms;
+} oc_prompt_args;
+int oc_prompt_attention(const oc_prompt_args* args, void* stream);
+
+/* Page bookkeeping.  refcounts (num_pages) int32 counts the table entries
+ * that name a page; 0 is free.  caches is a host array of num_caches device
+ * pointers whose pages are page_bytes contiguous bytes at multiples of
+ * page_strides[i] bytes. */
+
+/* Copies page src[i] to dst[i] of every cache; a negative id skips the pair.
+ * No dst may be another pair's src or dst. */
+int oc_copy_pages(void* const* caches, const int64_t* page_strides, int num_caches, int64_t page_bytes,
+                  int64_t num_pages, const int32_t* src, const int32_t* dst, int64_t n, uint32_t* status, int num_sms,
+                  void* stream);
+
+/* Row i of the outputs becomes sequence source[i] of the inputs (all rows at
+ * once): i keeps the row whole, another row shares the pages that hold its
+ * tokens, a negative source frees the row.  refs_out = refs_in with the
+ * entries that came and went.  Outputs do not alias inputs. */
+int oc_fork_sequences(const int32_t* table_in, int64_t table_in_stride, int32_t* table_out, int64_t table_out_stride,
+                      const int32_t* lens_in, int32_t* lens_out, const int32_t* refs_in, int32_t* refs_out,
+                      const int32_t* source, int num_seqs, int max_blocks, int64_t num_pages, int block_size,
+                      uint32_t* status, void* stream);
+
+/* Gives every sequence room for wanted[i] tokens, in place: a partly filled
+ * last page that others hold too is copied (the last of its holders keeps it
+ * if all of them grow), and pages are added.  The k-th page needed, by row and
+ * column, is the k-th lowest free one.  All or nothing: if pages or table
+ * columns do not suffice, nothing changes and OC_STATUS_PAGES is set.
+ * workspace: oc_reserve_workspace_bytes(num_seqs, num_pages) bytes. */
+size_t oc_reserve_workspace_bytes(int num_seqs, int64_t num_pages);
+int oc_reserve_pages(void* const* caches, const int64_t* page_strides, int num_caches, int64_t page_bytes,
+                     int32_t* table, int64_t table_stride, const int32_t* lens, int32_t* refs, const int32_t* wanted,
+                     int num_seqs, int max_blocks, int64_t num_pages, int block_size, void* workspace,
+                     size_t workspace_bytes, uint32_t* status, int num_sms, void* stream);
+
+/* Moves the pages in use to the lowest ids: the k-th used page at or above
+ * their number goes to the k-th free one below it.  Cache contents move in
+ * place; the table and the counts are written to outputs that do not alias
+ * the inputs.  workspace: oc_compact_workspace_bytes(num_pages) bytes. */
+size_t oc_compact_workspace_bytes(int64_t num_pages);
+int oc_compact_pages(void* const* caches, const int64_t* page_strides, int num_caches, int64_t page_bytes,
+                     const int32_t* table_in, int64_t table_in_stride, int32_t* table_out, int64_t table_out_stride,
+                     const int32_t* refs_in, int32_t* refs_out, int num_seqs, int max_blocks, int64_t num_pages,
+                     void* workspace, size_t workspace_bytes, uint32_t* status, int num_sms, void* stream);
 
 #ifdef __cplusplus
 }

@@ -29,6 +29,9 @@ from .decode_gate import (
 from .gqa_eviction import fused_orthocache_attention_v3_gqa
 from .paged_eviction import fused_orthocache_attention_paged
 from .norm_cache import SpectralNormCache, create_norm_cache_for_model, tile_high_norms
+from .exact_attention import paged_decode_attention, prompt_attention
+from .pages import PagedKVCache, compact_pages, copy_pages, fork_sequences, reserve_pages
+from .rotary import rotary_append_paged, rotary_embedding, rotary_tables
 from .pipeline import BypassFlag, GPUProfile, TelemetryLevel, format_bypass_reason, orthocache_forward
 
 __version__ = "0.1.0"
@@ -54,6 +57,16 @@ __all__ = [
     "SpectralNormCache",
     "create_norm_cache_for_model",
     "tile_high_norms",
+    "rotary_tables",
+    "rotary_embedding",
+    "rotary_append_paged",
+    "paged_decode_attention",
+    "prompt_attention",
+    "PagedKVCache",
+    "copy_pages",
+    "fork_sequences",
+    "reserve_pages",
+    "compact_pages",
     "TILE_SIZE",
     "BAND_DC_64",
     "BAND_LOW_64",

@@ -21,7 +21,9 @@ OC_F32, OC_F16, OC_BF16, OC_F8E4M3 = 0, 1, 2, 3
 OC_GATE_ZETA, OC_GATE_CAUCHY_SCHWARZ = 0, 2
 STATUS_BITS = {1: "a shared-memory pipeline wait timed out",
                2: "a block-table entry was outside [0, num_blocks)",
-               4: "a seq_lens entry was negative, not a multiple of 64, or beyond the block table"}
+               4: "a seq_lens entry was negative, not a multiple of 64, or beyond the block table",
+               8: "a position, length or sequence was outside its tables",
+               16: "too few free pages or block-table columns: no page was reserved"}
 
 _DTYPE = {torch.float32: OC_F32, torch.float16: OC_F16, torch.bfloat16: OC_BF16,
           torch.float8_e4m3fn: OC_F8E4M3}
@@ -63,6 +65,18 @@ SIGNATURES = {
     "oc_gemv_qkv_rope": (_i, [_vp, _vp, _vp, C.c_float, _vp, _vp, _i64, _i64, _i, _i, _i, _vp, _vp, _vp, _vp, _vp,
                               _vp, _i64, _i, _vp]),
     "oc_tail_merge": (_i, [_vp, _i, _i, _i, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _vp, C.c_float, _vp, _i, _vp]),
+    "oc_rotary_append_paged": (_i, [_vp, _vp]),
+    "oc_paged_decode_workspace_bytes": (_sz, [_vp]),
+    "oc_paged_decode_attention": (_i, [_vp, _vp]),
+    "oc_prompt_attention": (_i, [_vp, _vp]),
+    "oc_copy_pages": (_i, [_vp, _vp, _i, _i64, _i64, _vp, _vp, _i64, _vp, _i, _vp]),
+    "oc_fork_sequences": (_i, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i, _i, _i64, _i, _vp, _vp]),
+    "oc_reserve_workspace_bytes": (_sz, [_i, _i64]),
+    "oc_reserve_pages": (_i, [_vp, _vp, _i, _i64, _vp, _i64, _vp, _vp, _vp, _i, _i, _i64, _i, _vp, _sz, _vp, _i,
+                              _vp]),
+    "oc_compact_workspace_bytes": (_sz, [_i64]),
+    "oc_compact_pages": (_i, [_vp, _vp, _i, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i, _i, _i64, _vp, _sz, _vp, _i,
+                              _vp]),
     "oc_fused_attention_v3_shard": (_i, [_vp, _i, _i64, _vp, _i, _i64, _i64, _vp, _i, _i64, _i64, _i, _i, _i64,
                                          _i, _d, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
 }
@@ -113,6 +127,25 @@ def binding():
             spec.loader.exec_module(mod)
             _binding = mod
     return _binding
+
+
+def require_binding():
+    """The compiled binding; raises if it has not been built (the serving operators have no ctypes path)."""
+    b = binding()
+    if b is None:
+        raise RuntimeError("orthocache_gpu_b200: the compiled binding (_lib/oc_torch.so) is not built, or "
+                           "ORTHOCACHE_B200_LIB selects another library; run `python -m orthocache_gpu_b200._build`")
+    return b
+
+
+def call_context(t: torch.Tensor):
+    """(SM count, status word address, stream) of a call on ``t``'s device; zeros for a CPU tensor, which the
+    binding refuses."""
+    dev = t.device
+    if dev.type != "cuda":
+        return 0, 0, 0
+    st = stream_ptr(dev)
+    return num_sms(dev), workspace(dev, st).status_ptr, st
 
 
 def dtype_code(t: torch.Tensor) -> int:
