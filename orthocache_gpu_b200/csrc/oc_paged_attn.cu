@@ -1,10 +1,632 @@
 // Exact attention of one new token per sequence over its pages.
+//
+//   s_j = cap(scale q.k_j) + slope (j - (n - 1)),  o = sum_j 2^(s_j - m) v_j / sum_j 2^(s_j - m)
+//
+// Each key and value is read once and used for the query heads of its group
+// only, so the kernel is bound by HBM; the tensor cores (mma.sync m16n8k16)
+// keep the arithmetic out of the way at any group size.  Keys are the rows of
+// the products: S^T = K Q^T (16 keys x 8 heads) and O^T = V^T P^T (16 columns
+// x 8 heads), so a group of up to 8 heads fills a tile and P moves from the
+// first product to the second in registers (one 8x8 transpose per 8 keys).
+//
+// Work is cut into tiles of 4 warps x KW keys.  All tiles of the batch form
+// one sequence of which every CTA of one resident wave takes an equal run
+// (lengths are read on the device, so ragged batches balance without the
+// host); a unit (sequence, kv head, 16 heads) that is split over CTAs leaves
+// partial states in the workspace, which a small dependent launch joins in a
+// fixed order.  Each warp streams its own keys through a private ring of
+// cp.async stages (16-byte copies, page id looked up one tile ahead): no CTA
+// barrier until a unit ends.  Slots of a page beyond the sequence are filled
+// with zeros by the copy and masked, so their contents have no effect.
 #include "oc_attn_row.cuh"
+#include "oc_ptx.cuh"
 
 namespace {
 
 using namespace oc;
 
+constexpr int kWarps = 4;
+constexpr int kStages = 3;
+constexpr int kMinShare = 4;    // tiles that a CTA takes at least before a unit is split
+constexpr int kDirectTiles = 8; // units of at most so many tiles get a CTA each and no joining launch
+
+// ------------------------------------------------------------------ tile shape
+template <int ES, int DP>
+struct Shape {
+  // 16-key groups of one warp tile: 4 KB of keys, and K + V of at least 16 heads' partial output
+  static constexpr int KT = (4096 / (16 * DP * ES)) > (2 / ES) ? (4096 / (16 * DP * ES)) : (2 / ES);
+  static constexpr int KW = 16 * KT;                // keys of a warp tile
+  static constexpr int CT = kWarps * KW;            // keys of a CTA tile
+  static constexpr int ROW = DP * ES;               // bytes of a row
+  static constexpr int CH = ROW / 16;               // 16-byte chunks of a row
+  static constexpr int HALF = KW * ROW;             // bytes of a K (or V) tile
+  static constexpr int SLOT = 2 * HALF;
+  static constexpr int SMEM = kWarps * kStages * SLOT;
+  static constexpr int PER_SM = 227 * 1024 / (SMEM + 2048);  // resident CTAs
+  // XOR of a row's chunk index that spreads 8 rows of ldmatrix over all banks
+  static __device__ __forceinline__ int swz(int row) { return CH >= 8 ? row & 7 : (row >> 1) & (CH - 1); }
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+  if constexpr (BF16) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  } else {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+}
+__device__ __forceinline__ uint32_t fp8x2_to_half2(uint32_t two) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(two & 0xffffu), __NV_E4M3);
+  return (uint32_t)h.x | ((uint32_t)h.y << 16);
+}
+
+// Visible keys [lo, n) of a sequence.
+struct Span {
+  int lo, n;
+};
+__device__ __forceinline__ Span span_of(const oc_paged_decode_args& a, int seq) {
+  int n = a.seq_lens[seq];
+  const int64_t room = (int64_t)a.max_blocks * a.block_size;
+  if (n < 0 || n > room) {
+    raise_status(a.status, OC_STATUS_POSITION);
+    n = n < 0 ? 0 : (int)room;
+  }
+  return Span{a.window > 0 && n > a.window ? n - a.window : 0, n};
+}
+template <int CT>
+__device__ __forceinline__ int tiles_of(Span s) {
+  const int t = (s.n - s.lo + CT - 1) / CT;
+  return t < 1 ? 1 : t;  // an empty sequence still has an output to write
+}
+
+// Exclusive prefix sum over the CTA's kWarps * 32 threads.
+__device__ __forceinline__ int scan128(int v, int& total, int* part) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  int x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();
+  if (lane == 31) part[w] = x;
+  __syncthreads();
+  int before = 0;
+  total = 0;
+#pragma unroll
+  for (int i = 0; i < kWarps; ++i) {
+    before += i < w ? part[i] : 0;
+    total += part[i];
+  }
+  return before + x - v;
+}
+
+// Walks the tiles of the batch in order: sequence, then unit, then tile.
+template <int CT>
+struct Walk {
+  int seq, sub, tile, tiles;
+  Span span;
+  __device__ __forceinline__ void enter(const oc_paged_decode_args& a) {
+    span = span_of(a, seq);
+    tiles = tiles_of<CT>(span);
+  }
+  __device__ __forceinline__ void next(const oc_paged_decode_args& a, int subs) {
+    if (++tile < tiles) return;
+    tile = 0;
+    if (++sub < subs) return;
+    sub = 0;
+    if (++seq < a.num_seqs) enter(a);
+  }
+};
+
+// Workspace: header (tiles before each sequence, and in all, then the run
+// length), then per CTA two states of 8 NT heads: acc, m, l.
+struct Space {
+  int32_t* before;  // num_seqs + 1, then the run length
+  float* states;
+  __host__ __device__ static size_t header(int num_seqs) { return (((size_t)num_seqs + 2) * 4 + 15) / 16 * 16; }
+  __host__ __device__ Space(void* p, int num_seqs)
+      : before(static_cast<int32_t*>(p)), states(reinterpret_cast<float*>(static_cast<char*>(p) + header(num_seqs))) {}
+};
+__host__ __device__ constexpr int state_floats(int heads, int dp) { return heads * (dp + 2); }
+
+template <typename T, typename C, int DP, int NT, bool DIRECT>
+__global__ void __launch_bounds__(kWarps * 32, Shape<sizeof(C), DP>::PER_SM) decode_kernel(const __grid_constant__ oc_paged_decode_args a) {
+  using S = Shape<sizeof(C), DP>;
+  constexpr bool F8 = sizeof(C) == 1;
+  constexpr bool BF16 = !F8 && std::is_same<T, __nv_bfloat16>::value;  // 8-bit caches multiply in float16
+  constexpr int HT = 8 * NT;
+  constexpr int KS = DP / 16;  // steps of 16 columns
+  extern __shared__ __align__(128) char ring[];
+  __shared__ int part[kWarps];
+  __shared__ int found[3];  // sequence, unit, tile
+  __shared__ float stat[kWarps][HT][2];
+
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int gtiles = (a.group + HT - 1) / HT, subs = a.kv_heads * gtiles;
+  pdl_launch_dependents();
+  pdl_wait();
+
+  // ---------------------------------------------------------------- this CTA's run of tiles
+  Walk<S::CT> cs;
+  int count;
+  int64_t start = 0;
+  if constexpr (DIRECT) {
+    cs.seq = blockIdx.x / subs;
+    cs.sub = blockIdx.x - cs.seq * subs;
+    cs.tile = 0;
+    cs.enter(a);
+    count = cs.tiles;
+  } else {
+    const Space ws(a.workspace, a.num_seqs);
+    int mine = 0, own = 0;  // own: tiles of sequence threadIdx.x
+    for (int s = threadIdx.x; s < a.num_seqs; s += kWarps * 32) {
+      const int n = tiles_of<S::CT>(span_of(a, s)) * subs;
+      if (s == (int)threadIdx.x) own = n;
+      mine += n;
+    }
+    int total;
+    scan128(mine, total, part);
+    int share = (total + gridDim.x - 1) / gridDim.x;
+    share = share < kMinShare ? kMinShare : share;
+    start = (int64_t)blockIdx.x * share;
+    count = start < total ? (int)min((int64_t)share, total - start) : 0;
+    if (count == 0 && blockIdx.x != 0) return;
+    // the sequence that holds tile `start` (CTA 0 also leaves the prefix sums for the joining launch)
+    int base = 0;
+    for (int s0 = 0; s0 < a.num_seqs; s0 += kWarps * 32) {
+      const int s = s0 + threadIdx.x;
+      const int n = s >= a.num_seqs ? 0 : s0 == 0 ? own : tiles_of<S::CT>(span_of(a, s)) * subs;
+      int sum;
+      const int at = base + scan128(n, sum, part);
+      if (s < a.num_seqs && start >= at && start < at + n) {
+        found[0] = s;
+        found[1] = (int)(start - at) / (n / subs);
+        found[2] = (int)(start - at) % (n / subs);
+      }
+      if (blockIdx.x == 0 && s < a.num_seqs) ws.before[s] = at;
+      base += sum;
+      if (blockIdx.x != 0 && start < base) break;
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+      ws.before[a.num_seqs] = total;
+      ws.before[a.num_seqs + 1] = share;
+    }
+    __syncthreads();
+    cs.seq = found[0];
+    cs.sub = found[1];
+    cs.tile = found[2];
+    cs.enter(a);
+  }
+
+  // ---------------------------------------------------------------- the copy stream of this warp
+  const uint32_t my_ring = smem_u32(ring) + warp * kStages * S::SLOT;
+  const int chunks = a.head_dim * (int)sizeof(C) / 16, block_shift = __ffs(a.block_size) - 1;
+  Walk<S::CT> ld = cs;
+  int ld_left = count;
+  struct Pending {
+    int page[(S::KW + 31) / 32];  // of key key0 + lane (+ 32); -1: zeros
+    int key0, hk;
+  } pend;
+  // looks up the pages of the next tile
+  auto look = [&](Pending& p) {
+    p.key0 = 0;
+    p.hk = 0;
+#pragma unroll
+    for (int i = 0; i < (S::KW + 31) / 32; ++i) p.page[i] = -1;
+    if (ld_left <= 0) return;
+    p.key0 = ld.span.lo + ld.tile * S::CT + warp * S::KW;
+    p.hk = ld.sub / gtiles;
+    const int32_t* table = a.block_tables + (int64_t)ld.seq * a.block_table_stride;
+#pragma unroll
+    for (int i = 0; i < (S::KW + 31) / 32; ++i) {
+      const int j = p.key0 + lane + 32 * i;
+      if (lane + 32 * i < S::KW && j < ld.span.n) {
+        const int page = table[j >> block_shift];
+        if (page >= 0 && page < a.num_blocks) p.page[i] = page;
+        else raise_status(a.status, OC_STATUS_BAD_PAGE);
+      }
+    }
+    --ld_left;
+    if (ld_left > 0) ld.next(a, subs);
+  };
+  auto issue = [&](const Pending& p, int stage) {
+    const uint32_t kd = my_ring + stage * S::SLOT, vd = kd + S::HALF;
+    const char* kb = static_cast<const char*>(a.k_cache) + (int64_t)p.hk * a.kc_head_stride * sizeof(C);
+    const char* vb = static_cast<const char*>(a.v_cache) + (int64_t)p.hk * a.vc_head_stride * sizeof(C);
+#pragma unroll
+    for (int i = 0; i < S::KW * S::CH / 32; ++i) {
+      const int idx = i * 32 + lane, row = idx / S::CH, ch = idx % S::CH;
+      const int page = __shfl_sync(0xffffffffu, p.page[row / 32], row & 31);
+      const int slot = (p.key0 + row) & (a.block_size - 1);
+      const bool on = page >= 0 && ch < chunks;
+      const int64_t ko = on ? ((int64_t)page * a.kc_block_stride + (int64_t)slot * a.kc_tok_stride) * sizeof(C) + ch * 16 : 0;
+      const int64_t vo = on ? ((int64_t)page * a.vc_block_stride + (int64_t)slot * a.vc_tok_stride) * sizeof(C) + ch * 16 : 0;
+      const uint32_t at = row * S::ROW + ((ch ^ S::swz(row)) << 4);
+      cp_async16(kd + at, kb + ko, on ? 16 : 0);
+      cp_async16(vd + at, vb + vo, on ? 16 : 0);
+    }
+  };
+  {
+    Pending first[kStages];
+#pragma unroll
+    for (int s = 0; s < kStages; ++s) look(first[s]);
+#pragma unroll
+    for (int s = 0; s < kStages - 1; ++s) {
+      issue(first[s], s);
+      cp_commit();
+    }
+    pend = first[kStages - 1];
+  }
+
+  // ---------------------------------------------------------------- the unit's state
+  uint32_t qf[KS][NT][2];
+  float acc[KS][NT][4], m[NT][2], mu[NT][2], l[NT][2], sc[NT][2], slope[NT][2];
+  const float inv_cap = a.softcap > 0.f ? 1.f / a.softcap : 0.f;
+
+  auto begin_unit = [&]() {
+    const int hk = cs.sub / gtiles, h0 = hk * a.group + (cs.sub % gtiles) * HT;
+    const int heads = min(HT, a.group - (cs.sub % gtiles) * HT);
+    float qscale[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int hr = n * 8 + g;
+      const T* q = static_cast<const T*>(a.q) + (int64_t)cs.seq * a.q_seq_stride + (int64_t)(h0 + hr) * a.q_head_stride;
+      auto at = [&](int d) { return hr < heads && d < a.head_dim ? to_f32(q[d]) : 0.f; };
+      qscale[n] = 1.f;
+      if constexpr (F8 && std::is_same<T, __nv_bfloat16>::value) {
+        // bfloat16 queries go through float16 times a power of two that puts their largest below 2^8
+        float top = 0.f;
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(at(k * 16 + 4 * t + e)));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        if (top > 0.f && top < INFINITY) {
+          int e = 7 - ilogbf(top);
+          e = e > 120 ? 120 : e;
+          qscale[n] = exp2f((float)e);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        if constexpr (F8) {  // column order of the converted keys: 4t, 4t + 1 | 4t + 2, 4t + 3
+          const int d = k * 16 + 4 * t;
+          qf[k][n][0] = pack16<BF16>(at(d) * qscale[n], at(d + 1) * qscale[n]);
+          qf[k][n][1] = pack16<BF16>(at(d + 2) * qscale[n], at(d + 3) * qscale[n]);
+        } else {
+          const int d = k * 16 + 2 * t;
+          qf[k][n][0] = pack16<BF16>(at(d), at(d + 1));
+          qf[k][n][1] = pack16<BF16>(at(d + 8), at(d + 9));
+        }
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int hr = n * 8 + 2 * t + c;
+        const float qs = __shfl_sync(0xffffffffu, qscale[n], (2 * t + c) * 4);
+        sc[n][c] = a.scale * a.k_scale / qs;
+        slope[n][c] = a.slopes && hr < heads ? a.slopes[h0 + hr] * kLog2e : 0.f;
+        m[n][c] = -INFINITY;
+        mu[n][c] = 0.f;
+        l[n][c] = 0.f;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) acc[k][n][c] = acc[k][n][c + 2] = 0.f;
+      }
+  };
+
+  // ---------------------------------------------------------------- one warp tile
+  auto compute = [&](int stage) {
+    const uint32_t kd = my_ring + stage * S::SLOT, vd = kd + S::HALF;
+    const int key0 = cs.span.lo + cs.tile * S::CT + warp * S::KW;
+    if (key0 >= cs.span.n) return;
+    float s[S::KT][NT][4];
+#pragma unroll
+    for (int kt = 0; kt < S::KT; ++kt) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) s[kt][n][c] = 0.f;
+      const int row = kt * 16 + (lane & 15);
+      const uint32_t base = kd + row * S::ROW;
+      const int x = S::swz(row);
+      if constexpr (F8) {
+#pragma unroll
+        for (int k = 0; k < KS; k += 2) {
+          uint32_t r[4];
+          ldsm_x4(base + (((k + (lane >> 4)) ^ x) << 4), r);
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const uint32_t f[4] = {fp8x2_to_half2(r[2 * u]), fp8x2_to_half2(r[2 * u + 1]),
+                                   fp8x2_to_half2(r[2 * u] >> 16), fp8x2_to_half2(r[2 * u + 1] >> 16)};
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma16816<BF16>(s[kt][n], f, qf[k + u][n][0], qf[k + u][n][1]);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          uint32_t r[4];
+          ldsm_x4(base + (((2 * k + (lane >> 4)) ^ x) << 4), r);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma16816<BF16>(s[kt][n], r, qf[k][n][0], qf[k][n][1]);
+        }
+      }
+    }
+    // scores in log2 units; the mask on the last tile only (tiles start at the first visible key)
+    const bool whole = key0 + S::KW <= cs.span.n;
+    bool grow = false;
+#pragma unroll
+    for (int kt = 0; kt < S::KT; ++kt)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int j = key0 + kt * 16 + g + (c >> 1) * 8;
+          float x = s[kt][n][c] * sc[n][c & 1];
+          if (a.softcap > 0.f) x = a.softcap * tanhf(x * inv_cap);
+          x = fmaf(slope[n][c & 1], (float)(j - (cs.span.n - 1)), x * kLog2e);
+          if (!whole && j >= cs.span.n) x = -INFINITY;
+          s[kt][n][c] = x;
+          grow |= x > m[n][c & 1] + 8.f;
+        }
+    // The maximum moves only when a score exceeds it by 2^8 (sums stay in float32, p below 2^8 in 16
+    // bits loses nothing): most tiles skip the reduction and the rescaling.
+    if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float top = m[n][c];
+#pragma unroll
+          for (int kt = 0; kt < S::KT; ++kt) top = fmaxf(top, fmaxf(s[kt][n][c], s[kt][n][c + 2]));
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+          const float back = m[n][c] == -INFINITY ? 0.f : exp2f(m[n][c] - top);
+          m[n][c] = top;
+          mu[n][c] = top == -INFINITY ? 0.f : top;
+          l[n][c] *= back;
+#pragma unroll
+          for (int k = 0; k < KS; ++k) {
+            acc[k][n][c] *= back;
+            acc[k][n][c + 2] *= back;
+          }
+        }
+    }
+#pragma unroll
+    for (int kt = 0; kt < S::KT; ++kt) {
+      uint32_t p[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float e[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          e[c] = ex2(s[kt][n][c] - mu[n][c & 1]);
+          l[n][c & 1] += e[c];
+        }
+        p[n][0] = transpose8x8(pack16<BF16>(e[0], e[1]));
+        p[n][1] = transpose8x8(pack16<BF16>(e[2], e[3]));
+      }
+      const int row = kt * 16 + (lane & 7) + ((lane >> 4) << 3);
+      const uint32_t base = vd + row * S::ROW;
+      const int x = S::swz(row);
+      if constexpr (F8) {
+        // matrices: keys 0-7 and 8-15 of one 16-column chunk, then of the next
+        const int row8 = kt * 16 + (lane & 15);
+        const uint32_t base8 = vd + row8 * S::ROW;
+#pragma unroll
+        for (int k = 0; k < KS; k += 2) {
+          uint32_t r[4];
+          ldsm_x4_t(base8 + (((k + (lane >> 4)) ^ S::swz(row8)) << 4), r);
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const uint32_t r0 = r[2 * u], r1 = r[2 * u + 1];
+            const uint32_t f[4] = {fp8x2_to_half2(__byte_perm(r0, 0, 0x4420)), fp8x2_to_half2(__byte_perm(r0, 0, 0x4431)),
+                                   fp8x2_to_half2(__byte_perm(r1, 0, 0x4420)), fp8x2_to_half2(__byte_perm(r1, 0, 0x4431))};
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma16816<BF16>(acc[k + u][n], f, p[n][0], p[n][1]);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          uint32_t r[4];
+          ldsm_x4_t(base + (((2 * k + ((lane >> 3) & 1)) ^ x) << 4), r);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma16816<BF16>(acc[k][n], r, p[n][0], p[n][1]);
+        }
+      }
+    }
+  };
+
+  // ---------------------------------------------------------------- end of a unit (or of the CTA's part of it)
+  // Each warp's state goes through the ring slot that it has just consumed.
+  auto end_unit = [&](int stage, bool complete, int slot) {
+    float* mine = reinterpret_cast<float*>(ring + warp * kStages * S::SLOT + stage * S::SLOT);
+    __syncwarp();
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float sum = l[n][c];
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        const int hr = n * 8 + 2 * t + c;
+        if (g == 0) {
+          stat[warp][hr][0] = m[n][c];
+          stat[warp][hr][1] = sum;
+        }
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {  // columns are XORed by the head so that the four lanes of a row spread over banks
+          const int d0 = F8 ? k * 16 + 2 * g : k * 16 + g, d1 = F8 ? d0 + 1 : d0 + 8;
+          mine[hr * DP + (d0 ^ (t << 3))] = acc[k][n][c];
+          mine[hr * DP + (d1 ^ (t << 3))] = acc[k][n][c + 2];
+        }
+      }
+    __syncthreads();
+    const int hk = cs.sub / gtiles, h0 = hk * a.group + (cs.sub % gtiles) * HT;
+    const int heads = min(HT, a.group - (cs.sub % gtiles) * HT);
+    // a warp per head
+    for (int hr = warp; hr < heads; hr += kWarps) {
+      float top = -INFINITY, sum = 0.f, f[kWarps];
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) top = fmaxf(top, stat[w][hr][0]);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        // a maximum of -inf with a sum that is not 0 is a NaN score: it stays
+        f[w] = stat[w][hr][0] == -INFINITY ? (stat[w][hr][1] == 0.f ? 0.f : 1.f) : exp2f(stat[w][hr][0] - top);
+        sum += stat[w][hr][1] * f[w];
+      }
+      const int swz = ((hr >> 1) & 3) << 3;
+      const float inv = sum == 0.f ? 0.f : a.v_scale / sum;
+      float* state = nullptr;
+      if constexpr (!DIRECT)
+        state = Space(a.workspace, a.num_seqs).states + (int64_t)(2 * blockIdx.x + slot) * state_floats(HT, DP);
+      T* out = static_cast<T*>(a.out) + (int64_t)cs.seq * a.out_seq_stride + (int64_t)(h0 + hr) * a.out_head_stride;
+#pragma unroll
+      for (int i = 0; i < DP / 32; ++i) {
+        const int d = lane + 32 * i;
+        float x = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float* o = reinterpret_cast<const float*>(ring + w * kStages * S::SLOT + stage * S::SLOT);
+          x = fmaf(o[hr * DP + (d ^ swz)], f[w], x);
+        }
+        if (DIRECT || complete) {
+          if (d < a.head_dim) out[d] = from_f32<T>(x * inv);
+        } else {
+          state[hr * DP + d] = x;
+        }
+      }
+      if (lane == 0) {
+        if (DIRECT || complete) {
+          if (a.lse)
+            a.lse[(int64_t)cs.seq * a.kv_heads * a.group + h0 + hr] =
+                sum == 0.f ? -INFINITY : ((top == -INFINITY ? 0.f : top) + log2f(sum)) * kLn2;
+        } else {
+          state[HT * DP + 2 * hr] = top;
+          state[HT * DP + 2 * hr + 1] = sum;
+        }
+      }
+    }
+    __syncthreads();
+  };
+
+  // ---------------------------------------------------------------- main loop
+  begin_unit();
+  bool from_start = cs.tile == 0;  // this CTA has the unit from its first tile
+  int stage = 0, ahead = kStages - 1;
+  for (int i = 0; i < count; ++i) {
+    cp_wait<kStages - 2>();
+    __syncwarp();
+    compute(stage);
+    __syncwarp();
+    const bool last_tile = cs.tile + 1 == cs.tiles;
+    if (last_tile || i + 1 == count) {
+      const bool complete = from_start && last_tile;
+      // a CTA leaves at most two partial states: of a unit begun by others, and of one that it began
+      end_unit(stage, complete, from_start ? 1 : 0);
+    }
+    // the slot consumed before this one is free in every case: refill
+    issue(pend, ahead);
+    cp_commit();
+    look(pend);
+    stage = stage + 1 == kStages ? 0 : stage + 1;
+    ahead = ahead + 1 == kStages ? 0 : ahead + 1;
+    if (i + 1 < count) {
+      cs.next(a, subs);
+      if (cs.tile == 0) {
+        begin_unit();
+        from_start = true;
+      }
+    }
+  }
+  cp_wait<0>();
+}
+
+// Joins the partial states of the units that were split: one CTA per
+// (unit, head), its warps take the parts in turn, and their sums are added in
+// a fixed order.
+template <typename T, int DP, int NT, int CT>
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ oc_paged_decode_args a) {
+  constexpr int HT = 8 * NT, W = 8;
+  __shared__ float sm[W][2];
+  __shared__ float so[W][DP];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int gtiles = (a.group + HT - 1) / HT, subs = a.kv_heads * gtiles;
+  const int h = blockIdx.x, seq = blockIdx.y, hk = h / a.group, hg = h - hk * a.group;
+  const int sub = hk * gtiles + hg / HT, hr = hg % HT;
+  const Space ws(a.workspace, a.num_seqs);
+  const int before = ws.before[seq], tiles = (ws.before[seq + 1] - before) / subs, share = ws.before[a.num_seqs + 1];
+  const int t0 = before + sub * tiles, t1 = t0 + tiles, c0 = t0 / share, c1 = (t1 - 1) / share;
+  if (c0 == c1) return;  // one CTA had it all and wrote the output
+  auto state = [&](int c) {
+    // the unit is the CTA's first unless it starts inside the CTA's run
+    const int slot = t0 >= c * share ? 1 : 0;
+    return ws.states + (int64_t)(2 * c + slot) * state_floats(HT, DP);
+  };
+  float top = -INFINITY;
+  for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, state(c)[HT * DP + 2 * hr]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  float sum = 0.f, x[DP / 32];
+#pragma unroll
+  for (int i = 0; i < DP / 32; ++i) x[i] = 0.f;
+#pragma unroll 2
+  for (int c = c0 + warp; c <= c1; c += W) {
+    const float* s = state(c);
+    const float mc = s[HT * DP + 2 * hr], lc = s[HT * DP + 2 * hr + 1];
+    const float f = mc == -INFINITY ? (lc == 0.f ? 0.f : 1.f) : exp2f(mc - top);
+    sum = fmaf(lc, f, sum);
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i) x[i] = fmaf(s[hr * DP + lane + 32 * i], f, x[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < DP / 32; ++i) so[warp][lane + 32 * i] = x[i];
+  if (lane == 0) sm[warp][0] = sum;
+  __syncthreads();
+  float all = 0.f;
+#pragma unroll
+  for (int w = 0; w < W; ++w) all += sm[w][0];
+  const float inv = all == 0.f ? 0.f : a.v_scale / all;
+  T* out = static_cast<T*>(a.out) + (int64_t)seq * a.out_seq_stride + (int64_t)h * a.out_head_stride;
+  for (int d = threadIdx.x; d < a.head_dim; d += blockDim.x) {
+    float y = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) y += so[w][d];
+    out[d] = from_f32<T>(y * inv);
+  }
+  if (a.lse && threadIdx.x == 0)
+    a.lse[(int64_t)seq * a.kv_heads * a.group + h] =
+        all == 0.f ? -INFINITY : ((top == -INFINITY ? 0.f : top) + log2f(all)) * kLn2;
+}
+
+// ------------------------------------------------------------------ any type, any alignment
 // One warp per (sequence, query head).
 template <typename T, typename C>
 __global__ void __launch_bounds__(32) decode_row_kernel(const oc_paged_decode_args a) {
@@ -15,13 +637,7 @@ __global__ void __launch_bounds__(32) decode_row_kernel(const oc_paged_decode_ar
   const T* q = static_cast<const T*>(a.q) + seq * a.q_seq_stride + h * a.q_head_stride;
   for (int d = lane; d < a.head_dim; d += 32) qs[d] = to_f32(q[d]);
   __syncwarp();
-  int n = a.seq_lens[seq];
-  const int64_t room = (int64_t)a.max_blocks * a.block_size;
-  if (n < 0 || n > room) {
-    if (lane == 0) raise_status(a.status, OC_STATUS_POSITION);
-    n = n < 0 ? 0 : (int)room;
-  }
-  const int first = a.window > 0 && n > a.window ? n - a.window : 0;
+  const Span span = span_of(a, seq);
   const int32_t* table = a.block_tables + seq * a.block_table_stride;
   auto row = [&](const void* cache, int64_t bs, int64_t hs, int64_t ts, int j) -> const C* {
     const int64_t page = table[j / a.block_size];
@@ -33,11 +649,11 @@ __global__ void __launch_bounds__(32) decode_row_kernel(const oc_paged_decode_ar
   };
   T* out = static_cast<T*>(a.out) + seq * a.out_seq_stride + h * a.out_head_stride;
   const float lse = attend_row<C>(
-      qs, a.head_dim, RowScore{a.scale * a.k_scale, a.softcap, a.slopes ? a.slopes[h] : 0.f}, a.v_scale, first, n,
-      [](int) { return false; },
+      qs, a.head_dim, RowScore{a.scale * a.k_scale, a.softcap, a.slopes ? a.slopes[h] : 0.f}, a.v_scale, span.lo,
+      span.n, [](int) { return false; },
       [&](int j) { return row(a.k_cache, a.kc_block_stride, a.kc_head_stride, a.kc_tok_stride, j); },
       [&](int j) { return row(a.v_cache, a.vc_block_stride, a.vc_head_stride, a.vc_tok_stride, j); },
-      [&](int j) { return (float)(j - (n - 1)); }, [&](int d, float x) { out[d] = from_f32<T>(x); });
+      [&](int j) { return (float)(j - (span.n - 1)); }, [&](int d, float x) { out[d] = from_f32<T>(x); });
   if (a.lse && lane == 0) a.lse[(int64_t)seq * a.kv_heads * a.group + h] = lse;
 }
 
@@ -47,28 +663,126 @@ int launch_rows(const oc_paged_decode_args& a, void* stream) {
                     stream, a);
 }
 
+// ------------------------------------------------------------------ host side
+int padded(int head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
+
+// Tiles by 16-byte copies: 16-bit inputs, rows and pages at multiples of 16 bytes.
+bool tiled(const oc_paged_decode_args& a) {
+  if (a.dtype == OC_F32 || a.max_blocks == 0) return false;
+  const int es = type_bytes(a.cache_dtype);
+  auto ok = [&](int64_t s) { return (s * es) % 16 == 0; };
+  return a.head_dim * es % 16 == 0 && a.head_dim >= 16 && aligned_to(a.k_cache, 16) && aligned_to(a.v_cache, 16) &&
+         ok(a.kc_block_stride) && ok(a.kc_head_stride) && ok(a.kc_tok_stride) && ok(a.vc_block_stride) &&
+         ok(a.vc_head_stride) && ok(a.vc_tok_stride);
+}
+
+struct Plan {
+  bool direct;
+  int64_t grid;
+  int nt;
+};
+
+template <int ES, int DP>
+Plan plan_of(const oc_paged_decode_args& a) {
+  using S = Shape<ES, DP>;
+  Plan p;
+  p.nt = a.group <= 8 ? 1 : 2;
+  const int64_t gt = (a.group + 8 * p.nt - 1) / (8 * p.nt), units = a.num_seqs * (int64_t)a.kv_heads * gt;
+  int64_t most = (int64_t)a.max_blocks * a.block_size;
+  if (a.window > 0 && a.window < most) most = a.window;
+  p.direct = most <= (int64_t)S::CT * kDirectTiles;
+    const int64_t tiles = units * ((most + S::CT - 1) / S::CT), wave = (int64_t)a.num_sms * S::PER_SM;
+  const int64_t useful = (tiles + kMinShare - 1) / kMinShare;
+  p.grid = p.direct ? units : useful < wave ? useful : wave;
+  return p;
+}
+
+template <typename F>
+auto by_shape(const oc_paged_decode_args& a, F f) {
+  const int dp = padded(a.head_dim);
+  if (a.cache_dtype == OC_F8E4M3) {
+    if (dp == 64) return f(std::integral_constant<int, 1>(), std::integral_constant<int, 64>());
+    if (dp == 128) return f(std::integral_constant<int, 1>(), std::integral_constant<int, 128>());
+    return f(std::integral_constant<int, 1>(), std::integral_constant<int, 256>());
+  }
+  if (dp == 64) return f(std::integral_constant<int, 2>(), std::integral_constant<int, 64>());
+  if (dp == 128) return f(std::integral_constant<int, 2>(), std::integral_constant<int, 128>());
+  return f(std::integral_constant<int, 2>(), std::integral_constant<int, 256>());
+}
+
+template <typename T, typename C, int DP, int NT>
+int launch_tiled(const oc_paged_decode_args& a, const Plan& p, void* stream) {
+  using S = Shape<sizeof(C), DP>;
+  auto kernel = p.direct ? decode_kernel<T, C, DP, NT, true> : decode_kernel<T, C, DP, NT, false>;
+  if (S::SMEM > 48 * 1024 &&
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM) != cudaSuccess) {
+    cudaGetLastError();
+    return OC_ERR_CUDA;
+  }
+  int rc = launch_pdl(kernel, dim3((unsigned)p.grid), dim3(kWarps * 32), S::SMEM, stream, a);
+  if (rc != OC_OK || p.direct) return rc;
+  return launch_pdl(join_kernel<T, DP, NT, S::CT>, dim3((unsigned)(a.kv_heads * a.group), (unsigned)a.num_seqs),
+                    dim3(256), 0, stream, a);
+}
+
+template <typename T, typename C, int DP>
+int launch_nt(const oc_paged_decode_args& a, void* stream) {
+  const Plan p = plan_of<sizeof(C), DP>(a);
+  if (p.grid > 0x7fffffff) return OC_ERR_TOO_LARGE;
+  return p.nt == 1 ? launch_tiled<T, C, DP, 1>(a, p, stream) : launch_tiled<T, C, DP, 2>(a, p, stream);
+}
+
+template <typename T, typename C>
+int launch_type(const oc_paged_decode_args& a, void* stream) {
+  switch (padded(a.head_dim)) {
+    case 64: return launch_nt<T, C, 64>(a, stream);
+    case 128: return launch_nt<T, C, 128>(a, stream);
+    default: return launch_nt<T, C, 256>(a, stream);
+  }
+}
+
+int invalid(const oc_paged_decode_args& a) {
+  if (a.num_seqs < 0 || a.kv_heads < 1 || a.group < 1 || a.head_dim < 1 || a.block_size < 1 ||
+      (a.block_size & (a.block_size - 1)) || a.max_blocks < 0 || a.window < 0 || a.num_sms < 1 || a.num_blocks < 0 ||
+      !(a.softcap >= 0.f))
+    return OC_ERR_INVALID;
+  if (a.head_dim > kRowMaxDim) return OC_ERR_UNSUPPORTED;
+  if (a.cache_dtype != a.dtype && a.cache_dtype != OC_F8E4M3) return OC_ERR_UNSUPPORTED;
+  if (a.dtype != OC_F32 && a.dtype != OC_F16 && a.dtype != OC_BF16) return OC_ERR_UNSUPPORTED;
+  if (a.num_seqs > 65535 || (int64_t)a.max_blocks * a.block_size > 0x7fffff00) return OC_ERR_TOO_LARGE;
+  return OC_OK;
+}
+
 }  // namespace
 
-extern "C" size_t oc_paged_decode_workspace_bytes(const oc_paged_decode_args*) { return 0; }
+extern "C" size_t oc_paged_decode_workspace_bytes(const oc_paged_decode_args* a) {
+  if (!a || invalid(*a) != OC_OK || a->num_seqs == 0 || !tiled(*a)) return 0;
+  return by_shape(*a, [&](auto es, auto dp) -> size_t {
+    const Plan p = plan_of<es(), dp()>(*a);
+    if (p.direct) return 0;
+    return Space::header(a->num_seqs) + (size_t)p.grid * 2 * state_floats(8 * p.nt, dp()) * sizeof(float);
+  });
+}
 
 extern "C" int oc_paged_decode_attention(const oc_paged_decode_args* args, void* stream) {
   if (!args) return OC_ERR_INVALID;
   const oc_paged_decode_args& a = *args;
-  if (a.num_seqs < 0 || a.kv_heads < 1 || a.group < 1 || a.head_dim < 1 || a.block_size < 1 || a.max_blocks < 0 ||
-      a.window < 0 || a.num_sms < 1 || a.num_blocks < 0 || !(a.softcap >= 0.f))
-    return OC_ERR_INVALID;
+  const int bad = invalid(a);
+  if (bad != OC_OK) return bad;
   if (a.num_seqs == 0) return OC_OK;
   if (!a.q || !a.out || !a.seq_lens || (a.max_blocks && (!a.block_tables || !a.k_cache || !a.v_cache)))
     return OC_ERR_INVALID;
-  if (a.head_dim > kRowMaxDim) return OC_ERR_UNSUPPORTED;
-  if (a.num_seqs > 65535) return OC_ERR_TOO_LARGE;
-  if (a.cache_dtype != a.dtype && a.cache_dtype != OC_F8E4M3) return OC_ERR_UNSUPPORTED;
   const bool f8 = a.cache_dtype == OC_F8E4M3;
+  if (tiled(a)) {
+    const size_t need = oc_paged_decode_workspace_bytes(&a);
+    if (need && (!a.workspace || !aligned_to(a.workspace, 16) || a.workspace_bytes < need)) return OC_ERR_WORKSPACE;
+    if (a.dtype == OC_F16) return f8 ? launch_type<__half, fp8_t>(a, stream) : launch_type<__half, __half>(a, stream);
+    return f8 ? launch_type<__nv_bfloat16, fp8_t>(a, stream) : launch_type<__nv_bfloat16, __nv_bfloat16>(a, stream);
+  }
   switch (a.dtype) {
     case OC_F32: return f8 ? launch_rows<float, fp8_t>(a, stream) : launch_rows<float, float>(a, stream);
     case OC_F16: return f8 ? launch_rows<__half, fp8_t>(a, stream) : launch_rows<__half, __half>(a, stream);
-    case OC_BF16:
+    default:
       return f8 ? launch_rows<__nv_bfloat16, fp8_t>(a, stream) : launch_rows<__nv_bfloat16, __nv_bfloat16>(a, stream);
-    default: return OC_ERR_UNSUPPORTED;
   }
 }
