@@ -14,10 +14,19 @@
 // (lengths are read on the device, so ragged batches balance without the
 // host); a unit (sequence, kv head, 16 heads) that is split over CTAs leaves
 // partial states in the workspace, which a small dependent launch joins in a
-// fixed order.  Each warp streams its own keys through a private ring of
-// cp.async stages (16-byte copies, page id looked up one tile ahead): no CTA
-// barrier until a unit ends.  Slots of a page beyond the sequence are filled
-// with zeros by the copy and masked, so their contents have no effect.
+// fixed order.  Each warp streams its own keys and values through a private
+// ring of three 4 KB buffers (K, V, K, ...) that tiled TMA copies fill, a
+// 128-byte-swizzled box per page and 128 bytes of columns, the page id looked
+// up two tiles ahead: no CTA barrier until a unit ends, and 16 warps per SM to
+// cover the latency of one another's products.  Values in slots that are not
+// visible are zeroed in shared memory before use and their scores masked, so
+// their contents have no effect.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <mutex>
+#include <utility>
+
 #include "oc_attn_row.cuh"
 #include "oc_ptx.cuh"
 
@@ -26,35 +35,35 @@ namespace {
 using namespace oc;
 
 constexpr int kWarps = 4;
-constexpr int kStages = 3;
-constexpr int kMinShare = 4;    // tiles that a CTA takes at least before a unit is split
-constexpr int kDirectTiles = 8; // units of at most so many tiles get a CTA each and no joining launch
+constexpr int kBufs = 3;         // buffers of a warp's ring
+constexpr int kMinShare = 4;     // tiles that a CTA takes at least before a unit is split
+constexpr int kDirectTiles = 8;  // units of at most so many tiles get a CTA each and no joining launch
+constexpr uint32_t kPolls = 1u << 22;  // bound of a wait for a copy
 
 // ------------------------------------------------------------------ tile shape
-template <int ES, int DP>
+template <int ES, int DP, int NT>
 struct Shape {
-  // 16-key groups of one warp tile: 4 KB of keys, and K + V of at least 16 heads' partial output
-  static constexpr int KT = (4096 / (16 * DP * ES)) > (2 / ES) ? (4096 / (16 * DP * ES)) : (2 / ES);
-  static constexpr int KW = 16 * KT;                // keys of a warp tile
-  static constexpr int CT = kWarps * KW;            // keys of a CTA tile
-  static constexpr int ROW = DP * ES;               // bytes of a row
-  static constexpr int CH = ROW / 16;               // 16-byte chunks of a row
-  static constexpr int HALF = KW * ROW;             // bytes of a K (or V) tile
-  static constexpr int SLOT = 2 * HALF;
-  static constexpr int SMEM = kWarps * kStages * SLOT;
-  static constexpr int PER_SM = 227 * 1024 / (SMEM + 2048);  // resident CTAs
-  // XOR of a row's chunk index that spreads 8 rows of ldmatrix over all banks
-  static __device__ __forceinline__ int swz(int row) { return CH >= 8 ? row & 7 : (row >> 1) & (CH - 1); }
+  static constexpr int ROW = DP * ES;                       // bytes of a row
+  // 16-key groups of a warp tile: 4 KB of keys or more, and room for 8 heads' output
+  static constexpr int KT = 16 * ROW < 4096 ? 4096 / (16 * ROW) : ES == 1 ? 2 : 1;
+  static constexpr int KW = 16 * KT;                        // keys of a warp tile
+  static constexpr int CT = kWarps * KW;                    // keys of a CTA tile
+  static constexpr int BUF = KW * ROW;                      // bytes of a K (or V) tile, and of 8 heads' output at most
+  static constexpr int PANEL = ROW < 128 ? ROW : 128;       // bytes of columns that one box brings
+  static constexpr int PANELS = ROW / PANEL;
+  static_assert(PANEL == 128 || PANEL == 64, "one of the copy engine's swizzles");
+  static constexpr int SMEM = kWarps * kBufs * BUF + 1024;  // + alignment of the swizzle pattern
+  static constexpr int PER_SM = DP == 256 || NT == 2 ? 2 : 4;  // resident CTAs, by registers (and shared memory)
+  static_assert(BUF >= 8 * DP * 4, "a buffer holds 8 heads' partial output");
+  // Byte offset of 16-byte chunk ch of row r: panels of KW rows.  The swizzle is as wide as a panel: with a
+  // wider one the copy engine pads every row to the swizzle's width.
+  static __device__ __forceinline__ uint32_t at(int r, int ch) {
+    constexpr int PC = PANEL / 16;
+    const uint32_t lin = (uint32_t)(r * PANEL + (ch % PC) * 16);
+    return (uint32_t)(ch / PC) * (KW * PANEL) + (lin ^ ((lin >> 3) & (PANEL == 128 ? 0x70 : 0x30)));
+  }
 };
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -75,12 +84,19 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&v);
   }
 }
+// Two 8-bit values (the low half of `two`) as two float16.
 __device__ __forceinline__ uint32_t fp8x2_to_half2(uint32_t two) {
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(two & 0xffffu), __NV_E4M3);
-  return (uint32_t)h.x | ((uint32_t)h.y << 16);
+  uint32_t h;
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(h) : "r"(two));
+  return h;
+}
+__device__ __forceinline__ uint32_t fp8x2_to_half2_hi(uint32_t two) {
+  uint32_t h;
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, hi;\n\t}" : "=r"(h) : "r"(two));
+  return h;
 }
 
-// Visible keys [lo, n) of a sequence.
+// Visible keys [lo, n) of a sequence; its tiles start at base, a multiple of KW.
 struct Span {
   int lo, n;
 };
@@ -93,9 +109,9 @@ __device__ __forceinline__ Span span_of(const oc_paged_decode_args& a, int seq) 
   }
   return Span{a.window > 0 && n > a.window ? n - a.window : 0, n};
 }
-template <int CT>
+template <typename S>
 __device__ __forceinline__ int tiles_of(Span s) {
-  const int t = (s.n - s.lo + CT - 1) / CT;
+  const int t = (s.n - (s.lo & -S::KW) + S::CT - 1) / S::CT;
   return t < 1 ? 1 : t;  // an empty sequence still has an output to write
 }
 
@@ -122,13 +138,13 @@ __device__ __forceinline__ int scan128(int v, int& total, int* part) {
 }
 
 // Walks the tiles of the batch in order: sequence, then unit, then tile.
-template <int CT>
+template <typename S>
 struct Walk {
   int seq, sub, tile, tiles;
   Span span;
   __device__ __forceinline__ void enter(const oc_paged_decode_args& a) {
     span = span_of(a, seq);
-    tiles = tiles_of<CT>(span);
+    tiles = tiles_of<S>(span);
   }
   __device__ __forceinline__ void next(const oc_paged_decode_args& a, int subs) {
     if (++tile < tiles) return;
@@ -150,25 +166,44 @@ struct Space {
 };
 __host__ __device__ constexpr int state_floats(int heads, int dp) { return heads * (dp + 2); }
 
+// A cache as the copy engine sees it: dimension 0 is a row's columns, the
+// others (slot, kv head, page) are ordered by their strides; role[i] says
+// which of them (0, 1, 2) dimension i + 1 is.
+struct Maps {
+  CUtensorMap k, v;
+  int k_role[3], v_role[3];
+};
+
 template <typename T, typename C, int DP, int NT, bool DIRECT>
-__global__ void __launch_bounds__(kWarps * 32, Shape<sizeof(C), DP>::PER_SM) decode_kernel(const __grid_constant__ oc_paged_decode_args a) {
-  using S = Shape<sizeof(C), DP>;
+__global__ void __launch_bounds__(kWarps * 32, Shape<sizeof(C), DP, NT>::PER_SM)
+    decode_kernel(const __grid_constant__ oc_paged_decode_args a, const __grid_constant__ Maps maps) {
+  using S = Shape<sizeof(C), DP, NT>;
   constexpr bool F8 = sizeof(C) == 1;
   constexpr bool BF16 = !F8 && std::is_same<T, __nv_bfloat16>::value;  // 8-bit caches multiply in float16
   constexpr int HT = 8 * NT;
   constexpr int KS = DP / 16;  // steps of 16 columns
-  extern __shared__ __align__(128) char ring[];
+  extern __shared__ char raw[];
+  __shared__ __align__(8) uint64_t bars[kWarps][kBufs];
   __shared__ int part[kWarps];
   __shared__ int found[3];  // sequence, unit, tile
-  __shared__ float stat[kWarps][HT][2];
+  __shared__ float stat[kWarps][8][2];
+  char* const ring = raw + (-smem_u32(raw) & 1023u);
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int gtiles = (a.group + HT - 1) / HT, subs = a.kv_heads * gtiles;
+  const uint32_t my_ring = smem_u32(ring) + warp * kBufs * S::BUF, my_bar = smem_u32(bars[warp]);
+  if (lane == 0) {
+    for (int i = 0; i < kBufs; ++i) mbar_init(my_bar + 8 * i, 1);
+    mbar_init_fence();
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.k) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.v) : "memory");
+  }
+  __syncwarp();
   pdl_launch_dependents();
   pdl_wait();
 
   // ---------------------------------------------------------------- this CTA's run of tiles
-  Walk<S::CT> cs;
+  Walk<S> cs;
   int count;
   int64_t start = 0;
   if constexpr (DIRECT) {
@@ -181,7 +216,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<sizeof(C), DP>::PER_SM) dec
     const Space ws(a.workspace, a.num_seqs);
     int mine = 0, own = 0;  // own: tiles of sequence threadIdx.x
     for (int s = threadIdx.x; s < a.num_seqs; s += kWarps * 32) {
-      const int n = tiles_of<S::CT>(span_of(a, s)) * subs;
+      const int n = tiles_of<S>(span_of(a, s)) * subs;
       if (s == (int)threadIdx.x) own = n;
       mine += n;
     }
@@ -196,7 +231,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<sizeof(C), DP>::PER_SM) dec
     int base = 0;
     for (int s0 = 0; s0 < a.num_seqs; s0 += kWarps * 32) {
       const int s = s0 + threadIdx.x;
-      const int n = s >= a.num_seqs ? 0 : s0 == 0 ? own : tiles_of<S::CT>(span_of(a, s)) * subs;
+      const int n = s >= a.num_seqs ? 0 : s0 == 0 ? own : tiles_of<S>(span_of(a, s)) * subs;
       int sum;
       const int at = base + scan128(n, sum, part);
       if (s < a.num_seqs && start >= at && start < at + n) {
@@ -220,69 +255,78 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<sizeof(C), DP>::PER_SM) dec
   }
 
   // ---------------------------------------------------------------- the copy stream of this warp
-  const uint32_t my_ring = smem_u32(ring) + warp * kStages * S::SLOT;
-  const int chunks = a.head_dim * (int)sizeof(C) / 16, block_shift = __ffs(a.block_size) - 1;
-  Walk<S::CT> ld = cs;
+  // A run is the part of a warp tile that lies in one page: KW keys, or a whole
+  // page where pages are smaller.  Lane r copies run r.
+  const int block_shift = __ffs(a.block_size) - 1;
+  const int run_rows = a.block_size < S::KW ? a.block_size : S::KW, runs = S::KW / run_rows;
+  Walk<S> ld = cs;
   int ld_left = count;
-  struct Pending {
-    int page[(S::KW + 31) / 32];  // of key key0 + lane (+ 32); -1: zeros
-    int key0, hk;
-  } pend;
-  // looks up the pages of the next tile
-  auto look = [&](Pending& p) {
-    p.key0 = 0;
-    p.hk = 0;
-#pragma unroll
-    for (int i = 0; i < (S::KW + 31) / 32; ++i) p.page[i] = -1;
-    if (ld_left <= 0) return;
-    p.key0 = ld.span.lo + ld.tile * S::CT + warp * S::KW;
+  struct Source {
+    int page, slot, hk;  // of run `lane` (+ 32 where pages are single slots); page -1: nothing to copy
+    int page2;
+  };
+  // the pages of the next tile
+  auto look = [&]() {
+    Source p = {-1, 0, 0, -1};
+    if (ld_left <= 0) return p;
+    const int key0 = (ld.span.lo & -S::KW) + ld.tile * S::CT + warp * S::KW;
     p.hk = ld.sub / gtiles;
     const int32_t* table = a.block_tables + (int64_t)ld.seq * a.block_table_stride;
-#pragma unroll
-    for (int i = 0; i < (S::KW + 31) / 32; ++i) {
-      const int j = p.key0 + lane + 32 * i;
-      if (lane + 32 * i < S::KW && j < ld.span.n) {
-        const int page = table[j >> block_shift];
-        if (page >= 0 && page < a.num_blocks) p.page[i] = page;
-        else raise_status(a.status, OC_STATUS_BAD_PAGE);
-      }
-    }
+    auto page_of = [&](int r) {
+      const int j = key0 + r * run_rows;
+      if (r >= runs || j >= ld.span.n || j + run_rows <= ld.span.lo) return -1;
+      const int page = table[j >> block_shift];
+      if (page >= 0 && page < a.num_blocks) return page;
+      raise_status(a.status, OC_STATUS_BAD_PAGE);
+      return -1;
+    };
+    p.slot = key0 & (a.block_size - 1);  // 0 where a tile has several runs
+    p.page = page_of(lane);
+    if (S::KW > 32 && runs > 32) p.page2 = page_of(lane + 32);
     --ld_left;
     if (ld_left > 0) ld.next(a, subs);
+    return p;
   };
-  auto issue = [&](const Pending& p, int stage) {
-    const uint32_t kd = my_ring + stage * S::SLOT, vd = kd + S::HALF;
-    const char* kb = static_cast<const char*>(a.k_cache) + (int64_t)p.hk * a.kc_head_stride * sizeof(C);
-    const char* vb = static_cast<const char*>(a.v_cache) + (int64_t)p.hk * a.vc_head_stride * sizeof(C);
-#pragma unroll
-    for (int i = 0; i < S::KW * S::CH / 32; ++i) {
-      const int idx = i * 32 + lane, row = idx / S::CH, ch = idx % S::CH;
-      const int page = __shfl_sync(0xffffffffu, p.page[row / 32], row & 31);
-      const int slot = (p.key0 + row) & (a.block_size - 1);
-      const bool on = page >= 0 && ch < chunks;
-      const int64_t ko = on ? ((int64_t)page * a.kc_block_stride + (int64_t)slot * a.kc_tok_stride) * sizeof(C) + ch * 16 : 0;
-      const int64_t vo = on ? ((int64_t)page * a.vc_block_stride + (int64_t)slot * a.vc_tok_stride) * sizeof(C) + ch * 16 : 0;
-      const uint32_t at = row * S::ROW + ((ch ^ S::swz(row)) << 4);
-      cp_async16(kd + at, kb + ko, on ? 16 : 0);
-      cp_async16(vd + at, vb + vo, on ? 16 : 0);
-    }
+  const uint64_t policy = policy_evict_first();
+  auto copy_run = [&](const CUtensorMap* map, const int* role, const Source& p, int page, int r, uint32_t buf,
+                      uint32_t bar) {
+    auto coord = [&](int i) { return role[i] == 0 ? p.slot : role[i] == 1 ? p.hk : page; };
+    const int c1 = coord(0), c2 = coord(1), c3 = coord(2);
+    for (int x = 0; x < S::PANELS; ++x)  // columns from head_dim on arrive as zeros
+      tma_load_4d(buf + x * (S::KW * S::PANEL) + r * run_rows * S::PANEL, map, x * (S::PANEL / (int)sizeof(C)), c1, c2,
+                  c3, bar, policy);
   };
+  // fills buffer b with K (or V) of a tile
+  auto issue = [&](const CUtensorMap* map, const int* role, const Source& p, int b) {
+    const uint32_t buf = my_ring + b * S::BUF, bar = my_bar + 8 * b;
+    int n = __popc(__ballot_sync(0xffffffffu, p.page >= 0));
+    if (S::KW > 32) n += __popc(__ballot_sync(0xffffffffu, p.page2 >= 0));
+    if (lane == 0) mbar_arrive_expect_tx(bar, n * S::PANELS * run_rows * S::PANEL);
+    __syncwarp();
+    if (p.page >= 0) copy_run(map, role, p, p.page, lane, buf, bar);
+    if (S::KW > 32 && p.page2 >= 0) copy_run(map, role, p, p.page2, lane + 32, buf, bar);
+  };
+  Source for_v, for_k;  // the tile whose values, and the one whose keys, are copied next
   {
-    Pending first[kStages];
-#pragma unroll
-    for (int s = 0; s < kStages; ++s) look(first[s]);
-#pragma unroll
-    for (int s = 0; s < kStages - 1; ++s) {
-      issue(first[s], s);
-      cp_commit();
-    }
-    pend = first[kStages - 1];
+    const Source s0 = look(), s1 = look();
+    for_k = look();
+    issue(&maps.k, maps.k_role, s0, 0);
+    issue(&maps.v, maps.v_role, s0, 1);
+    issue(&maps.k, maps.k_role, s1, 2);
+    for_v = s1;
   }
+  uint32_t parity = 0;  // bit b: the phase of buffer b that completes next
+  auto arrived = [&](int b) {
+    const bool ok = mbar_wait_bounded(my_bar + 8 * b, parity >> b & 1, kPolls);
+    parity ^= 1u << b;
+    return ok;
+  };
 
   // ---------------------------------------------------------------- the unit's state
   uint32_t qf[KS][NT][2];
-  float acc[KS][NT][4], m[NT][2], mu[NT][2], l[NT][2], sc[NT][2], slope[NT][2];
-  const float inv_cap = a.softcap > 0.f ? 1.f / a.softcap : 0.f;
+  float acc[KS][NT][4], m[NT][2], l[NT][2], sc[NT][2], slope[NT][2];
+  const bool capped = a.softcap > 0.f, biased = a.slopes != nullptr;
+  const float cap2 = a.softcap * kLog2e;
 
   auto begin_unit = [&]() {
     const int hk = cs.sub / gtiles, h0 = hk * a.group + (cs.sub % gtiles) * HT;
@@ -328,10 +372,9 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<sizeof(C), DP>::PER_SM) dec
       for (int c = 0; c < 2; ++c) {
         const int hr = n * 8 + 2 * t + c;
         const float qs = __shfl_sync(0xffffffffu, qscale[n], (2 * t + c) * 4);
-        sc[n][c] = a.scale * a.k_scale / qs;
-        slope[n][c] = a.slopes && hr < heads ? a.slopes[h0 + hr] * kLog2e : 0.f;
+        sc[n][c] = a.scale * a.k_scale / qs * (capped ? 1.f / a.softcap : kLog2e);
+        slope[n][c] = biased && hr < heads ? a.slopes[h0 + hr] * kLog2e : 0.f;
         m[n][c] = -INFINITY;
-        mu[n][c] = 0.f;
         l[n][c] = 0.f;
 #pragma unroll
         for (int k = 0; k < KS; ++k) acc[k][n][c] = acc[k][n][c + 2] = 0.f;
@@ -339,11 +382,11 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<sizeof(C), DP>::PER_SM) dec
   };
 
   // ---------------------------------------------------------------- one warp tile
-  auto compute = [&](int stage) {
-    const uint32_t kd = my_ring + stage * S::SLOT, vd = kd + S::HALF;
-    const int key0 = cs.span.lo + cs.tile * S::CT + warp * S::KW;
-    if (key0 >= cs.span.n) return;
-    float s[S::KT][NT][4];
+  float s[S::KT][NT][4];
+  // scores in log2 units, the mask, and the running maximum
+  auto scores = [&](int b) {
+    const uint32_t kd = my_ring + b * S::BUF;
+    const int key0 = (cs.span.lo & -S::KW) + cs.tile * S::CT + warp * S::KW;
 #pragma unroll
     for (int kt = 0; kt < S::KT; ++kt) {
 #pragma unroll
@@ -351,17 +394,15 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<sizeof(C), DP>::PER_SM) dec
 #pragma unroll
         for (int c = 0; c < 4; ++c) s[kt][n][c] = 0.f;
       const int row = kt * 16 + (lane & 15);
-      const uint32_t base = kd + row * S::ROW;
-      const int x = S::swz(row);
       if constexpr (F8) {
 #pragma unroll
         for (int k = 0; k < KS; k += 2) {
           uint32_t r[4];
-          ldsm_x4(base + (((k + (lane >> 4)) ^ x) << 4), r);
+          ldsm_x4(kd + S::at(row, k + (lane >> 4)), r);
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            const uint32_t f[4] = {fp8x2_to_half2(r[2 * u]), fp8x2_to_half2(r[2 * u + 1]),
-                                   fp8x2_to_half2(r[2 * u] >> 16), fp8x2_to_half2(r[2 * u + 1] >> 16)};
+            const uint32_t f[4] = {fp8x2_to_half2(r[2 * u]), fp8x2_to_half2(r[2 * u + 1]), fp8x2_to_half2_hi(r[2 * u]),
+                                   fp8x2_to_half2_hi(r[2 * u + 1])};
 #pragma unroll
             for (int n = 0; n < NT; ++n) mma16816<BF16>(s[kt][n], f, qf[k + u][n][0], qf[k + u][n][1]);
           }
@@ -370,44 +411,69 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<sizeof(C), DP>::PER_SM) dec
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
           uint32_t r[4];
-          ldsm_x4(base + (((2 * k + (lane >> 4)) ^ x) << 4), r);
+          ldsm_x4(kd + S::at(row, 2 * k + (lane >> 4)), r);
 #pragma unroll
           for (int n = 0; n < NT; ++n) mma16816<BF16>(s[kt][n], r, qf[k][n][0], qf[k][n][1]);
         }
       }
     }
-    // scores in log2 units; the mask on the last tile only (tiles start at the first visible key)
-    const bool whole = key0 + S::KW <= cs.span.n;
-    bool grow = false;
 #pragma unroll
     for (int kt = 0; kt < S::KT; ++kt)
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
+        for (int c = 0; c < 4; ++c) s[kt][n][c] *= sc[n][c & 1];
+    if (capped) {
+#pragma unroll
+      for (int kt = 0; kt < S::KT; ++kt)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) s[kt][n][c] = cap2 * tanhf(s[kt][n][c]);
+    }
+    if (biased) {
+#pragma unroll
+      for (int kt = 0; kt < S::KT; ++kt)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            s[kt][n][c] = fmaf(slope[n][c & 1], (float)(key0 + kt * 16 + g + (c >> 1) * 8 - (cs.span.n - 1)), s[kt][n][c]);
+    }
+    if (key0 < cs.span.lo || key0 + S::KW > cs.span.n) {
+#pragma unroll
+      for (int kt = 0; kt < S::KT; ++kt)
+#pragma unroll
         for (int c = 0; c < 4; ++c) {
           const int j = key0 + kt * 16 + g + (c >> 1) * 8;
-          float x = s[kt][n][c] * sc[n][c & 1];
-          if (a.softcap > 0.f) x = a.softcap * tanhf(x * inv_cap);
-          x = fmaf(slope[n][c & 1], (float)(j - (cs.span.n - 1)), x * kLog2e);
-          if (!whole && j >= cs.span.n) x = -INFINITY;
-          s[kt][n][c] = x;
-          grow |= x > m[n][c & 1] + 8.f;
+          if (j < cs.span.lo || j >= cs.span.n)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) s[kt][n][c] = -INFINITY;
         }
+    }
     // The maximum moves only when a score exceeds it by 2^8 (sums stay in float32, p below 2^8 in 16
     // bits loses nothing): most tiles skip the reduction and the rescaling.
+    bool grow = false;
+    float top[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        top[n][c] = fmaxf(s[0][n][c], s[0][n][c + 2]);
+#pragma unroll
+        for (int kt = 1; kt < S::KT; ++kt) top[n][c] = fmaxf(top[n][c], fmaxf(s[kt][n][c], s[kt][n][c + 2]));
+        grow |= top[n][c] > m[n][c] + 8.f;
+      }
     if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          float top = m[n][c];
+          float x = fmaxf(m[n][c], top[n][c]);
 #pragma unroll
-          for (int kt = 0; kt < S::KT; ++kt) top = fmaxf(top, fmaxf(s[kt][n][c], s[kt][n][c + 2]));
-#pragma unroll
-          for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-          const float back = m[n][c] == -INFINITY ? 0.f : exp2f(m[n][c] - top);
-          m[n][c] = top;
-          mu[n][c] = top == -INFINITY ? 0.f : top;
+          for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+          const float back = m[n][c] == -INFINITY ? 0.f : exp2f(m[n][c] - x);
+          m[n][c] = x;
           l[n][c] *= back;
 #pragma unroll
           for (int k = 0; k < KS; ++k) {
@@ -416,6 +482,21 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<sizeof(C), DP>::PER_SM) dec
           }
         }
     }
+  };
+  // values that the mask hides become zeros: 0 times what a free slot holds need not be 0
+  auto clear_hidden = [&](int b) {
+    const int key0 = (cs.span.lo & -S::KW) + cs.tile * S::CT + warp * S::KW;
+    if (key0 >= cs.span.lo && key0 + S::KW <= cs.span.n) return;
+    char* vb = ring + (warp * kBufs + b) * S::BUF;
+    for (int i = lane; i < S::KW * (S::ROW / 16); i += 32) {
+      const int r = i / (S::ROW / 16), j = key0 + r;
+      if (j < cs.span.lo || j >= cs.span.n) *reinterpret_cast<uint4*>(vb + S::at(r, i % (S::ROW / 16))) = uint4{0, 0, 0, 0};
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the next copy into the buffer
+    __syncwarp();
+  };
+  auto values = [&](int b) {
+    const uint32_t vd = my_ring + b * S::BUF;
 #pragma unroll
     for (int kt = 0; kt < S::KT; ++kt) {
       uint32_t p[NT][2];
@@ -424,37 +505,35 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<sizeof(C), DP>::PER_SM) dec
         float e[4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          e[c] = ex2(s[kt][n][c] - mu[n][c & 1]);
+          const float mc = m[n][c & 1];
+          e[c] = ex2(s[kt][n][c] - (mc == -INFINITY ? 0.f : mc));
           l[n][c & 1] += e[c];
         }
         p[n][0] = transpose8x8(pack16<BF16>(e[0], e[1]));
         p[n][1] = transpose8x8(pack16<BF16>(e[2], e[3]));
       }
-      const int row = kt * 16 + (lane & 7) + ((lane >> 4) << 3);
-      const uint32_t base = vd + row * S::ROW;
-      const int x = S::swz(row);
       if constexpr (F8) {
         // matrices: keys 0-7 and 8-15 of one 16-column chunk, then of the next
-        const int row8 = kt * 16 + (lane & 15);
-        const uint32_t base8 = vd + row8 * S::ROW;
+        const int row = kt * 16 + (lane & 15);
 #pragma unroll
         for (int k = 0; k < KS; k += 2) {
           uint32_t r[4];
-          ldsm_x4_t(base8 + (((k + (lane >> 4)) ^ S::swz(row8)) << 4), r);
+          ldsm_x4_t(vd + S::at(row, k + (lane >> 4)), r);
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            const uint32_t r0 = r[2 * u], r1 = r[2 * u + 1];
-            const uint32_t f[4] = {fp8x2_to_half2(__byte_perm(r0, 0, 0x4420)), fp8x2_to_half2(__byte_perm(r0, 0, 0x4431)),
-                                   fp8x2_to_half2(__byte_perm(r1, 0, 0x4420)), fp8x2_to_half2(__byte_perm(r1, 0, 0x4431))};
+            // bytes (key 2t: d, d + 1; key 2t + 1: d, d + 1) to (d: both keys; d + 1: both keys)
+            const uint32_t r0 = __byte_perm(r[2 * u], 0, 0x3120), r1 = __byte_perm(r[2 * u + 1], 0, 0x3120);
+            const uint32_t f[4] = {fp8x2_to_half2(r0), fp8x2_to_half2_hi(r0), fp8x2_to_half2(r1), fp8x2_to_half2_hi(r1)};
 #pragma unroll
             for (int n = 0; n < NT; ++n) mma16816<BF16>(acc[k + u][n], f, p[n][0], p[n][1]);
           }
         }
       } else {
+        const int row = kt * 16 + (lane & 7) + ((lane >> 4) << 3);
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
           uint32_t r[4];
-          ldsm_x4_t(base + (((2 * k + ((lane >> 3) & 1)) ^ x) << 4), r);
+          ldsm_x4_t(vd + S::at(row, 2 * k + ((lane >> 3) & 1)), r);
 #pragma unroll
           for (int n = 0; n < NT; ++n) mma16816<BF16>(acc[k][n], r, p[n][0], p[n][1]);
         }
@@ -463,18 +542,21 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<sizeof(C), DP>::PER_SM) dec
   };
 
   // ---------------------------------------------------------------- end of a unit (or of the CTA's part of it)
-  // Each warp's state goes through the ring slot that it has just consumed.
-  auto end_unit = [&](int stage, bool complete, int slot) {
-    float* mine = reinterpret_cast<float*>(ring + warp * kStages * S::SLOT + stage * S::SLOT);
-    __syncwarp();
+  // The warps' states meet in the buffers that each has just consumed, 8 heads at a time.
+  auto end_unit = [&](int b, bool complete, int slot) {
+    float* mine = reinterpret_cast<float*>(ring + (warp * kBufs + b) * S::BUF);
+    const int hk = cs.sub / gtiles, h0 = hk * a.group + (cs.sub % gtiles) * HT;
+    const int heads = min(HT, a.group - (cs.sub % gtiles) * HT);
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int n = 0; n < NT; ++n) {
+      if (n * 8 >= heads) break;
+      __syncthreads();  // every warp has left its buffer (and the round before) behind
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         float sum = l[n][c];
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        const int hr = n * 8 + 2 * t + c;
+        const int hr = 2 * t + c;
         if (g == 0) {
           stat[warp][hr][0] = m[n][c];
           stat[warp][hr][1] = sum;
@@ -486,76 +568,78 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<sizeof(C), DP>::PER_SM) dec
           mine[hr * DP + (d1 ^ (t << 3))] = acc[k][n][c + 2];
         }
       }
-    __syncthreads();
-    const int hk = cs.sub / gtiles, h0 = hk * a.group + (cs.sub % gtiles) * HT;
-    const int heads = min(HT, a.group - (cs.sub % gtiles) * HT);
-    // a warp per head
-    for (int hr = warp; hr < heads; hr += kWarps) {
-      float top = -INFINITY, sum = 0.f, f[kWarps];
+      __syncthreads();
+      // a warp per head
+      for (int hr = warp; hr < min(8, heads - n * 8); hr += kWarps) {
+        float top = -INFINITY, sum = 0.f, f[kWarps];
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) top = fmaxf(top, stat[w][hr][0]);
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        // a maximum of -inf with a sum that is not 0 is a NaN score: it stays
-        f[w] = stat[w][hr][0] == -INFINITY ? (stat[w][hr][1] == 0.f ? 0.f : 1.f) : exp2f(stat[w][hr][0] - top);
-        sum += stat[w][hr][1] * f[w];
-      }
-      const int swz = ((hr >> 1) & 3) << 3;
-      const float inv = sum == 0.f ? 0.f : a.v_scale / sum;
-      float* state = nullptr;
-      if constexpr (!DIRECT)
-        state = Space(a.workspace, a.num_seqs).states + (int64_t)(2 * blockIdx.x + slot) * state_floats(HT, DP);
-      T* out = static_cast<T*>(a.out) + (int64_t)cs.seq * a.out_seq_stride + (int64_t)(h0 + hr) * a.out_head_stride;
-#pragma unroll
-      for (int i = 0; i < DP / 32; ++i) {
-        const int d = lane + 32 * i;
-        float x = 0.f;
+        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, stat[w][hr][0]);
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-          const float* o = reinterpret_cast<const float*>(ring + w * kStages * S::SLOT + stage * S::SLOT);
-          x = fmaf(o[hr * DP + (d ^ swz)], f[w], x);
+          // a maximum of -inf with a sum that is not 0 is a NaN score: it stays
+          f[w] = stat[w][hr][0] == -INFINITY ? (stat[w][hr][1] == 0.f ? 0.f : 1.f) : exp2f(stat[w][hr][0] - top);
+          sum = fmaf(stat[w][hr][1], f[w], sum);
         }
-        if (DIRECT || complete) {
-          if (d < a.head_dim) out[d] = from_f32<T>(x * inv);
-        } else {
-          state[hr * DP + d] = x;
+        const int swz = ((hr >> 1) & 3) << 3, head = h0 + n * 8 + hr;
+        const float inv = sum == 0.f ? 0.f : a.v_scale / sum;
+        float* state = nullptr;
+        if constexpr (!DIRECT)
+          state = Space(a.workspace, a.num_seqs).states + (int64_t)(2 * blockIdx.x + slot) * state_floats(HT, DP);
+        T* out = static_cast<T*>(a.out) + (int64_t)cs.seq * a.out_seq_stride + (int64_t)head * a.out_head_stride;
+#pragma unroll
+        for (int i = 0; i < DP / 32; ++i) {
+          const int d = lane + 32 * i;
+          float x = 0.f;
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w)
+            x = fmaf(reinterpret_cast<const float*>(ring + (w * kBufs + b) * S::BUF)[hr * DP + (d ^ swz)], f[w], x);
+          if (DIRECT || complete) {
+            if (d < a.head_dim) out[d] = from_f32<T>(x * inv);
+          } else {
+            state[(n * 8 + hr) * DP + d] = x;
+          }
         }
-      }
-      if (lane == 0) {
-        if (DIRECT || complete) {
-          if (a.lse)
-            a.lse[(int64_t)cs.seq * a.kv_heads * a.group + h0 + hr] =
-                sum == 0.f ? -INFINITY : ((top == -INFINITY ? 0.f : top) + log2f(sum)) * kLn2;
-        } else {
-          state[HT * DP + 2 * hr] = top;
-          state[HT * DP + 2 * hr + 1] = sum;
+        if (lane == 0) {
+          if (DIRECT || complete) {
+            if (a.lse)
+              a.lse[(int64_t)cs.seq * a.kv_heads * a.group + head] =
+                  sum == 0.f ? -INFINITY : ((top == -INFINITY ? 0.f : top) + log2f(sum)) * kLn2;
+          } else {
+            state[HT * DP + 2 * (n * 8 + hr)] = top;
+            state[HT * DP + 2 * (n * 8 + hr) + 1] = sum;
+          }
         }
       }
     }
     __syncthreads();
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the next copy into the buffer
+    __syncwarp();
   };
 
   // ---------------------------------------------------------------- main loop
   begin_unit();
   bool from_start = cs.tile == 0;  // this CTA has the unit from its first tile
-  int stage = 0, ahead = kStages - 1;
+  int kb = 0;                      // buffer of the tile's keys; its values are in the next one
+  bool late = false;               // a copy did not arrive within the bound
   for (int i = 0; i < count; ++i) {
-    cp_wait<kStages - 2>();
+    const int vb = kb + 1 == kBufs ? 0 : kb + 1;
+    late = !arrived(kb);
+    if (late) break;
+    scores(kb);
     __syncwarp();
-    compute(stage);
+    if (i + 1 < count) issue(&maps.v, maps.v_role, for_v, kb);
+    late = !arrived(vb);
+    if (late) break;
+    clear_hidden(vb);
+    values(vb);
     __syncwarp();
     const bool last_tile = cs.tile + 1 == cs.tiles;
-    if (last_tile || i + 1 == count) {
-      const bool complete = from_start && last_tile;
-      // a CTA leaves at most two partial states: of a unit begun by others, and of one that it began
-      end_unit(stage, complete, from_start ? 1 : 0);
-    }
-    // the slot consumed before this one is free in every case: refill
-    issue(pend, ahead);
-    cp_commit();
-    look(pend);
-    stage = stage + 1 == kStages ? 0 : stage + 1;
-    ahead = ahead + 1 == kStages ? 0 : ahead + 1;
+    // a CTA leaves at most two partial states: of a unit begun by others, and of one that it began
+    if (last_tile || i + 1 == count) end_unit(vb, from_start && last_tile, from_start ? 1 : 0);
+    if (i + 2 < count) issue(&maps.k, maps.k_role, for_k, vb);
+    for_v = for_k;
+    for_k = look();
+    kb = vb + 1 == kBufs ? 0 : vb + 1;
     if (i + 1 < count) {
       cs.next(a, subs);
       if (cs.tile == 0) {
@@ -564,13 +648,17 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<sizeof(C), DP>::PER_SM) dec
       }
     }
   }
-  cp_wait<0>();
+  if (late) {  // report it, and let this warp's other copies land before the CTA's memory is reused
+    raise_status(a.status, OC_STATUS_TIMEOUT);
+#pragma unroll 1
+    for (int b = 0; b < kBufs; ++b) mbar_wait_bounded(my_bar + 8 * b, parity >> b & 1, kPolls);
+  }
 }
 
 // Joins the partial states of the units that were split: one CTA per
 // (unit, head), its warps take the parts in turn, and their sums are added in
 // a fixed order.
-template <typename T, int DP, int NT, int CT>
+template <typename T, int DP, int NT>
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ oc_paged_decode_args a) {
   constexpr int HT = 8 * NT, W = 8;
   __shared__ float sm[W][2];
@@ -671,6 +759,8 @@ bool tiled(const oc_paged_decode_args& a) {
   if (a.dtype == OC_F32 || a.max_blocks == 0) return false;
   const int es = type_bytes(a.cache_dtype);
   auto ok = [&](int64_t s) { return (s * es) % 16 == 0; };
+  // a box of the copy engine lands on a multiple of 128 bytes
+  if (padded(a.head_dim) * es * a.block_size < 128) return false;
   return a.head_dim * es % 16 == 0 && a.head_dim >= 16 && aligned_to(a.k_cache, 16) && aligned_to(a.v_cache, 16) &&
          ok(a.kc_block_stride) && ok(a.kc_head_stride) && ok(a.kc_tok_stride) && ok(a.vc_block_stride) &&
          ok(a.vc_head_stride) && ok(a.vc_tok_stride);
@@ -682,19 +772,73 @@ struct Plan {
   int nt;
 };
 
+template <int ES, int DP, int NT>
+void plan_nt(const oc_paged_decode_args& a, Plan& p) {
+  using S = Shape<ES, DP, NT>;
+  const int64_t gt = (a.group + 8 * NT - 1) / (8 * NT), units = a.num_seqs * (int64_t)a.kv_heads * gt;
+  int64_t most = (int64_t)a.max_blocks * a.block_size;
+  if (a.window > 0 && a.window + S::KW < most) most = a.window + S::KW;
+  const int64_t tiles = (most + S::CT - 1) / S::CT, wave = (int64_t)a.num_sms * S::PER_SM;
+  const int64_t useful = (units * tiles + kMinShare - 1) / kMinShare;
+  p.nt = NT;
+  p.direct = tiles <= kDirectTiles;
+  p.grid = p.direct ? units : useful < wave ? useful : wave;
+}
 template <int ES, int DP>
 Plan plan_of(const oc_paged_decode_args& a) {
-  using S = Shape<ES, DP>;
   Plan p;
-  p.nt = a.group <= 8 ? 1 : 2;
-  const int64_t gt = (a.group + 8 * p.nt - 1) / (8 * p.nt), units = a.num_seqs * (int64_t)a.kv_heads * gt;
-  int64_t most = (int64_t)a.max_blocks * a.block_size;
-  if (a.window > 0 && a.window < most) most = a.window;
-  p.direct = most <= (int64_t)S::CT * kDirectTiles;
-    const int64_t tiles = units * ((most + S::CT - 1) / S::CT), wave = (int64_t)a.num_sms * S::PER_SM;
-  const int64_t useful = (tiles + kMinShare - 1) / kMinShare;
-  p.grid = p.direct ? units : useful < wave ? useful : wave;
+  // groups above 8 take two tiles of 8 heads at once, where the state fits the registers
+  if constexpr (DP < 256) {
+    if (a.group > 8) {
+      plan_nt<ES, DP, 2>(a, p);
+      return p;
+    }
+  }
+  plan_nt<ES, DP, 1>(a, p);
   return p;
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 map_encoder() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+  });
+  return fn;
+}
+
+bool encode(CUtensorMap* map, int (&role)[3], const void* base, const oc_paged_decode_args& a, int64_t tok_stride,
+            int64_t head_stride, int64_t block_stride, int panel_bytes, int rows) {
+  const auto enc = map_encoder();
+  if (!enc) return false;
+  const int es = type_bytes(a.cache_dtype);
+  const int64_t size[3] = {a.block_size, a.kv_heads, a.num_blocks}, stride[3] = {tok_stride, head_stride, block_stride};
+  auto key = [&](int r) { return size[r] == 1 ? INT64_MAX : stride[r]; };  // the stride of a single entry is free
+  for (int i = 0; i < 3; ++i) role[i] = i;
+  for (int i = 0; i < 3; ++i)
+    for (int j = i + 1; j < 3; ++j)
+      if (key(role[j]) < key(role[i])) std::swap(role[i], role[j]);
+  cuuint64_t dim[4] = {(cuuint64_t)a.head_dim}, bytes[3];
+  cuuint32_t box[4] = {(cuuint32_t)(panel_bytes / es)}, step[4] = {1, 1, 1, 1};
+  int64_t nest = ((int64_t)a.head_dim * es + 15) / 16 * 16;
+  for (int i = 0; i < 3; ++i) {
+    const int64_t b = size[role[i]] == 1 ? nest : stride[role[i]] * es;
+    if (b < nest && size[role[i]] > 1) return false;  // rows that overlap (broadcast caches)
+    dim[i + 1] = (cuuint64_t)size[role[i]];
+    bytes[i] = (cuuint64_t)b;
+    box[i + 1] = role[i] == 0 ? rows : 1;
+    nest = b;
+  }
+  const CUtensorMapDataType type = a.cache_dtype == OC_F8E4M3 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                   : a.cache_dtype == OC_F16  ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                              : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  return enc(map, type, 4, const_cast<void*>(base), dim, bytes, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             panel_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <typename F>
@@ -712,24 +856,31 @@ auto by_shape(const oc_paged_decode_args& a, F f) {
 
 template <typename T, typename C, int DP, int NT>
 int launch_tiled(const oc_paged_decode_args& a, const Plan& p, void* stream) {
-  using S = Shape<sizeof(C), DP>;
+  using S = Shape<sizeof(C), DP, NT>;
+  Maps maps;
+  const int rows = a.block_size < S::KW ? a.block_size : S::KW;
+  if (!encode(&maps.k, maps.k_role, a.k_cache, a, a.kc_tok_stride, a.kc_head_stride, a.kc_block_stride, S::PANEL, rows) ||
+      !encode(&maps.v, maps.v_role, a.v_cache, a, a.vc_tok_stride, a.vc_head_stride, a.vc_block_stride, S::PANEL, rows))
+    return launch_rows<T, C>(a, stream);
   auto kernel = p.direct ? decode_kernel<T, C, DP, NT, true> : decode_kernel<T, C, DP, NT, false>;
-  if (S::SMEM > 48 * 1024 &&
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM) != cudaSuccess) {
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM) != cudaSuccess) {
     cudaGetLastError();
     return OC_ERR_CUDA;
   }
-  int rc = launch_pdl(kernel, dim3((unsigned)p.grid), dim3(kWarps * 32), S::SMEM, stream, a);
+  int rc = launch_pdl(kernel, dim3((unsigned)p.grid), dim3(kWarps * 32), S::SMEM, stream, a, maps);
   if (rc != OC_OK || p.direct) return rc;
-  return launch_pdl(join_kernel<T, DP, NT, S::CT>, dim3((unsigned)(a.kv_heads * a.group), (unsigned)a.num_seqs),
-                    dim3(256), 0, stream, a);
+  return launch_pdl(join_kernel<T, DP, NT>, dim3((unsigned)(a.kv_heads * a.group), (unsigned)a.num_seqs), dim3(256), 0,
+                    stream, a);
 }
 
 template <typename T, typename C, int DP>
 int launch_nt(const oc_paged_decode_args& a, void* stream) {
   const Plan p = plan_of<sizeof(C), DP>(a);
   if (p.grid > 0x7fffffff) return OC_ERR_TOO_LARGE;
-  return p.nt == 1 ? launch_tiled<T, C, DP, 1>(a, p, stream) : launch_tiled<T, C, DP, 2>(a, p, stream);
+  if constexpr (DP < 256) {
+    if (p.nt == 2) return launch_tiled<T, C, DP, 2>(a, p, stream);
+  }
+  return launch_tiled<T, C, DP, 1>(a, p, stream);
 }
 
 template <typename T, typename C>
