@@ -1,22 +1,489 @@
 // Attention of packed prompts over themselves.
+//
+//   s_ij = cap(scale q_i.k_j) - slope |p_i - j|,  o_i = sum_j 2^(s_ij - m_i) v_j / sum_j 2^(s_ij - m_i)
+//
+// over the keys that the mask leaves.  4 D operations per query-key pair
+// against one exponential: on this part a 128 x 128 tile takes 1024 cycles of
+// the tensor cores at D = 128 (512 at D = 64) and 1024 cycles of the
+// exponential unit (16 a cycle), so the two are kept busy at the same time:
+// a CTA works on two tiles of 128 queries in turn, and while one tile's scores
+// go through the softmax the tensor cores multiply for the other.
+//
+// Roles: 4 + 4 softmax warps (a thread per query row), one warp that issues
+// the matrix instructions, one that issues the copies.  Q, K and V arrive by
+// TMA in 128-byte-swizzled panels of 64 columns; S = Q K^T and O += P V
+// accumulate in tensor memory (S0 S1 O0 O1, 512 columns); P overwrites S in 16
+// bits and is the second product's operand from there, V is read as it lies
+// (contiguous in D).  O is rescaled only when a row's maximum has grown by
+// 2^8: almost never after the first tiles.  Key tiles that the mask hides from
+// all 128 queries are neither copied nor multiplied.
+//
+// A key that the mask hides weighs 0, but 0 times an infinity or NaN in its
+// value (or in a neighbouring document that shares the tile) is not 0; rows
+// whose sum comes out not finite are therefore computed again from the
+// definition, over their visible keys only.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <mutex>
+#include <type_traits>
+
 #include "oc_attn_row.cuh"
+#include "oc_tc.cuh"
 
 namespace {
 
 using namespace oc;
 
-// The document of query row t: binary search in cu (docs + 1 entries); -1 if none.
-__device__ __forceinline__ int find_doc(const int32_t* cu, int docs, int64_t t) {
-  if (docs < 1 || t < cu[0] || t >= cu[docs]) return -1;
-  int lo = 0, hi = docs;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (cu[mid] <= t) lo = mid;
-    else hi = mid;
+// ------------------------------------------------------------------ documents and masks
+// One document: query rows [q0, q1), keys [k0, k0 + n); query row r sits at r - q0 + shift.
+struct Doc {
+  int64_t q0, q1, k0;
+  int n, shift, prefix;
+};
+
+// Rows outside every document form documents -1 (before the first) and docs (after the last), without keys.
+__device__ __forceinline__ Doc get_doc(const oc_prompt_args& a, int d) {
+  Doc r = {0, a.tokens, 0, (int)a.key_tokens, 0, 0};
+  if (a.cu_q) {
+    r.q0 = d < 0 ? 0 : a.cu_q[d];
+    r.q1 = d >= a.docs ? a.tokens : a.cu_q[d + 1];
+    bool bad = r.q0 < 0 || r.q1 < r.q0 || r.q1 > a.tokens;
+    r.n = 0;
+    if (d >= 0 && d < a.docs) {
+      r.k0 = a.cu_k[d];
+      const int64_t k1 = a.cu_k[d + 1];
+      bad = bad || r.k0 < 0 || k1 < r.k0 || k1 > a.key_tokens;
+      r.n = (int)(k1 - r.k0);
+    }
+    if (bad) {
+      raise_status(a.status, OC_STATUS_POSITION);
+      r.q0 = min(max(r.q0, (int64_t)0), a.tokens);
+      r.q1 = min(max(r.q1, r.q0), a.tokens);
+      r.k0 = 0;
+      r.n = 0;
+    }
   }
-  return lo;
+  r.shift = r.n - (int)(r.q1 - r.q0);
+  r.prefix = a.prefix_lens && d >= 0 && d < a.docs ? min(a.prefix_lens[d], r.n) : 0;
+  return r;
 }
 
+// Keys that a query at position p sees: [lo, hi) and [0, prefix).
+struct Sight {
+  int lo, hi;
+};
+__device__ __forceinline__ Sight sight_of(const oc_prompt_args& a, const Doc& d, int p) {
+  const int lo = a.window > 0 ? p - a.window + 1 : 0;
+  return Sight{lo < 0 ? 0 : lo, a.causal ? min(p + 1, d.n) : d.n};
+}
+
+// ------------------------------------------------------------------ the tiled kernel
+constexpr int kBM = 128;       // queries of a tile; two tiles a CTA
+constexpr int kBN = 128;       // keys of a tile
+constexpr int kThreads = 384;  // softmax 0, softmax 1, matrix warp, copy warp, two idle warps
+constexpr uint32_t kPolls = 1u << 22;  // bound of a wait
+
+template <int DP>
+struct Tile {
+  static constexpr int PANEL = kBN * 128;      // bytes of 128 rows of 64 columns
+  static constexpr int PANELS = DP / 64;
+  static constexpr int BYTES = PANEL * PANELS;  // of a Q, K or V tile
+  static constexpr int STAGES = DP == 128 ? 5 : 8;
+  static constexpr int SMEM = (2 + STAGES) * BYTES + 1024;
+};
+
+struct Maps {
+  CUtensorMap q, k, v;
+  int q_swap, k_swap, v_swap;  // dimensions are (columns, head, row), or (columns, row, head)
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+  if constexpr (BF16) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  } else {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+}
+
+// GENERAL: scores are capped, biased or scaled by a factor that is not
+// positive; else the scale is folded into the exponential.
+template <typename T, int DP, bool GENERAL>
+__global__ void __launch_bounds__(kThreads, 1)
+    prompt_kernel(const __grid_constant__ oc_prompt_args a, const __grid_constant__ Maps maps) {
+  using L = Tile<DP>;
+  constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+  extern __shared__ char raw[];
+  __shared__ __align__(8) uint64_t bars[2 * L::STAGES + 8];
+  __shared__ uint32_t tmem_at;
+  __shared__ Doc s_doc;
+  __shared__ int s_tile;  // which pair of query tiles of the document; -1: none
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
+  const uint32_t bar0 = smem_u32(bars);
+  auto kv_full = [&](int s) { return bar0 + 8 * s; };
+  auto kv_empty = [&](int s) { return bar0 + 8 * (L::STAGES + s); };
+  auto q_full = [&](int t) { return bar0 + 8 * (2 * L::STAGES + t); };
+  auto s_full = [&](int t) { return bar0 + 8 * (2 * L::STAGES + 2 + t); };
+  auto p_full = [&](int t) { return bar0 + 8 * (2 * L::STAGES + 4 + t); };
+  auto o_full = [&](int t) { return bar0 + 8 * (2 * L::STAGES + 6 + t); };
+
+  if (warp == 8 && lane == 0) {
+    for (int s = 0; s < L::STAGES; ++s) {
+      mbar_init(kv_full(s), 1);
+      mbar_init(kv_empty(s), 1);
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(q_full(t), 1);
+      mbar_init(s_full(t), 1);
+      mbar_init(p_full(t), 4);
+      mbar_init(o_full(t), 1);
+    }
+    mbar_init_fence();
+  }
+  if (warp == 9) tmem_alloc(smem_u32(&tmem_at), 512);
+  pdl_launch_dependents();
+  pdl_wait();
+  // the pair of query tiles of this CTA, the document's last pair first (causal: the longest)
+  if (warp == 0) {
+    int before = 0, doc = -2, tile = -1;
+    for (int d0 = a.cu_q ? -1 : 0; d0 <= a.docs && tile < 0; d0 += 32) {
+      const int d = d0 + lane;
+      int n = 0;
+      if (d <= a.docs && (a.cu_q || d == 0)) {
+        const Doc x = get_doc(a, d);
+        n = (int)((x.q1 - x.q0 + 2 * kBM - 1) / (2 * kBM));
+      }
+      int up = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, up, o);
+        if (lane >= o) up += y;
+      }
+      const int at = (int)blockIdx.x - before - (up - n);
+      const unsigned hit = __ballot_sync(0xffffffffu, at >= 0 && at < n);
+      if (hit) {
+        const int who = __ffs(hit) - 1;
+        doc = d0 + who;
+        tile = __shfl_sync(0xffffffffu, n - 1 - at, who);
+      }
+      before += __shfl_sync(0xffffffffu, up, 31);
+    }
+    if (lane == 0) {
+      s_tile = tile;
+      if (tile >= 0) s_doc = get_doc(a, doc);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_at;
+  const int pair = s_tile;
+  if (pair >= 0) {
+    const Doc doc = s_doc;
+    const int h = blockIdx.y, hk = h / a.group;
+    const int64_t row0 = doc.q0 + (int64_t)pair * 2 * kBM;  // first query row of tile 0
+    const int rows = (int)min((int64_t)2 * kBM, doc.q1 - row0);
+    const int key_tiles = (doc.n + kBN - 1) / kBN;
+    // whether any query of tile t sees a key of key tile j
+    auto need = [&](int t, int j) {
+      const int r = min(kBM, rows - t * kBM);
+      if (r <= 0) return false;
+      const int p = (int)(row0 - doc.q0) + t * kBM + doc.shift;
+      const Sight first = sight_of(a, doc, p), last = sight_of(a, doc, p + r - 1);
+      return j * kBN < doc.prefix || (j * kBN < last.hi && (j + 1) * kBN > first.lo);
+    };
+    auto next = [&](int j) {
+      for (++j; j < key_tiles; ++j)
+        if (need(0, j) || need(1, j)) break;
+      return j;
+    };
+    const int start = next(-1);
+    bool ok = true;
+    auto wait = [&](uint32_t bar, uint32_t parity) {
+      if (ok) ok = mbar_wait_bounded(bar, parity, kPolls);
+      return ok;
+    };
+
+    // registers: 8 warps x 32 x 216 + 4 x 32 x 72 = 384 x 168, what the CTA was launched with
+    if (warp >= 8) {
+     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+     if (warp == 9) {
+      // ------------------------------------------------------------ copies
+      if (lane == 0) {
+        auto tile_in = [&](const CUtensorMap* map, int swap, int head, int64_t row, uint32_t dst, uint32_t bar) {
+          mbar_arrive_expect_tx(bar, L::BYTES);
+#pragma unroll
+          for (int p = 0; p < L::PANELS; ++p)
+            tma_load_3d(dst + p * L::PANEL, map, p * 64, swap ? (int)row : head, swap ? head : (int)row, bar);
+        };
+        int idx = 0;
+        auto stage_in = [&](const CUtensorMap* map, int swap, int j) {
+          const int s = idx % L::STAGES;
+          if (!wait(kv_empty(s), ((idx / L::STAGES) & 1) ^ 1)) return;
+          tile_in(map, swap, hk, doc.k0 + (int64_t)j * kBN, base + (2 + s) * L::BYTES, kv_full(s));
+          ++idx;
+        };
+        if (start < key_tiles) {
+          tile_in(&maps.q, maps.q_swap, h, row0, base, q_full(0));
+          stage_in(&maps.k, maps.k_swap, start);
+          if (rows > kBM) tile_in(&maps.q, maps.q_swap, h, row0 + kBM, base + L::BYTES, q_full(1));
+          for (int j = start; j < key_tiles && ok;) {
+            stage_in(&maps.v, maps.v_swap, j);
+            j = next(j);
+            if (j < key_tiles) stage_in(&maps.k, maps.k_swap, j);
+          }
+        }
+        // every copy has landed before the CTA's memory is given back
+        if (start < key_tiles) {
+          mbar_wait_bounded(q_full(0), 0, kPolls);
+          if (rows > kBM) mbar_wait_bounded(q_full(1), 0, kPolls);
+        }
+        for (int i = idx > L::STAGES ? idx - L::STAGES : 0; i < idx; ++i)
+          mbar_wait_bounded(kv_full(i % L::STAGES), (i / L::STAGES) & 1, kPolls);
+      }
+      __syncwarp();
+     } else if (warp == 8) {
+      // ------------------------------------------------------------ matrix instructions
+      if (lane == 0 && start < key_tiles) {
+        constexpr uint32_t qk = instr_desc(kBM, kBN, BF16, false), pv = instr_desc(kBM, DP, BF16, true);
+        int done[2] = {0, 0};  // tiles whose P V has been issued
+        auto scores = [&](int t, int stage) {
+          const uint32_t qa = base + t * L::BYTES, ka = base + (2 + stage) * L::BYTES;
+#pragma unroll
+          for (int k = 0; k < DP / 16; ++k) {
+            const uint32_t off = (k / 4) * L::PANEL + (k % 4) * 32;
+            tc_mma_ss(tmem + t * 128, smem_desc(qa + off, 16, 1024), smem_desc(ka + off, 16, 1024), qk, k > 0);
+          }
+          tc_commit(s_full(t));
+        };
+        auto values = [&](int t, int stage) {
+          const uint32_t va = base + (2 + stage) * L::BYTES;
+#pragma unroll
+          for (int k = 0; k < kBN / 16; ++k)
+            tc_mma_ts(tmem + 256 + t * 128, tmem + t * 128 + k * 8, smem_desc(va + k * 2048, L::PANEL, 1024), pv,
+                      done[t] > 0 || k > 0);
+          tc_commit(o_full(t));
+          ++done[t];
+        };
+        int idx = 0;  // ring position of K of tile j
+        int last = -1;  // ring position of the last V
+        bool q_in[2] = {false, false};
+        auto query = [&](int t) {
+          if (!q_in[t]) {
+            wait(q_full(t), 0);
+            q_in[t] = true;
+          }
+        };
+        wait(kv_full(0), 0);
+        for (int t = 0; t < 2 && ok; ++t)
+          if (need(t, start)) {
+            query(t);
+            if (ok) scores(t, 0);
+          }
+        tc_commit(kv_empty(0));
+        for (int j = start; j < key_tiles && ok;) {
+          const int jn = next(j), iv = idx + 1, ik = idx + 2;
+          const int sv = iv % L::STAGES, sk = ik % L::STAGES;
+          wait(kv_full(sv), (iv / L::STAGES) & 1);
+          for (int t = 0; t < 2 && ok; ++t) {
+            if (need(t, j)) {
+              if (!wait(p_full(t), done[t] & 1)) break;
+              tc_fence_after();
+              values(t, sv);
+            }
+            if (t == 1) tc_commit(kv_empty(sv));
+            if (jn < key_tiles) {
+              if (t == 0) wait(kv_full(sk), (ik / L::STAGES) & 1);
+              if (need(t, jn)) {
+                query(t);
+                if (ok) scores(t, sk);
+              }
+              if (t == 1) tc_commit(kv_empty(sk));
+            }
+          }
+          last = iv;
+          j = jn;
+          idx += 2;
+        }
+        // the last arrival that the matrix unit owes a barrier of this CTA
+        if (last >= 0) wait(kv_empty(last % L::STAGES), (last / L::STAGES) & 1);
+      }
+      __syncwarp();
+     }
+    } else {
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+      // ------------------------------------------------------------ softmax: a thread per query row
+      const int t = warp >> 2, r = t * kBM + (warp & 3) * 32 + lane;  // row of the pair
+      const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+      const uint32_t s_at = tmem + lanes + t * 128, o_at = tmem + lanes + 256 + t * 128;
+      const bool active = rows > t * kBM;
+      if (active) {
+        auto wait_all = [&](uint32_t bar, uint32_t parity) {  // the same answer for the whole warp
+          ok = __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, kPolls));
+          return ok;
+        };
+        const bool mine = r < rows;
+        const int p = (int)(row0 - doc.q0) + r + doc.shift;
+        const Sight see = sight_of(a, doc, p);
+        const float slope = a.slopes ? a.slopes[h] : 0.f;
+        // GENERAL: scores become log2 units at once; else they stay products and c is applied in the exponent
+        const float c = GENERAL ? 1.f : a.scale * kLog2e;
+        const float inv_cap = a.softcap > 0.f ? a.scale / a.softcap : 0.f;
+        float m = -INFINITY, l = 0.f;
+        int done = 0;
+        for (int j = next(-1); j < key_tiles; j = next(j)) {
+          if (!need(t, j)) continue;
+          if (!wait_all(s_full(t), done & 1)) break;
+          tc_fence_after();
+          uint32_t u[128];
+          float* s = reinterpret_cast<float*>(u);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) tmem_ld32(s_at + i * 32, u + i * 32);
+          tmem_wait_ld();
+          const int k0 = j * kBN;
+          if constexpr (GENERAL) {
+            if (a.softcap > 0.f) {
+#pragma unroll
+              for (int i = 0; i < 128; ++i) s[i] = a.softcap * kLog2e * tanhf(s[i] * inv_cap);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 128; ++i) s[i] *= a.scale * kLog2e;
+            }
+            if (a.slopes) {
+#pragma unroll
+              for (int i = 0; i < 128; ++i) s[i] = fmaf(-slope * kLog2e, fabsf((float)(p - k0 - i)), s[i]);
+            }
+          }
+          // the mask, where it cuts this tile for some row of the warp
+          const bool whole = k0 + kBN <= doc.prefix || (k0 >= see.lo && k0 + kBN <= see.hi);
+          if (!__all_sync(0xffffffffu, whole)) {
+#pragma unroll
+            for (int i = 0; i < 128; ++i)
+              if (!(k0 + i < doc.prefix || (k0 + i >= see.lo && k0 + i < see.hi))) s[i] = -INFINITY;
+          }
+          float top[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+          for (int i = 4; i < 128; ++i) top[i & 3] = fmaxf(top[i & 3], s[i]);
+          const float mt = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+          // the maximum moves when it has grown by 2^8: sums are in float32 and p stays below 2^8
+          const bool grow = (mt - m) * c > 8.f;
+          if (__any_sync(0xffffffffu, grow)) {
+            const float m_new = grow ? mt : m;
+            const float back = grow ? (m == -INFINITY ? 0.f : ex2((m - m_new) * c)) : 1.f;
+            m = m_new;
+            l *= back;
+            if (done > 0) {
+              if (!wait_all(o_full(t), (done - 1) & 1)) break;
+              tc_fence_after();
+#pragma unroll
+              for (int i = 0; i < DP / 32; ++i) {
+                uint32_t o[32];
+                tmem_ld32(o_at + i * 32, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * back);
+                tmem_st32(o_at + i * 32, o);
+              }
+              tmem_wait_st();
+            }
+          }
+          const float mc = m == -INFINITY ? 0.f : m * c;
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int i = 0; i < 128; ++i) {
+            s[i] = ex2(fmaf(s[i], c, -mc));
+            sum[i & 3] += s[i];
+          }
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          uint32_t q[64];
+#pragma unroll
+          for (int i = 0; i < 64; ++i) q[i] = pack16<BF16>(s[2 * i], s[2 * i + 1]);
+          tmem_st32(s_at, q);
+          tmem_st32(s_at + 32, q + 32);
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(p_full(t));
+          ++done;
+        }
+        // ---------------------------------------------------------- output
+        if (ok && done > 0) wait_all(o_full(t), (done - 1) & 1);
+        tc_fence_after();
+        if (ok) {
+          const float inv = l == 0.f ? 0.f : 1.f / l;
+          T* out = static_cast<T*>(a.out) + (row0 + r) * a.out_tok_stride + (int64_t)h * a.out_head_stride;
+          float odd = 0.f;  // becomes NaN if a column is not finite
+#pragma unroll
+          for (int i = 0; i < DP / 32; ++i) {
+            uint32_t o[32];
+            if (done > 0) {
+              tmem_ld32(o_at + i * 32, o);
+              tmem_wait_ld();
+            }
+            if (l == 0.f) {
+#pragma unroll
+              for (int x = 0; x < 32; ++x) o[x] = 0;
+            }
+#pragma unroll
+            for (int x = 0; x < 32; x += 8) {
+              Vec<T, 8> v;
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const float y = __uint_as_float(o[x + e]) * inv;
+                odd = fmaf(y, 0.f, odd);
+                v.e[e] = from_f32<T>(y);
+              }
+              const int d = i * 32 + x;
+              if (mine && d < a.head_dim) *reinterpret_cast<Vec<T, 8>*>(out + d) = v;
+            }
+          }
+          if (mine && a.lse)
+            a.lse[(row0 + r) * a.lse_tok_stride + h] =
+                l == 0.f ? -INFINITY : ((m == -INFINITY ? 0.f : m * c) + log2f(l)) * kLn2;
+          // rows that are not finite, again from the definition (their tile of Q is no longer needed)
+          unsigned again = __ballot_sync(0xffffffffu, mine && !(odd == 0.f));
+          float* qs = reinterpret_cast<float*>(raw + (base - smem_u32(raw)) + t * L::BYTES + (warp & 3) * 1024);
+          while (again) {
+            const int who = __ffs(again) - 1;
+            again &= again - 1;
+            const int64_t row = row0 + t * kBM + (warp & 3) * 32 + who;
+            const int pw = __shfl_sync(0xffffffffu, p, who);
+            const Sight sw = sight_of(a, doc, pw);
+            const T* q = static_cast<const T*>(a.q) + row * a.q_tok_stride + (int64_t)h * a.q_head_stride;
+            __syncwarp();
+            for (int d = lane; d < a.head_dim; d += 32) qs[d] = to_f32(q[d]);
+            __syncwarp();
+            const T* k = static_cast<const T*>(a.k) + doc.k0 * a.k_tok_stride + (int64_t)hk * a.k_head_stride;
+            const T* v = static_cast<const T*>(a.v) + doc.k0 * a.v_tok_stride + (int64_t)hk * a.v_head_stride;
+            T* o = static_cast<T*>(a.out) + row * a.out_tok_stride + (int64_t)h * a.out_head_stride;
+            const float lse = attend_row<T>(
+                qs, a.head_dim, RowScore{a.scale, a.softcap, -slope}, 1.f, 0, doc.n,
+                [&](int x) { return !(x < doc.prefix || (x >= sw.lo && x < sw.hi)); },
+                [&](int x) { return k + x * a.k_tok_stride; }, [&](int x) { return v + x * a.v_tok_stride; },
+                [&](int x) { return fabsf((float)(pw - x)); }, [&](int d, float x) { o[d] = from_f32<T>(x); });
+            if (a.lse && lane == 0) a.lse[row * a.lse_tok_stride + h] = lse;
+          }
+        }
+      }
+    }
+    if (!ok && lane == 0) raise_status(a.status, OC_STATUS_TIMEOUT);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) tmem_free(tmem, 512);
+}
+
+// ------------------------------------------------------------------ any type, any alignment
 // One warp per (query row, head).
 template <typename T>
 __global__ void __launch_bounds__(32) prompt_row_kernel(const oc_prompt_args a) {
@@ -28,35 +495,111 @@ __global__ void __launch_bounds__(32) prompt_row_kernel(const oc_prompt_args a) 
   const T* q = static_cast<const T*>(a.q) + t * a.q_tok_stride + h * a.q_head_stride;
   for (int d = lane; d < a.head_dim; d += 32) qs[d] = to_f32(q[d]);
   __syncwarp();
-  const int doc = a.cu_q ? find_doc(a.cu_q, a.docs, t) : 0;
-  int64_t k0 = 0;
-  int n = 0, pos = 0, prefix = 0;
-  if (doc >= 0) {
-    const int64_t q0 = a.cu_q ? a.cu_q[doc] : 0, q1 = a.cu_q ? a.cu_q[doc + 1] : a.tokens;
-    k0 = a.cu_q ? a.cu_k[doc] : 0;
-    int64_t k1 = a.cu_q ? a.cu_k[doc + 1] : a.key_tokens;
-    if (k0 < 0 || k1 < k0 || k1 > a.key_tokens) {
-      if (lane == 0) raise_status(a.status, OC_STATUS_POSITION);
-      k0 = k1 = 0;
+  // the document of the row: binary search
+  int lo = -1, hi = a.docs;
+  if (!a.cu_q) lo = 0;
+  else if (t >= a.cu_q[0]) {
+    lo = 0;
+    hi = a.docs + 1;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (a.cu_q[mid] <= t) lo = mid;
+      else hi = mid;
     }
-    n = (int)(k1 - k0);
-    pos = (int)(t - q0 + n - (q1 - q0));
-    prefix = a.prefix_lens ? a.prefix_lens[doc] : 0;
   }
-  const T* k = static_cast<const T*>(a.k) + k0 * a.k_tok_stride + hk * a.k_head_stride;
-  const T* v = static_cast<const T*>(a.v) + k0 * a.v_tok_stride + hk * a.v_head_stride;
+  const Doc doc = get_doc(a, lo);
+  const int p = (int)(t - doc.q0) + doc.shift;
+  const Sight see = sight_of(a, doc, p);
+  const T* k = static_cast<const T*>(a.k) + doc.k0 * a.k_tok_stride + hk * a.k_head_stride;
+  const T* v = static_cast<const T*>(a.v) + doc.k0 * a.v_tok_stride + hk * a.v_head_stride;
   T* out = static_cast<T*>(a.out) + t * a.out_tok_stride + h * a.out_head_stride;
   const float lse = attend_row<T>(
-      qs, a.head_dim, RowScore{a.scale, a.softcap, a.slopes ? -a.slopes[h] : 0.f}, 1.f, 0, n,
-      [&](int j) { return !(j < prefix || ((j <= pos || !a.causal) && (a.window == 0 || j > pos - a.window))); },
+      qs, a.head_dim, RowScore{a.scale, a.softcap, a.slopes ? -a.slopes[h] : 0.f}, 1.f, 0, doc.n,
+      [&](int j) { return !(j < doc.prefix || (j >= see.lo && j < see.hi)); },
       [&](int j) { return k + j * a.k_tok_stride; }, [&](int j) { return v + j * a.v_tok_stride; },
-      [&](int j) { return fabsf((float)(pos - j)); }, [&](int d, float x) { out[d] = from_f32<T>(x); });
+      [&](int j) { return fabsf((float)(p - j)); }, [&](int d, float x) { out[d] = from_f32<T>(x); });
   if (a.lse && lane == 0) a.lse[t * a.lse_tok_stride + h] = lse;
 }
 
 template <typename T>
 int launch_rows(const oc_prompt_args& a, void* stream) {
   return launch_pdl(prompt_row_kernel<T>, dim3((unsigned)a.tokens, (unsigned)(a.kv_heads * a.group)), 32, 0, stream, a);
+}
+
+// ------------------------------------------------------------------ host side
+PFN_cuTensorMapEncodeTiled_v12000 map_encoder() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+  });
+  return fn;
+}
+
+// A (rows, heads, head_dim) tensor of 16-bit elements as boxes of 128 rows of 64 columns of one head.
+bool encode(CUtensorMap* map, int& swap, const void* base, int dtype, int head_dim, int64_t rows, int heads,
+            int64_t tok_stride, int64_t head_stride) {
+  const auto enc = map_encoder();
+  if (!enc || !aligned_to(base, 16) || rows < 1) return false;
+  const int64_t row_bytes = (int64_t)head_dim * 2;
+  int64_t size[2] = {heads, rows}, stride[2] = {head_stride * 2, tok_stride * 2};
+  // dimensions by increasing stride; the stride of a single entry is free
+  swap = size[0] == 1 || (size[1] > 1 && stride[1] < stride[0]);
+  cuuint64_t dim[3] = {(cuuint64_t)head_dim}, bytes[2];
+  cuuint32_t box[3] = {64}, step[3] = {1, 1, 1};
+  int64_t nest = (row_bytes + 15) / 16 * 16;
+  for (int i = 0; i < 2; ++i) {
+    const int r = swap ? 1 - i : i;
+    int64_t b = stride[r];
+    if (size[r] == 1) b = nest;
+    if (b < nest || b % 16) return false;
+    dim[i + 1] = (cuuint64_t)size[r];
+    bytes[i] = (cuuint64_t)b;
+    box[i + 1] = r == 1 ? kBN : 1;
+    nest = size[r] == 1 ? nest : b;
+  }
+  return enc(map, dtype == OC_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+             const_cast<void*>(base), dim, bytes, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int DP, bool GENERAL>
+int launch_tiled(const oc_prompt_args& a, const Maps& maps, unsigned tiles, void* stream) {
+  auto kernel = prompt_kernel<T, DP, GENERAL>;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<DP>::SMEM) != cudaSuccess) {
+    cudaGetLastError();
+    return OC_ERR_CUDA;
+  }
+  return launch_pdl(kernel, dim3(tiles, (unsigned)(a.kv_heads * a.group)), dim3(kThreads), Tile<DP>::SMEM, stream, a,
+                    maps);
+}
+
+template <typename T>
+int launch(const oc_prompt_args& a, void* stream) {
+  Maps maps;
+  const int es_ok = a.head_dim % 8 == 0 && a.head_dim <= 128 && aligned_to(a.out, 16) && a.out_tok_stride % 8 == 0 &&
+                    a.out_head_stride % 8 == 0;
+  if (!es_ok ||
+      !encode(&maps.q, maps.q_swap, a.q, a.dtype, a.head_dim, a.tokens, a.kv_heads * a.group, a.q_tok_stride,
+              a.q_head_stride) ||
+      !encode(&maps.k, maps.k_swap, a.k, a.dtype, a.head_dim, a.key_tokens, a.kv_heads, a.k_tok_stride,
+              a.k_head_stride) ||
+      !encode(&maps.v, maps.v_swap, a.v, a.dtype, a.head_dim, a.key_tokens, a.kv_heads, a.v_tok_stride,
+              a.v_head_stride))
+    return launch_rows<T>(a, stream);
+  // pairs of query tiles: the documents' lengths are on the device, so an upper bound; the rest leave at once
+  const int64_t tiles = a.tokens / (2 * kBM) + (a.cu_q ? a.docs + 2 : 1);
+  if (tiles > 0x7fffffff) return OC_ERR_TOO_LARGE;
+  const bool general = a.softcap > 0.f || a.slopes || !(a.scale > 0.f);
+  if (a.head_dim <= 64)
+    return general ? launch_tiled<T, 64, true>(a, maps, (unsigned)tiles, stream)
+                   : launch_tiled<T, 64, false>(a, maps, (unsigned)tiles, stream);
+  return general ? launch_tiled<T, 128, true>(a, maps, (unsigned)tiles, stream)
+                 : launch_tiled<T, 128, false>(a, maps, (unsigned)tiles, stream);
 }
 
 }  // namespace
@@ -69,12 +612,12 @@ extern "C" int oc_prompt_attention(const oc_prompt_args* args, void* stream) {
     return OC_ERR_INVALID;
   if (a.tokens == 0) return OC_OK;
   if (!a.q || !a.out || (a.cu_q && !a.cu_k) || (a.key_tokens && (!a.k || !a.v))) return OC_ERR_INVALID;
-  if (a.tokens > 0x7fffffff || a.key_tokens > 0x7fffffff) return OC_ERR_TOO_LARGE;
+  if (a.tokens > 0x7fffff00 || a.key_tokens > 0x7fffff00) return OC_ERR_TOO_LARGE;
   if (a.head_dim > kRowMaxDim) return OC_ERR_UNSUPPORTED;
   switch (a.dtype) {
     case OC_F32: return launch_rows<float>(a, stream);
-    case OC_F16: return launch_rows<__half>(a, stream);
-    case OC_BF16: return launch_rows<__nv_bfloat16>(a, stream);
+    case OC_F16: return launch<__half>(a, stream);
+    case OC_BF16: return launch<__nv_bfloat16>(a, stream);
     default: return OC_ERR_UNSUPPORTED;
   }
 }
