@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int y = __shfl_up_sync(0xffffffffu, up, o);
         if (lane >= o) up += y;
       }
-      const int at = (int)blockIdx.x - before - (up - n);
+      const int at = (int)blockIdx.y - before - (up - n);
       const unsigned hit = __ballot_sync(0xffffffffu, at >= 0 && at < n);
       if (hit) {
         const int who = __ffs(hit) - 1;
@@ -190,22 +190,30 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int pair = s_tile;
   if (pair >= 0) {
     const Doc doc = s_doc;
-    const int h = blockIdx.y, hk = h / a.group;
+    const int h = blockIdx.x, hk = h / a.group;
     const int64_t row0 = doc.q0 + (int64_t)pair * 2 * kBM;  // first query row of tile 0
     const int rows = (int)min((int64_t)2 * kBM, doc.q1 - row0);
     const int key_tiles = (doc.n + kBN - 1) / kBN;
-    // whether any query of tile t sees a key of key tile j
+    // key tiles that some query of tile t sees: [lo, hi) of t, and those below `shared` (the prefix)
+    const int shared = (doc.prefix + kBN - 1) / kBN;
+    int from[2] = {key_tiles, key_tiles}, to[2] = {0, 0};
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int n = min(kBM, rows - t * kBM), p = (int)(row0 - doc.q0) + t * kBM + doc.shift;
+      const Sight first = sight_of(a, doc, p), last = sight_of(a, doc, p + n - 1);
+      if (n > 0 && last.hi > first.lo) {
+        from[t] = first.lo / kBN;
+        to[t] = (last.hi + kBN - 1) / kBN;
+      }
+    }
+    const int from_any = min(from[0], from[1]), to_any = max(to[0], to[1]);
     auto need = [&](int t, int j) {
-      const int r = min(kBM, rows - t * kBM);
-      if (r <= 0) return false;
-      const int p = (int)(row0 - doc.q0) + t * kBM + doc.shift;
-      const Sight first = sight_of(a, doc, p), last = sight_of(a, doc, p + r - 1);
-      return j * kBN < doc.prefix || (j * kBN < last.hi && (j + 1) * kBN > first.lo);
+      return (j < shared && rows > t * kBM) || (j >= (t ? from[1] : from[0]) && j < (t ? to[1] : to[0]));
     };
-    auto next = [&](int j) {
-      for (++j; j < key_tiles; ++j)
-        if (need(0, j) || need(1, j)) break;
-      return j;
+    auto next = [&](int j) {  // the next key tile that one of the two needs
+      ++j;
+      if (j >= shared && j < from_any) j = from_any;
+      return j < shared || j < to_any ? j : key_tiles;
     };
     const int start = next(-1);
     bool ok = true;
@@ -214,9 +222,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       return ok;
     };
 
-    // registers: 8 warps x 32 x 216 + 4 x 32 x 72 = 384 x 168, what the CTA was launched with
+    // registers: 8 warps x 32 x 208 + 4 x 32 x 88 = 384 x 168, what the CTA was launched with
     if (warp >= 8) {
-     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
      if (warp == 9) {
       // ------------------------------------------------------------ copies
       if (lane == 0) {
@@ -321,7 +329,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
      }
     } else {
-      asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
       // ------------------------------------------------------------ softmax: a thread per query row
       const int t = warp >> 2, r = t * kBM + (warp & 3) * 32 + lane;  // row of the pair
       const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
@@ -373,8 +381,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           float top[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-          for (int i = 4; i < 128; ++i) top[i & 3] = fmaxf(top[i & 3], s[i]);
-          const float mt = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+          for (int i = 4; i + 1 < 128; i += 2) top[(i >> 1) & 3] = max3(top[(i >> 1) & 3], s[i], s[i + 1]);
+          const float mt = max3(fmaxf(top[0], top[1]), top[2], top[3]);
           // the maximum moves when it has grown by 2^8: sums are in float32 and p stays below 2^8
           const bool grow = (mt - m) * c > 8.f;
           if (__any_sync(0xffffffffu, grow)) {
@@ -398,18 +406,23 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
           const float mc = m == -INFINITY ? 0.f : m * c;
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+          const float2 c2 = {c, c}, mc2 = {-mc, -mc};
+          float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
 #pragma unroll
-          for (int i = 0; i < 128; ++i) {
-            s[i] = ex2(fmaf(s[i], c, -mc));
-            sum[i & 3] += s[i];
+          for (int x = 0; x < 4; ++x) {  // 32 keys at a time: P goes out while the next are computed
+            uint32_t q[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              float2 e = fma2(float2{s[x * 32 + 2 * i], s[x * 32 + 2 * i + 1]}, c2, mc2);
+              e.x = ex2(e.x);
+              e.y = ex2(e.y);
+              sum[i & 1] = add2(sum[i & 1], e);
+              q[i] = pack16<BF16>(e.x, e.y);
+            }
+            tmem_st16(s_at + x * 16, q);
           }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-          uint32_t q[64];
-#pragma unroll
-          for (int i = 0; i < 64; ++i) q[i] = pack16<BF16>(s[2 * i], s[2 * i + 1]);
-          tmem_st32(s_at, q);
-          tmem_st32(s_at + 32, q + 32);
+          sum[0] = add2(sum[0], sum[1]);
+          l += sum[0].x + sum[0].y;
           tmem_wait_st();
           tc_fence_before();
           __syncwarp();
@@ -574,7 +587,7 @@ int launch_tiled(const oc_prompt_args& a, const Maps& maps, unsigned tiles, void
     cudaGetLastError();
     return OC_ERR_CUDA;
   }
-  return launch_pdl(kernel, dim3(tiles, (unsigned)(a.kv_heads * a.group)), dim3(kThreads), Tile<DP>::SMEM, stream, a,
+  return launch_pdl(kernel, dim3((unsigned)(a.kv_heads * a.group), tiles), dim3(kThreads), Tile<DP>::SMEM, stream, a,
                     maps);
 }
 
@@ -593,7 +606,7 @@ int launch(const oc_prompt_args& a, void* stream) {
     return launch_rows<T>(a, stream);
   // pairs of query tiles: the documents' lengths are on the device, so an upper bound; the rest leave at once
   const int64_t tiles = a.tokens / (2 * kBM) + (a.cu_q ? a.docs + 2 : 1);
-  if (tiles > 0x7fffffff) return OC_ERR_TOO_LARGE;
+  if (tiles > 65535) return OC_ERR_TOO_LARGE;
   const bool general = a.softcap > 0.f || a.slopes || !(a.scale > 0.f);
   if (a.head_dim <= 64)
     return general ? launch_tiled<T, 64, true>(a, maps, (unsigned)tiles, stream)
