@@ -127,7 +127,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ Doc s_doc;
   __shared__ int s_tile;  // which pair of query tiles of the document; -1: none
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
   const uint32_t bar0 = smem_u32(bars);
   auto kv_full = [&](int s) { return bar0 + 8 * s; };
@@ -186,10 +186,17 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = tmem_at;
-  const int pair = s_tile;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_at, 0);
+  const int pair = __shfl_sync(0xffffffffu, s_tile, 0);
   if (pair >= 0) {
-    const Doc doc = s_doc;
+    // through a shuffle: warp-uniform for the compiler, so that the matrix warp works in uniform registers
+    Doc doc;
+    doc.q0 = __shfl_sync(0xffffffffu, s_doc.q0, 0);
+    doc.q1 = __shfl_sync(0xffffffffu, s_doc.q1, 0);
+    doc.k0 = __shfl_sync(0xffffffffu, s_doc.k0, 0);
+    doc.n = __shfl_sync(0xffffffffu, s_doc.n, 0);
+    doc.shift = __shfl_sync(0xffffffffu, s_doc.shift, 0);
+    doc.prefix = __shfl_sync(0xffffffffu, s_doc.prefix, 0);
     const int h = blockIdx.x, hk = h / a.group;
     const int64_t row0 = doc.q0 + (int64_t)pair * 2 * kBM;  // first query row of tile 0
     const int rows = (int)min((int64_t)2 * kBM, doc.q1 - row0);
@@ -219,6 +226,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     auto wait = [&](uint32_t bar, uint32_t parity) {
       if (ok) ok = mbar_wait_bounded(bar, parity, kPolls);
+      return ok;
+    };
+
+    auto wait_all = [&](uint32_t bar, uint32_t parity) {  // the same answer for the whole warp
+      ok = __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, kPolls));
       return ok;
     };
 
@@ -262,69 +274,73 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
      } else if (warp == 8) {
       // ------------------------------------------------------------ matrix instructions
-      if (lane == 0 && start < key_tiles) {
+      if (start < key_tiles) {
         constexpr uint32_t qk = instr_desc(kBM, kBN, BF16, false), pv = instr_desc(kBM, DP, BF16, true);
+        constexpr uint32_t hi = smem_desc_hi(1024);
+        const bool one = elect_one();
+        const uint32_t q_lo = smem_desc_lo(base, 16), k_lo = smem_desc_lo(base + 2 * L::BYTES, 16),
+                       v_lo = smem_desc_lo(base + 2 * L::BYTES, L::PANEL);
         int done[2] = {0, 0};  // tiles whose P V has been issued
         auto scores = [&](int t, int stage) {
-          const uint32_t qa = base + t * L::BYTES, ka = base + (2 + stage) * L::BYTES;
+          if (one) {
+            const uint32_t qa = q_lo + t * (L::BYTES >> 4), ka = k_lo + stage * (L::BYTES >> 4);
 #pragma unroll
-          for (int k = 0; k < DP / 16; ++k) {
-            const uint32_t off = (k / 4) * L::PANEL + (k % 4) * 32;
-            tc_mma_ss(tmem + t * 128, smem_desc(qa + off, 16, 1024), smem_desc(ka + off, 16, 1024), qk, k > 0);
+            for (int k = 0; k < DP / 16; ++k) {
+              const uint32_t off = ((k / 4) * L::PANEL + (k % 4) * 32) >> 4;
+              tc_mma_ss(tmem + t * 128, qa + off, ka + off, hi, qk, k > 0);
+            }
+            tc_commit(s_full(t));
           }
-          tc_commit(s_full(t));
         };
         auto values = [&](int t, int stage) {
-          const uint32_t va = base + (2 + stage) * L::BYTES;
+          if (one) {
+            const uint32_t va = v_lo + stage * (L::BYTES >> 4);
 #pragma unroll
-          for (int k = 0; k < kBN / 16; ++k)
-            tc_mma_ts(tmem + 256 + t * 128, tmem + t * 128 + k * 8, smem_desc(va + k * 2048, L::PANEL, 1024), pv,
-                      done[t] > 0 || k > 0);
-          tc_commit(o_full(t));
+            for (int k = 0; k < kBN / 16; ++k)
+              tc_mma_ts(tmem + 256 + t * 128, tmem + t * 128 + k * 8, va + ((k * 2048) >> 4), hi, pv,
+                        done[t] > 0 || k > 0);
+            tc_commit(o_full(t));
+          }
           ++done[t];
         };
-        int idx = 0;  // ring position of K of tile j
-        int last = -1;  // ring position of the last V
-        bool q_in[2] = {false, false};
-        auto query = [&](int t) {
-          if (!q_in[t]) {
-            wait(q_full(t), 0);
-            q_in[t] = true;
-          }
+        auto free_stage = [&](int stage) {
+          if (one) tc_commit(kv_empty(stage));
         };
-        wait(kv_full(0), 0);
-        for (int t = 0; t < 2 && ok; ++t)
-          if (need(t, start)) {
-            query(t);
-            if (ok) scores(t, 0);
-          }
-        tc_commit(kv_empty(0));
+        wait_all(kv_full(0), 0);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          if (ok && rows > t * kBM && wait_all(q_full(t), 0) && need(t, start)) scores(t, 0);
+        free_stage(0);
+        int last = -1, sv = 1, sk = 2;         // stage of the last V; of V(j), of K(next j)
+        uint32_t ring = 0;                     // bit s: the phase of stage s that completes next
+        ring ^= 1u;
         for (int j = start; j < key_tiles && ok;) {
-          const int jn = next(j), iv = idx + 1, ik = idx + 2;
-          const int sv = iv % L::STAGES, sk = ik % L::STAGES;
-          wait(kv_full(sv), (iv / L::STAGES) & 1);
-          for (int t = 0; t < 2 && ok; ++t) {
-            if (need(t, j)) {
-              if (!wait(p_full(t), done[t] & 1)) break;
+          const int jn = next(j);
+          wait_all(kv_full(sv), ring >> sv & 1);
+          ring ^= 1u << sv;
+          if (jn < key_tiles) {
+            wait_all(kv_full(sk), ring >> sk & 1);
+            ring ^= 1u << sk;
+          }
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (ok && need(t, j) && wait_all(p_full(t), done[t] & 1)) {
               tc_fence_after();
               values(t, sv);
             }
-            if (t == 1) tc_commit(kv_empty(sv));
+            if (t == 1) free_stage(sv);
             if (jn < key_tiles) {
-              if (t == 0) wait(kv_full(sk), (ik / L::STAGES) & 1);
-              if (need(t, jn)) {
-                query(t);
-                if (ok) scores(t, sk);
-              }
-              if (t == 1) tc_commit(kv_empty(sk));
+              if (ok && need(t, jn)) scores(t, sk);
+              if (t == 1) free_stage(sk);
             }
           }
-          last = iv;
+          last = sv;
+          sv = sk + 1 == L::STAGES ? 0 : sk + 1;
+          sk = sv + 1 == L::STAGES ? 0 : sv + 1;
           j = jn;
-          idx += 2;
         }
-        // the last arrival that the matrix unit owes a barrier of this CTA
-        if (last >= 0) wait(kv_empty(last % L::STAGES), (last / L::STAGES) & 1);
+        // the last arrival that the matrix unit owes a barrier of this CTA: its phase is the one that V filled
+        if (ok && last >= 0) wait_all(kv_empty(last), (ring >> last & 1) ^ 1);
       }
       __syncwarp();
      }
@@ -336,10 +352,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t s_at = tmem + lanes + t * 128, o_at = tmem + lanes + 256 + t * 128;
       const bool active = rows > t * kBM;
       if (active) {
-        auto wait_all = [&](uint32_t bar, uint32_t parity) {  // the same answer for the whole warp
-          ok = __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, kPolls));
-          return ok;
-        };
         const bool mine = r < rows;
         const int p = (int)(row0 - doc.q0) + r + doc.shift;
         const Sight see = sight_of(a, doc, p);

@@ -79,10 +79,11 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 // ------------------------------------------------------------------ descriptors
 // Shared-memory operand with the 128-byte swizzle.  group: bytes between
 // groups of 8 rows (of 8 k for an operand whose contiguous dimension is not
-// k); lead: bytes between its 64-element column blocks (that form only).
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lead, uint32_t group) {
-  return (uint64_t)((addr >> 4) & 0x3fff) | (uint64_t)((lead >> 4) & 0x3fff) << 16 |
-         (uint64_t)((group >> 4) & 0x3fff) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+// k); lead: bytes between its 64-element column blocks (that form only).  The
+// address sits in the low word, so that an operand's steps are 32-bit sums.
+__host__ __device__ constexpr uint32_t smem_desc_hi(uint32_t group) { return ((group >> 4) & 0x3fff) | 1u << 14 | 2u << 29; }
+__device__ __forceinline__ uint32_t smem_desc_lo(uint32_t addr, uint32_t lead) {
+  return ((addr >> 4) & 0x3fff) | ((lead >> 4) & 0x3fff) << 16;
 }
 // M x N x 16, both operands f16 or both bf16; b_mn: B's contiguous dimension is n.
 __host__ __device__ constexpr uint32_t instr_desc(int m, int n, bool bf16, bool b_mn) {
@@ -91,19 +92,28 @@ __host__ __device__ constexpr uint32_t instr_desc(int m, int n, bool bf16, bool 
 }
 
 // ------------------------------------------------------------------ matrix instructions (one thread)
+// One lane of a converged warp, the same one every time.  The rest of the
+// issuing warp's code stays warp-uniform: the operands are uniform registers.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t yes;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(yes));
+  return yes != 0;
+}
 // D (tensor memory) = A B^T + (accumulate ? D : 0)
-__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc,
+                                          bool accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d),
+      "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"((uint32_t)accumulate)
       : "memory");
 }
-__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t hi, uint32_t idesc,
+                                          bool accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 b, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b_lo), "r"(hi), "r"(idesc), "r"((uint32_t)accumulate)
       : "memory");
 }
 // Arrives on the mbarrier when every matrix instruction issued so far by this thread has completed.
