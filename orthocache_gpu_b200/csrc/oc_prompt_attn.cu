@@ -114,6 +114,42 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
   }
 }
 
+// k tanh(r x) of 128 scores.  |r x| <= 3/4 for the whole warp, the rule with
+// caps of some tens: x times an even polynomial, fitted to the smallest largest
+// absolute error (1e-8), on the multiply units; else 1 - 2 / (1 + 2^(2 x log2 e)), two
+// operations of the exponential unit a score (absolute error some 1e-7).
+__device__ __forceinline__ void cap_scores(float* s, float r, float k) {
+  float top = 0.f;
+#pragma unroll
+  for (int i = 0; i < 128; i += 2) {
+    const float2 q = mul2(float2{s[i], s[i + 1]}, float2{s[i], s[i + 1]});
+    top = max3(top, q.x, q.y);
+  }
+  if (__all_sync(0xffffffffu, top * r * r <= 0.5625f)) {
+    const float2 r2 = both(r), kr = both(k * r);
+#pragma unroll
+    for (int i = 0; i < 128; i += 2) {
+      const float2 v = {s[i], s[i + 1]}, x = mul2(v, r2), q = mul2(x, x);
+      float2 p = fma2(q, both(-0.0044934507459402084f), both(0.019237229600548744f));
+      p = fma2(q, p, both(-0.053149256855249405f));
+      p = fma2(q, p, both(0.13320580124855042f));
+      p = fma2(q, p, both(-0.33332470059394836f));
+      p = fma2(q, p, both(0.9999998211860657f));
+      p = mul2(p, mul2(v, kr));
+      s[i] = p.x;
+      s[i + 1] = p.y;
+    }
+  } else {
+    const float z = 2.f * kLog2e * r;
+#pragma unroll
+    for (int i = 0; i < 128; ++i) {
+      float y;
+      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(1.f + ex2(s[i] * z)));
+      s[i] = fmaf(-2.f * k, y, k);
+    }
+  }
+}
+
 // GENERAL: scores are capped, biased or scaled by a factor that is not
 // positive; else the scale is folded into the exponential.
 template <typename T, int DP, bool GENERAL>
@@ -122,7 +158,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   using L = Tile<DP>;
   constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
   extern __shared__ char raw[];
-  __shared__ __align__(8) uint64_t bars[2 * L::STAGES + 8];
+  __shared__ __align__(8) uint64_t bars[2 * L::STAGES + 10];
   __shared__ uint32_t tmem_at;
   __shared__ Doc s_doc;
   __shared__ int s_tile;  // which pair of query tiles of the document; -1: none
@@ -136,6 +172,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto s_full = [&](int t) { return bar0 + 8 * (2 * L::STAGES + 2 + t); };
   auto p_full = [&](int t) { return bar0 + 8 * (2 * L::STAGES + 4 + t); };
   auto o_full = [&](int t) { return bar0 + 8 * (2 * L::STAGES + 6 + t); };
+  auto p_most = [&](int t) { return bar0 + 8 * (2 * L::STAGES + 8 + t); };  // P of the tile's first 96 keys
 
   if (warp == 8 && lane == 0) {
     for (int s = 0; s < L::STAGES; ++s) {
@@ -146,6 +183,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(q_full(t), 1);
       mbar_init(s_full(t), 1);
       mbar_init(p_full(t), 4);
+      mbar_init(p_most(t), 4);
       mbar_init(o_full(t), 1);
     }
     mbar_init_fence();
@@ -292,13 +330,23 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc_commit(s_full(t));
           }
         };
+        // P V, of the first 96 keys as soon as their P is there
         auto values = [&](int t, int stage) {
+          const uint32_t va = v_lo + stage * (L::BYTES >> 4);
+          if (!wait_all(p_most(t), done[t] & 1)) return;
+          tc_fence_after();
           if (one) {
-            const uint32_t va = v_lo + stage * (L::BYTES >> 4);
 #pragma unroll
-            for (int k = 0; k < kBN / 16; ++k)
+            for (int k = 0; k < 6; ++k)
               tc_mma_ts(tmem + 256 + t * 128, tmem + t * 128 + k * 8, va + ((k * 2048) >> 4), hi, pv,
                         done[t] > 0 || k > 0);
+          }
+          if (!wait_all(p_full(t), done[t] & 1)) return;
+          tc_fence_after();
+          if (one) {
+#pragma unroll
+            for (int k = 6; k < 8; ++k)
+              tc_mma_ts(tmem + 256 + t * 128, tmem + t * 128 + k * 8, va + ((k * 2048) >> 4), hi, pv, true);
             tc_commit(o_full(t));
           }
           ++done[t];
@@ -311,35 +359,40 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int t = 0; t < 2; ++t)
           if (ok && rows > t * kBM && wait_all(q_full(t), 0) && need(t, start)) scores(t, 0);
         free_stage(0);
-        int last = -1, sv = 1, sk = 2;         // stage of the last V; of V(j), of K(next j)
-        uint32_t ring = 0;                     // bit s: the phase of stage s that completes next
-        ring ^= 1u;
+        // A wait, even for a barrier that has completed, takes some 200 cycles next to operands that stream from
+        // shared memory: those for copies are made one tile ahead, while the unit is busy.
+        int last = -1, sv = 1, sk = 2;  // stage of the last V; of V(j), of K(next j)
+        uint32_t ring = 1u;             // bit s: the phase of stage s that completes next
+        auto arrive = [&](int s) {
+          wait_all(kv_full(s), ring >> s & 1);
+          ring ^= 1u << s;
+        };
+        int jn = next(start);
+        arrive(sv);
+        if (jn < key_tiles) arrive(sk);
+        bool has[2] = {need(0, start), need(1, start)};
         for (int j = start; j < key_tiles && ok;) {
-          const int jn = next(j);
-          wait_all(kv_full(sv), ring >> sv & 1);
-          ring ^= 1u << sv;
-          if (jn < key_tiles) {
-            wait_all(kv_full(sk), ring >> sk & 1);
-            ring ^= 1u << sk;
-          }
-#pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            if (ok && need(t, j) && wait_all(p_full(t), done[t] & 1)) {
-              tc_fence_after();
-              values(t, sv);
-            }
-            if (t == 1) free_stage(sv);
-            if (jn < key_tiles) {
-              if (ok && need(t, jn)) scores(t, sk);
-              if (t == 1) free_stage(sk);
-            }
-          }
+          const bool more = jn < key_tiles;
+          const int jm = more ? next(jn) : key_tiles;
+          const int mv = sk + 1 == L::STAGES ? 0 : sk + 1, mk = mv + 1 == L::STAGES ? 0 : mv + 1;
+          const bool then[2] = {more && need(0, jn), more && need(1, jn)};
+          if (ok && has[0]) values(0, sv);
+          if (ok && then[0]) scores(0, sk);
+          if (more) arrive(mv);
+          if (jm < key_tiles) arrive(mk);
+          if (ok && has[1]) values(1, sv);
+          free_stage(sv);
+          if (ok && then[1]) scores(1, sk);
+          if (more) free_stage(sk);
           last = sv;
-          sv = sk + 1 == L::STAGES ? 0 : sk + 1;
-          sk = sv + 1 == L::STAGES ? 0 : sv + 1;
+          sv = mv;
+          sk = mk;
+          has[0] = then[0];
+          has[1] = then[1];
           j = jn;
+          jn = jm;
         }
-        // the last arrival that the matrix unit owes a barrier of this CTA: its phase is the one that V filled
+        // the last arrival that the matrix unit owes a barrier of this CTA: of the phase that V filled
         if (ok && last >= 0) wait_all(kv_empty(last), (ring >> last & 1) ^ 1);
       }
       __syncwarp();
@@ -355,11 +408,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool mine = r < rows;
         const int p = (int)(row0 - doc.q0) + r + doc.shift;
         const Sight see = sight_of(a, doc, p);
-        const float slope = a.slopes ? a.slopes[h] : 0.f;
+        const float slope = a.slopes ? a.slopes[h] : 0.f, slope2 = slope * kLog2e;
         // GENERAL: scores become log2 units at once; else they stay products and c is applied in the exponent
         const float c = GENERAL ? 1.f : a.scale * kLog2e;
         const float inv_cap = a.softcap > 0.f ? a.scale / a.softcap : 0.f;
         float m = -INFINITY, l = 0.f;
+        float odd = 0.f;  // becomes NaN if a score or a result is not finite
         int done = 0;
         for (int j = next(-1); j < key_tiles; j = next(j)) {
           if (!need(t, j)) continue;
@@ -371,17 +425,32 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int i = 0; i < 4; ++i) tmem_ld32(s_at + i * 32, u + i * 32);
           tmem_wait_ld();
           const int k0 = j * kBN;
+          float offset = 0.f;  // what the scores of this tile lack, the same for all of them
           if constexpr (GENERAL) {
             if (a.softcap > 0.f) {
-#pragma unroll
-              for (int i = 0; i < 128; ++i) s[i] = a.softcap * kLog2e * tanhf(s[i] * inv_cap);
+              cap_scores(s, inv_cap, a.softcap * kLog2e);
             } else {
 #pragma unroll
-              for (int i = 0; i < 128; ++i) s[i] *= a.scale * kLog2e;
+              for (int i = 0; i < 128; i += 2) {
+                const float2 v = mul2(float2{s[i], s[i + 1]}, both(a.scale * kLog2e));
+                s[i] = v.x;
+                s[i + 1] = v.y;
+              }
             }
             if (a.slopes) {
+              if (__all_sync(0xffffffffu, p >= k0 + kBN - 1)) {  // no key after the query: the bias is linear
+                offset = -slope2 * (float)(p - k0);
 #pragma unroll
-              for (int i = 0; i < 128; ++i) s[i] = fmaf(-slope * kLog2e, fabsf((float)(p - k0 - i)), s[i]);
+                for (int i = 0; i < 128; i += 2) {
+                  const float2 v = fma2(float2{(float)i, (float)(i + 1)}, both(slope2), float2{s[i], s[i + 1]});
+                  s[i] = v.x;
+                  s[i + 1] = v.y;
+                }
+              } else {
+                const float d0 = (float)(p - k0);
+#pragma unroll
+                for (int i = 0; i < 128; ++i) s[i] = fmaf(-slope2, fabsf(d0 - (float)i), s[i]);
+              }
             }
           }
           // the mask, where it cuts this tile for some row of the warp
@@ -394,7 +463,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           float top[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
           for (int i = 4; i + 1 < 128; i += 2) top[(i >> 1) & 3] = max3(top[(i >> 1) & 3], s[i], s[i + 1]);
-          const float mt = max3(fmaxf(top[0], top[1]), top[2], top[3]);
+          const float mt = max3(max3(top[0], top[1], top[2]), top[3], top[3]) + offset;
+          odd = mt != mt ? NAN : odd;
           // the maximum moves when it has grown by 2^8: sums are in float32 and p stays below 2^8
           const bool grow = (mt - m) * c > 8.f;
           if (__any_sync(0xffffffffu, grow)) {
@@ -418,10 +488,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
           const float mc = m == -INFINITY ? 0.f : m * c;
-          const float2 c2 = {c, c}, mc2 = {-mc, -mc};
+          const float2 c2 = both(c), mc2 = both(offset - mc);
           float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {  // 32 keys at a time: P goes out while the next are computed
+          // 32 keys at a time: P goes out while the next are computed
+          auto weigh = [&](int x) {
             uint32_t q[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
@@ -432,13 +502,20 @@ __global__ void __launch_bounds__(kThreads, 1)
               q[i] = pack16<BF16>(e.x, e.y);
             }
             tmem_st16(s_at + x * 16, q);
-          }
+          };
+          auto hand_over = [&](uint32_t bar) {
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar);
+          };
+#pragma unroll
+          for (int x = 0; x < 3; ++x) weigh(x);
+          hand_over(p_most(t));
+          weigh(3);
+          hand_over(p_full(t));
           sum[0] = add2(sum[0], sum[1]);
           l += sum[0].x + sum[0].y;
-          tmem_wait_st();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(p_full(t));
           ++done;
         }
         // ---------------------------------------------------------- output
@@ -447,7 +524,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (ok) {
           const float inv = l == 0.f ? 0.f : 1.f / l;
           T* out = static_cast<T*>(a.out) + (row0 + r) * a.out_tok_stride + (int64_t)h * a.out_head_stride;
-          float odd = 0.f;  // becomes NaN if a column is not finite
 #pragma unroll
           for (int i = 0; i < DP / 32; ++i) {
             uint32_t o[32];
