@@ -37,6 +37,7 @@ using namespace oc;
 constexpr int kWarps = 4;
 constexpr int kBufs = 3;         // buffers of a warp's ring
 constexpr int kMinShare = 4;     // tiles that a CTA takes at least before a unit is split
+constexpr int kUnitCost = 3;     // what beginning and ending a unit costs, in tiles, when shares are equalised
 constexpr int kDirectTiles = 8;  // units of at most so many tiles get a CTA each and no joining launch
 constexpr uint32_t kPolls = 1u << 22;  // bound of a wait for a copy
 
@@ -73,6 +74,12 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// 1 - 2 / (1 + e^2x): absolute error some 1e-7
+__device__ __forceinline__ float tanh_of(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(1.f + ex2(x * (2.f * kLog2e))));
+  return fmaf(-2.f, y, 1.f);
 }
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
@@ -137,26 +144,32 @@ __device__ __forceinline__ int scan128(int v, int& total, int* part) {
   return before + x - v;
 }
 
-// Walks the tiles of the batch in order: sequence, then unit, then tile.
+// Walks the tiles of the batch in order: sequence, then unit, then tile.  `at`
+// is the tile's place when each unit takes its tiles and kUnitCost.
 template <typename S>
 struct Walk {
-  int seq, sub, tile, tiles;
+  int seq, sub, tile, tiles, at;
   Span span;
   __device__ __forceinline__ void enter(const oc_paged_decode_args& a) {
     span = span_of(a, seq);
     tiles = tiles_of<S>(span);
   }
-  __device__ __forceinline__ void next(const oc_paged_decode_args& a, int subs) {
-    if (++tile < tiles) return;
+  __device__ __forceinline__ void next_unit(const oc_paged_decode_args& a, int subs) {
     tile = 0;
     if (++sub < subs) return;
     sub = 0;
     if (++seq < a.num_seqs) enter(a);
   }
+  __device__ __forceinline__ void next(const oc_paged_decode_args& a, int subs) {
+    ++at;
+    if (++tile < tiles) return;
+    at += kUnitCost;
+    next_unit(a, subs);
+  }
 };
 
-// Workspace: header (tiles before each sequence, and in all, then the run
-// length), then per CTA two states of 8 NT heads: acc, m, l.
+// Workspace: header (the place before each sequence, and after all, then the
+// run length), then per CTA two states of 8 NT heads: acc, m, l.
 struct Space {
   int32_t* before;  // num_seqs + 1, then the run length
   float* states;
@@ -204,19 +217,19 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<sizeof(C), DP, NT>::PER_SM)
 
   // ---------------------------------------------------------------- this CTA's run of tiles
   Walk<S> cs;
-  int count;
-  int64_t start = 0;
+  int end;  // the run goes up to this place
   if constexpr (DIRECT) {
     cs.seq = blockIdx.x / subs;
     cs.sub = blockIdx.x - cs.seq * subs;
     cs.tile = 0;
+    cs.at = 0;
     cs.enter(a);
-    count = cs.tiles;
+    end = cs.tiles;
   } else {
     const Space ws(a.workspace, a.num_seqs);
-    int mine = 0, own = 0;  // own: tiles of sequence threadIdx.x
+    int mine = 0, own = 0;  // own: of sequence threadIdx.x
     for (int s = threadIdx.x; s < a.num_seqs; s += kWarps * 32) {
-      const int n = tiles_of<S>(span_of(a, s)) * subs;
+      const int n = (tiles_of<S>(span_of(a, s)) + kUnitCost) * subs;
       if (s == (int)threadIdx.x) own = n;
       mine += n;
     }
@@ -224,20 +237,21 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<sizeof(C), DP, NT>::PER_SM)
     scan128(mine, total, part);
     int share = (total + gridDim.x - 1) / gridDim.x;
     share = share < kMinShare ? kMinShare : share;
-    start = (int64_t)blockIdx.x * share;
-    count = start < total ? (int)min((int64_t)share, total - start) : 0;
-    if (count == 0 && blockIdx.x != 0) return;
-    // the sequence that holds tile `start` (CTA 0 also leaves the prefix sums for the joining launch)
+    const int64_t start = (int64_t)blockIdx.x * share;
+    if (start >= total && blockIdx.x != 0) return;
+    end = (int)min(start + share, (int64_t)total);
+    // the sequence that holds `start` (CTA 0 also leaves the prefix sums for the joining launch)
     int base = 0;
     for (int s0 = 0; s0 < a.num_seqs; s0 += kWarps * 32) {
       const int s = s0 + threadIdx.x;
-      const int n = s >= a.num_seqs ? 0 : s0 == 0 ? own : tiles_of<S>(span_of(a, s)) * subs;
+      const int n = s >= a.num_seqs ? 0 : s0 == 0 ? own : (tiles_of<S>(span_of(a, s)) + kUnitCost) * subs;
       int sum;
       const int at = base + scan128(n, sum, part);
       if (s < a.num_seqs && start >= at && start < at + n) {
+        const int unit = n / subs, off = (int)(start - at);
         found[0] = s;
-        found[1] = (int)(start - at) / (n / subs);
-        found[2] = (int)(start - at) % (n / subs);
+        found[1] = off / unit;
+        found[2] = off % unit;
       }
       if (blockIdx.x == 0 && s < a.num_seqs) ws.before[s] = at;
       base += sum;
@@ -251,7 +265,13 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<sizeof(C), DP, NT>::PER_SM)
     cs.seq = found[0];
     cs.sub = found[1];
     cs.tile = found[2];
+    cs.at = (int)start;
     cs.enter(a);
+    if (cs.tile >= cs.tiles) {  // in the cost of a unit that others have done
+      cs.at += cs.tiles + kUnitCost - cs.tile;
+      cs.next_unit(a, subs);
+      if (cs.at >= end) return;
+    }
   }
 
   // ---------------------------------------------------------------- the copy stream of this warp
@@ -260,15 +280,15 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<sizeof(C), DP, NT>::PER_SM)
   const int block_shift = __ffs(a.block_size) - 1;
   const int run_rows = a.block_size < S::KW ? a.block_size : S::KW, runs = S::KW / run_rows;
   Walk<S> ld = cs;
-  int ld_left = count;
   struct Source {
+    bool on;             // there is such a tile
     int page, slot, hk;  // of run `lane` (+ 32 where pages are single slots); page -1: nothing to copy
     int page2;
   };
   // the pages of the next tile
   auto look = [&]() {
-    Source p = {-1, 0, 0, -1};
-    if (ld_left <= 0) return p;
+    Source p = {ld.at < end, -1, 0, 0, -1};
+    if (!p.on) return p;
     const int key0 = (ld.span.lo & -S::KW) + ld.tile * S::CT + warp * S::KW;
     p.hk = ld.sub / gtiles;
     const int32_t* table = a.block_tables + (int64_t)ld.seq * a.block_table_stride;
@@ -283,8 +303,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<sizeof(C), DP, NT>::PER_SM)
     p.slot = key0 & (a.block_size - 1);  // 0 where a tile has several runs
     p.page = page_of(lane);
     if (S::KW > 32 && runs > 32) p.page2 = page_of(lane + 32);
-    --ld_left;
-    if (ld_left > 0) ld.next(a, subs);
+    ld.next(a, subs);
     return p;
   };
   const uint64_t policy = policy_evict_first();
@@ -312,7 +331,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<sizeof(C), DP, NT>::PER_SM)
     for_k = look();
     issue(&maps.k, maps.k_role, s0, 0);
     issue(&maps.v, maps.v_role, s0, 1);
-    issue(&maps.k, maps.k_role, s1, 2);
+    if (s1.on) issue(&maps.k, maps.k_role, s1, 2);
     for_v = s1;
   }
   uint32_t parity = 0;  // bit b: the phase of buffer b that completes next
@@ -429,7 +448,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<sizeof(C), DP, NT>::PER_SM)
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) s[kt][n][c] = cap2 * tanhf(s[kt][n][c]);
+          for (int c = 0; c < 4; ++c) s[kt][n][c] = cap2 * tanh_of(s[kt][n][c]);
     }
     if (biased) {
 #pragma unroll
@@ -621,13 +640,14 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<sizeof(C), DP, NT>::PER_SM)
   bool from_start = cs.tile == 0;  // this CTA has the unit from its first tile
   int kb = 0;                      // buffer of the tile's keys; its values are in the next one
   bool late = false;               // a copy did not arrive within the bound
-  for (int i = 0; i < count; ++i) {
+  for (;;) {
     const int vb = kb + 1 == kBufs ? 0 : kb + 1;
     late = !arrived(kb);
     if (late) break;
     scores(kb);
     __syncwarp();
-    if (i + 1 < count) issue(&maps.v, maps.v_role, for_v, kb);
+    const bool more = for_v.on;
+    if (more) issue(&maps.v, maps.v_role, for_v, kb);
     late = !arrived(vb);
     if (late) break;
     clear_hidden(vb);
@@ -635,17 +655,16 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<sizeof(C), DP, NT>::PER_SM)
     __syncwarp();
     const bool last_tile = cs.tile + 1 == cs.tiles;
     // a CTA leaves at most two partial states: of a unit begun by others, and of one that it began
-    if (last_tile || i + 1 == count) end_unit(vb, from_start && last_tile, from_start ? 1 : 0);
-    if (i + 2 < count) issue(&maps.k, maps.k_role, for_k, vb);
+    if (last_tile || !more) end_unit(vb, from_start && last_tile, from_start ? 1 : 0);
+    if (!more) break;
+    if (for_k.on) issue(&maps.k, maps.k_role, for_k, vb);
     for_v = for_k;
     for_k = look();
     kb = vb + 1 == kBufs ? 0 : vb + 1;
-    if (i + 1 < count) {
-      cs.next(a, subs);
-      if (cs.tile == 0) {
-        begin_unit();
-        from_start = true;
-      }
+    cs.next(a, subs);
+    if (cs.tile == 0) {
+      begin_unit();
+      from_start = true;
     }
   }
   if (late) {  // report it, and let this warp's other copies land before the CTA's memory is reused
@@ -670,8 +689,8 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ oc_pa
   const int h = blockIdx.x, seq = blockIdx.y, hk = h / a.group, hg = h - hk * a.group;
   const int sub = hk * gtiles + hg / HT, hr = hg % HT;
   const Space ws(a.workspace, a.num_seqs);
-  const int before = ws.before[seq], tiles = (ws.before[seq + 1] - before) / subs, share = ws.before[a.num_seqs + 1];
-  const int t0 = before + sub * tiles, t1 = t0 + tiles, c0 = t0 / share, c1 = (t1 - 1) / share;
+  const int before = ws.before[seq], tiles = (ws.before[seq + 1] - before) / subs - kUnitCost, share = ws.before[a.num_seqs + 1];
+  const int t0 = before + sub * (tiles + kUnitCost), t1 = t0 + tiles, c0 = t0 / share, c1 = (t1 - 1) / share;
   if (c0 == c1) return;  // one CTA had it all and wrote the output
   auto state = [&](int c) {
     // the unit is the CTA's first unless it starts inside the CTA's run
@@ -685,7 +704,7 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ oc_pa
   float sum = 0.f, x[DP / 32];
 #pragma unroll
   for (int i = 0; i < DP / 32; ++i) x[i] = 0.f;
-#pragma unroll 2
+#pragma unroll 4
   for (int c = c0 + warp; c <= c1; c += W) {
     const float* s = state(c);
     const float mc = s[HT * DP + 2 * hr], lc = s[HT * DP + 2 * hr + 1];
@@ -779,7 +798,7 @@ void plan_nt(const oc_paged_decode_args& a, Plan& p) {
   int64_t most = (int64_t)a.max_blocks * a.block_size;
   if (a.window > 0 && a.window + S::KW < most) most = a.window + S::KW;
   const int64_t tiles = (most + S::CT - 1) / S::CT, wave = (int64_t)a.num_sms * S::PER_SM;
-  const int64_t useful = (units * tiles + kMinShare - 1) / kMinShare;
+  const int64_t useful = (units * (tiles + kUnitCost) + kMinShare - 1) / kMinShare;
   p.nt = NT;
   p.direct = tiles <= kDirectTiles;
   p.grid = p.direct ? units : useful < wave ? useful : wave;

@@ -11,6 +11,7 @@
 #include <cooperative_groups.h>
 
 #include "oc_ops.cuh"
+#include "oc_ptx.cuh"
 
 namespace {
 
@@ -18,6 +19,7 @@ using namespace oc;
 
 constexpr int kMaxCaches = 128;  // pointers that travel in one launch's parameters
 constexpr int kThreads = 1024;
+constexpr int kShortList = 2048;  // pages handed out by a reserve call whose list stays in shared memory
 
 struct Caches {
   char* base[kMaxCaches];
@@ -55,64 +57,175 @@ __device__ __forceinline__ int block_scan(int v, int& total) {
 }
 
 // ------------------------------------------------------------------ page copies
-// Pairs come from arrays of n entries, or of *n_dev entries on the device.
-// One warp-group unit = (pair, cache, chunk of a page); a grid-stride loop.
-template <int BYTES>
-__global__ void __launch_bounds__(256) copy_kernel(const __grid_constant__ Caches caches, int num_caches,
-                                                   int64_t page_bytes, int64_t num_pages, const int32_t* src,
-                                                   const int32_t* dst, int64_t n, const int32_t* n_dev,
-                                                   uint32_t* status) {
+// The table of a compaction, renumbered by the launch that moves its pages.
+struct Renumber {
+  const int32_t *in, *to;
+  int32_t* out;
+  int64_t in_stride, out_stride, num_seqs, max_blocks;
+};
+
+__device__ __forceinline__ void renumber(const Renumber& table, int64_t num_pages, uint32_t* status) {
+  const int64_t entries = table.num_seqs * table.max_blocks;
+  for (int64_t e = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; e < entries; e += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t r = e / table.max_blocks, c = e - r * table.max_blocks;
+    const int32_t p = table.in[r * table.in_stride + c];
+    if (p >= num_pages) raise_status(status, OC_STATUS_BAD_PAGE);
+    table.out[r * table.out_stride + c] = p < 0 || p >= num_pages ? -1 : table.to[p];
+  }
+}
+
+// The copies of one launch: pairs come from arrays of n entries, or of *n_dev
+// entries on the device.
+struct Copies {
+  const int32_t *src, *dst, *n_dev;
+  int64_t n, page_bytes, num_pages;
+  int num_caches;
+};
+
+// Pages through shared memory, by bulk copies in both directions: one lane of
+// each warp keeps kStages pieces of up to 8 KB on their way, 192 KB an SM, and
+// spends no registers on them.  A warp takes an equal run of the pieces.
+constexpr int kCopyWarps = 6, kStages = 4, kPiece = 8192;
+constexpr uint32_t kPolls = 1u << 22;  // bound of a wait for a copy
+
+__global__ void __launch_bounds__(kCopyWarps * 32)
+    copy_bulk_kernel(const __grid_constant__ Caches caches, const __grid_constant__ Copies job, Renumber table,
+                     uint32_t* status) {
+  extern __shared__ __align__(128) char ring[];
+  __shared__ __align__(8) uint64_t bars[kCopyWarps][kStages];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t bar = smem_u32(bars[warp]), mine = smem_u32(ring) + warp * kStages * kPiece;
+  if (lane == 0) {
+    for (int i = 0; i < kStages; ++i) mbar_init(bar + 8 * i, 1);
+    mbar_init_fence();
+  }
   pdl_launch_dependents();
   pdl_wait();
-  if (n_dev) n = *n_dev;
-  constexpr int64_t kChunk = 256 * 4 * BYTES;
-  const int64_t chunks = (page_bytes + kChunk - 1) / kChunk, units = n * num_caches * chunks;
-  using V = Vec<uint8_t, BYTES>;
-  for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
-    const int64_t pc = u / chunks, chunk = u - pc * chunks;
-    const int64_t pair = pc / num_caches;
-    const int c = (int)(pc - pair * num_caches);
-    const int64_t s = src[pair], d = dst[pair];
+  if (table.out) renumber(table, job.num_pages, status);
+  if (lane != 0) return;
+  const int64_t n = job.n_dev ? *job.n_dev : job.n, per_page = (job.page_bytes + kPiece - 1) / kPiece;
+  const int64_t total = n * job.num_caches * per_page, warps = (int64_t)gridDim.x * kCopyWarps;
+  const int64_t me = (int64_t)blockIdx.x * kCopyWarps + warp;
+  const int64_t begin = total * me / warps, end = total * (me + 1) / warps;
+  if (begin >= end) return;
+  // walks over (pair, cache, piece of the page)
+  struct Walk {
+    int64_t pair, piece, from, to;
+    int cache;
+  };
+  auto enter = [&](Walk& w) {  // from -1: the pair is skipped
+    w.from = job.src[w.pair];
+    w.to = job.dst[w.pair];
+    if (w.from >= job.num_pages || w.to >= job.num_pages) {
+      raise_status(status, OC_STATUS_BAD_PAGE);
+      w.from = -1;
+    }
+    if (w.to < 0) w.from = -1;
+  };
+  auto next = [&](Walk& w, int64_t at) {  // to piece `at` of all
+    if (++w.piece < per_page) return;
+    w.piece = 0;
+    if (++w.cache < job.num_caches) return;
+    w.cache = 0;
+    ++w.pair;
+    if (at < end) enter(w);
+  };
+  Walk ld;
+  ld.pair = begin / (per_page * job.num_caches);
+  const int64_t rest = begin - ld.pair * per_page * job.num_caches;
+  ld.cache = (int)(rest / per_page);
+  ld.piece = rest - ld.cache * per_page;
+  enter(ld);
+  Walk st = ld;
+  auto bytes_of = [&](const Walk& w) { return (uint32_t)min((int64_t)kPiece, job.page_bytes - w.piece * kPiece); };
+  auto load = [&](int64_t at) {
+    if (at >= end) return;
+    const int s = (int)((at - begin) % kStages);
+    if (ld.from >= 0) {
+      mbar_arrive_expect_tx(bar + 8 * s, bytes_of(ld));
+      bulk_load(mine + s * kPiece, caches.base[ld.cache] + ld.from * caches.stride[ld.cache] + ld.piece * kPiece,
+                bytes_of(ld), bar + 8 * s);
+    } else {
+      mbar_arrive_expect_tx(bar + 8 * s, 0);
+    }
+    next(ld, at + 1);
+  };
+  for (int i = 0; i < kStages - 1; ++i) load(begin + i);
+  bool late = false;
+  for (int64_t at = begin; at < end; ++at) {
+    const int s = (int)((at - begin) % kStages);
+    late = !mbar_wait_bounded(bar + 8 * s, (uint32_t)((at - begin) / kStages) & 1, kPolls);
+    if (late) break;
+    if (st.from >= 0)
+      bulk_store(caches.base[st.cache] + st.to * caches.stride[st.cache] + st.piece * kPiece, mine + s * kPiece,
+                 bytes_of(st));
+    bulk_commit();
+    bulk_wait_read<1>();  // the piece before this one has left its buffer
+    load(at + kStages - 1);
+    next(st, at + 1);
+  }
+  if (late) {  // report it, and let the other copies land before the CTA's memory is reused
+    raise_status(status, OC_STATUS_TIMEOUT);
+    for (int64_t at = begin; at < end && at < begin + kStages; ++at) mbar_wait_bounded(bar + 8 * (at - begin), 0, kPolls);
+  }
+  bulk_wait<0>();
+}
+
+// Any size and alignment: a warp moves 128 bytes of one page at a time.
+__global__ void __launch_bounds__(256)
+    copy_bytes_kernel(const __grid_constant__ Caches caches, const __grid_constant__ Copies job, Renumber table,
+                      uint32_t* status) {
+  pdl_launch_dependents();
+  pdl_wait();
+  if (table.out) renumber(table, job.num_pages, status);
+  const int lane = threadIdx.x & 31;
+  const int64_t n = job.n_dev ? *job.n_dev : job.n, per_page = (job.page_bytes + 127) / 128;
+  const int64_t units = n * job.num_caches * per_page;
+  for (int64_t u = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); u < units; u += (int64_t)gridDim.x * 8) {
+    const int64_t pc = u / per_page, pair = pc / job.num_caches;
+    const int c = (int)(pc - pair * job.num_caches);
+    const int64_t s = job.src[pair], d = job.dst[pair];
     if (s < 0 || d < 0) continue;
-    if (s >= num_pages || d >= num_pages) {
-      if (threadIdx.x == 0) raise_status(status, OC_STATUS_BAD_PAGE);
+    if (s >= job.num_pages || d >= job.num_pages) {
+      if (lane == 0) raise_status(status, OC_STATUS_BAD_PAGE);
       continue;
     }
-    const char* from = caches.base[c] + s * caches.stride[c];
-    char* to = caches.base[c] + d * caches.stride[c];
-    const int64_t begin = chunk * kChunk + threadIdx.x * BYTES;
-    V v[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (begin + i * 256 * BYTES < page_bytes) v[i] = *reinterpret_cast<const V*>(from + begin + i * 256 * BYTES);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (begin + i * 256 * BYTES < page_bytes) *reinterpret_cast<V*>(to + begin + i * 256 * BYTES) = v[i];
+    for (int64_t i = (u - pc * per_page) * 128 + lane; i < min((u - pc * per_page + 1) * 128, job.page_bytes); i += 32)
+      caches.base[c][d * caches.stride[c] + i] = caches.base[c][s * caches.stride[c] + i];
   }
 }
 
 // Copies over every cache; at most `most` pairs.
 int copy_all(void* const* caches, const int64_t* strides, int num_caches, int64_t page_bytes, int64_t num_pages,
-             const int32_t* src, const int32_t* dst, int64_t most, const int32_t* n_dev, uint32_t* status, int num_sms,
-             void* stream) {
-  for (int first = 0; first < num_caches; first += kMaxCaches) {
+             const int32_t* src, const int32_t* dst, int64_t most, const int32_t* n_dev, Renumber table,
+             uint32_t* status, int num_sms, void* stream) {
+  for (int first = 0; first < num_caches || table.out; first += kMaxCaches) {
     const int m = num_caches - first < kMaxCaches ? num_caches - first : kMaxCaches;
-    Caches c = {};
+    Caches c;
     bool vec = page_bytes % 16 == 0;
     for (int i = 0; i < m; ++i) {
       c.base[i] = static_cast<char*>(caches[first + i]);
       c.stride[i] = strides[first + i];
       vec = vec && aligned_to(c.base[i], 16) && c.stride[i] % 16 == 0;
     }
-    const int64_t chunk = 256 * 4 * (vec ? 16 : 1);
-    const int64_t units = most * m * ((page_bytes + chunk - 1) / chunk);
-    const int64_t full = (int64_t)num_sms * 8;
-    const unsigned grid = (unsigned)(units < full ? (units < 1 ? 1 : units) : full);
-    const int rc = vec ? launch_pdl(copy_kernel<16>, grid, 256, 0, stream, c, m, page_bytes, num_pages, src, dst, most,
-                                    n_dev, status)
-                       : launch_pdl(copy_kernel<1>, grid, 256, 0, stream, c, m, page_bytes, num_pages, src, dst, most,
-                                    n_dev, status);
+    const Copies job = {src, dst, n_dev, most, page_bytes, num_pages, m};
+    constexpr int smem = kCopyWarps * kStages * kPiece;
+    int rc;
+    if (vec) {
+      const int64_t pieces = most * m * ((page_bytes + kPiece - 1) / kPiece), entries = table.num_seqs * table.max_blocks;
+      int64_t ctas = (pieces + kCopyWarps - 1) / kCopyWarps;
+      if (table.out && ctas < entries / (kCopyWarps * 32) + 1) ctas = entries / (kCopyWarps * 32) + 1;
+      ctas = ctas < 1 ? 1 : ctas < num_sms ? ctas : num_sms;
+      if (cudaFuncSetAttribute(copy_bulk_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
+        cudaGetLastError();
+        return OC_ERR_CUDA;
+      }
+      rc = launch_pdl(copy_bulk_kernel, (unsigned)ctas, kCopyWarps * 32, smem, stream, c, job, table, status);
+    } else {
+      rc = launch_pdl(copy_bytes_kernel, (unsigned)num_sms * 8, 256, 0, stream, c, job, table, status);
+    }
     if (rc != OC_OK) return rc;
+    table.out = nullptr;
   }
   return OC_OK;
 }
@@ -176,11 +289,24 @@ __global__ void __launch_bounds__(kThreads) reserve_kernel(int32_t* table, int64
                                                            int max_blocks, int64_t num_pages, int block_size,
                                                            void* workspace, uint32_t* status) {
   extern __shared__ int32_t shared_page[];  // num_seqs
+  __shared__ int32_t short_list[kShortList];
   __shared__ int bad;
   pdl_launch_dependents();
   pdl_wait();
   const ReserveSpace ws(workspace, num_seqs);
   if (threadIdx.x == 0) bad = 0;
+  // the counts of the first pages, read ahead of the rows that will ask for them
+  const bool quads = (reinterpret_cast<uintptr_t>(refs) & 15) == 0;
+  auto counts_at = [&](int64_t i) {
+    if (quads && i + 4 <= num_pages) return *reinterpret_cast<const int4*>(refs + i);
+    int4 r = {1, 1, 1, 1};
+    if (i < num_pages) r.x = refs[i];
+    if (i + 1 < num_pages) r.y = refs[i + 1];
+    if (i + 2 < num_pages) r.z = refs[i + 2];
+    if (i + 3 < num_pages) r.w = refs[i + 3];
+    return r;
+  };
+  const int4 first_counts = counts_at((int64_t)threadIdx.x * 4);
   // 1: the page that a growing sequence would write to and others hold too
   for (int r = threadIdx.x; r < num_seqs; r += blockDim.x) {
     const int len = lens[r], part = len / block_size;
@@ -223,26 +349,23 @@ __global__ void __launch_bounds__(kThreads) reserve_kernel(int32_t* table, int64
   int total;
   int rank = block_scan(need, total);
   // 3: the lowest free pages
+  int32_t* const list = total <= kShortList ? short_list : ws.free;
   int found = 0;
   for (int64_t base = 0; base < num_pages && found < total; base += (int64_t)blockDim.x * 4) {
     const int64_t i = base + threadIdx.x * 4;
-    int f[4], n = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      f[j] = i + j < num_pages && refs[i + j] == 0;
-      n += f[j];
-    }
+    const int4 r = base == 0 ? first_counts : counts_at(i);
+    const int f[4] = {r.x == 0, r.y == 0, r.z == 0, r.w == 0};
     int sum;
-    int at = found + block_scan(n, sum);
+    int at = found + block_scan(f[0] + f[1] + f[2] + f[3], sum);
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       if (f[j]) {
-        if (at < total) ws.free[at] = (int32_t)(i + j);
+        if (at < total) list[at] = (int32_t)(i + j);
         ++at;
       }
     found += sum;
   }
-  __syncthreads();  // ws.free and bad are complete
+  __syncthreads();  // the list and bad are complete
   int copied_before, all_copies;
   copied_before = block_scan(__popcll(copies), all_copies);
   if (bad || found < total) {
@@ -256,7 +379,7 @@ __global__ void __launch_bounds__(kThreads) reserve_kernel(int32_t* table, int64
   for (int r = r0; r < r1; ++r) {
     const int len = lens[r], goal = (int)(((int64_t)wanted[r] + block_size - 1) / block_size);
     if (copies >> (r - r0) & 1) {
-      const int p = shared_page[r], q = ws.free[rank++];
+      const int p = shared_page[r], q = list[rank++];
       table[r * stride + len / block_size] = q;
       refs[q] = 1;
       atomicSub(refs + p, 1);
@@ -266,7 +389,7 @@ __global__ void __launch_bounds__(kThreads) reserve_kernel(int32_t* table, int64
     int held = (len + block_size - 1) / block_size;
     while (held < goal && table[r * stride + held] >= 0) ++held;
     for (; held < goal; ++held) {
-      const int q = ws.free[rank++];
+      const int q = list[rank++];
       table[r * stride + held] = q;
       refs[q] = 1;
     }
@@ -327,20 +450,6 @@ __global__ void __launch_bounds__(kThreads) compact_plan_kernel(const int32_t* r
   if (threadIdx.x == 0) *ws.count = movers;
 }
 
-__global__ void __launch_bounds__(256) renumber_kernel(const int32_t* table_in, int64_t in_stride, int32_t* table_out,
-                                                       int64_t out_stride, int num_seqs, int max_blocks,
-                                                       int64_t num_pages, const int32_t* to, uint32_t* status) {
-  pdl_launch_dependents();
-  pdl_wait();
-  const int64_t entries = (int64_t)num_seqs * max_blocks;
-  for (int64_t e = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; e < entries; e += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t r = e / max_blocks, c = e - r * max_blocks;
-    const int32_t p = table_in[r * in_stride + c];
-    if (p >= num_pages) raise_status(status, OC_STATUS_BAD_PAGE);
-    table_out[r * out_stride + c] = p < 0 || p >= num_pages ? -1 : to[p];
-  }
-}
-
 bool bad_caches(void* const* caches, const int64_t* strides, int num_caches, int64_t page_bytes) {
   if (num_caches < 0 || page_bytes < 1 || (num_caches && (!caches || !strides))) return true;
   for (int i = 0; i < num_caches; ++i)
@@ -359,8 +468,8 @@ extern "C" int oc_copy_pages(void* const* caches, const int64_t* page_strides, i
       (n && (!src || !dst)))
     return OC_ERR_INVALID;
   if (n == 0) return OC_OK;
-  return copy_all(caches, page_strides, num_caches, page_bytes, num_pages, src, dst, n, nullptr, status, num_sms,
-                  stream);
+  return copy_all(caches, page_strides, num_caches, page_bytes, num_pages, src, dst, n, nullptr, Renumber{}, status,
+                  num_sms, stream);
 }
 
 extern "C" int oc_fork_sequences(const int32_t* table_in, int64_t table_in_stride, int32_t* table_out,
@@ -416,8 +525,8 @@ extern "C" int oc_reserve_pages(void* const* caches, const int64_t* page_strides
                             refs, wanted, num_seqs, max_blocks, num_pages, block_size, workspace, status);
   if (rc != OC_OK || num_caches == 0) return rc;
   const ReserveSpace ws(workspace, num_seqs);
-  return copy_all(caches, page_strides, num_caches, page_bytes, num_pages, ws.src, ws.dst, num_seqs, ws.count, status,
-                  num_sms, stream);
+  return copy_all(caches, page_strides, num_caches, page_bytes, num_pages, ws.src, ws.dst, num_seqs, ws.count,
+                  Renumber{}, status, num_sms, stream);
 }
 
 extern "C" size_t oc_compact_workspace_bytes(int64_t num_pages) {
@@ -437,15 +546,11 @@ extern "C" int oc_compact_pages(void* const* caches, const int64_t* page_strides
   if (!workspace || !aligned_to(workspace, 4) || workspace_bytes < oc_compact_workspace_bytes(num_pages))
     return OC_ERR_WORKSPACE;
   const CompactSpace ws(workspace, num_pages);
-  int rc = launch_pdl(compact_plan_kernel, 1, kThreads, 0, stream, refs_in, refs_out, num_pages, workspace);
-  const int64_t entries = (int64_t)num_seqs * max_blocks;
-  if (rc == OC_OK && entries > 0) {
-    const int64_t blocks = (entries + 255) / 256;
-    rc = launch_pdl(renumber_kernel, (unsigned)(blocks < num_sms * 8 ? blocks : num_sms * 8), 256, 0, stream, table_in,
-                    table_in_stride, table_out, table_out_stride, num_seqs, max_blocks, num_pages, ws.to, status);
-  }
-  if (rc == OC_OK && num_caches > 0)
-    rc = copy_all(caches, page_strides, num_caches, page_bytes, num_pages, ws.src, ws.dst, num_pages, ws.count, status,
-                  num_sms, stream);
-  return rc;
+  const int rc = launch_pdl(compact_plan_kernel, 1, kThreads, 0, stream, refs_in, refs_out, num_pages, workspace);
+  if (rc != OC_OK) return rc;
+  Renumber table = {};
+  if (num_seqs > 0 && max_blocks > 0)
+    table = Renumber{table_in, ws.to, table_out, table_in_stride, table_out_stride, num_seqs, max_blocks};
+  return copy_all(caches, page_strides, num_caches, page_bytes, num_pages, ws.src, ws.dst, num_pages, ws.count, table,
+                  status, num_sms, stream);
 }

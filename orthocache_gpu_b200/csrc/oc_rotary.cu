@@ -4,11 +4,12 @@
 //   y_a = x_a c - x_b s,  y_b = x_b c + x_a s   for each pair (a, b) of the
 //   first rotary_dim columns, c / s from float32 tables at the token's
 //   position, in float32, rounded once;  cache[table[seq, pos / bs], h,
-//   pos % bs] = round(k / k_scale).
+//   pos % bs] = round(k (1 / k_scale)).
 //
 // Every element is read once and written once (k twice where k_out is asked
 // for): memory bound for prompts, launch latency for steps.
 #include "oc_ops.cuh"
+#include "oc_ptx.cuh"
 
 namespace {
 
@@ -30,8 +31,17 @@ template <typename T, int N, bool ALIGNED>
 __device__ __forceinline__ void store_vec(T* p, int n, const float (&x)[N]) {
   if constexpr (ALIGNED) {
     Vec<T, N> v;
+    if constexpr (sizeof(T) == 1) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) v.e[i] = from_f32<T>(x[i]);
+      for (int i = 0; i < N; i += 2) {
+        const auto two = __nv_cvt_float2_to_fp8x2(float2{x[i], x[i + 1]}, __NV_SATFINITE, __NV_E4M3);
+        v.e[i].b = (uint8_t)(two & 0xff);
+        v.e[i + 1].b = (uint8_t)(two >> 8);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) v.e[i] = from_f32<T>(x[i]);
+    }
     *reinterpret_cast<Vec<T, N>*>(p) = v;
   } else {
 #pragma unroll
@@ -41,11 +51,11 @@ __device__ __forceinline__ void store_vec(T* p, int n, const float (&x)[N]) {
 }
 
 template <typename C, int N, bool ALIGNED>
-__device__ __forceinline__ void store_cache(C* p, int n, const float (&x)[N], float scale) {
+__device__ __forceinline__ void store_cache(C* p, int n, const float (&x)[N], float inv_scale) {
   if constexpr (sizeof(C) == 1) {
     float y[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) y[i] = __fdiv_rn(x[i], scale);
+    for (int i = 0; i < N; ++i) y[i] = x[i] * inv_scale;
     store_vec<C, N, ALIGNED>(p, n, y);
   } else {
     store_vec<C, N, ALIGNED>(p, n, x);
@@ -98,6 +108,7 @@ __global__ void __launch_bounds__(256) rotary_append_kernel(const oc_rotary_args
   C* kc = page >= 0 ? static_cast<C*>(a.k_cache) + page * a.kc_block_stride + (int64_t)slot * a.kc_tok_stride : nullptr;
   C* vc = page >= 0 ? static_cast<C*>(a.v_cache) + page * a.vc_block_stride + (int64_t)slot * a.vc_tok_stride : nullptr;
   const int nh = a.q_heads + a.kv_heads * (a.v ? 2 : 1);
+  const float k_inv = 1.f / a.k_scale, v_inv = 1.f / a.v_scale;
 
   for (int i = threadIdx.x; i < columns; i += blockDim.x) {
     // columns [lo, lo + n) and, in the half layout, their partners [hi, hi + n)
@@ -162,7 +173,7 @@ __global__ void __launch_bounds__(256) rotary_append_kernel(const oc_rotary_args
         }
         if (kc) {
           C* dst = is_k ? kc + hk * a.kc_head_stride : vc + hk * a.vc_head_stride;
-          const float scale = is_k ? a.k_scale : a.v_scale;
+          const float scale = is_k ? k_inv : v_inv;
           store_cache<C, N, ALIGNED>(dst + lo, n, x, scale);
           if (!INTER && hi >= 0) store_cache<C, N, ALIGNED>(dst + hi, n, y, scale);
         }
@@ -196,6 +207,253 @@ int launch(const oc_rotary_args& a, void* stream) {
                     dim3((unsigned)bx, (unsigned)by, (unsigned)bz), 0, stream, a, lanes, columns);
 }
 
+// ------------------------------------------------------------------ prompts
+// Enough tokens for every warp of the machine: the loads of the kernel above,
+// at most a few per thread between two stores, leave HBM half idle, so here
+// each warp keeps its input on the way ahead of it: a ring of kStages bulk
+// copies of up to 4 KB (a run of heads of q, k or v, which lie side by side),
+// 192 KB an SM.  A warp takes an equal run of those pieces, token after token.
+// Lane (head, column) holds its column's table entries; those, the page and
+// the position of the next tokens are read while this one is worked on.
+constexpr int kStages = 3, kStageBytes = 4096, kStreamWarps = 16;
+constexpr uint32_t kPolls = 1u << 22;  // bound of a wait for a copy
+
+template <typename T, typename C, int N, bool INTER>
+__global__ void __launch_bounds__(kStreamWarps * 32, 1)
+    rotary_stream_kernel(const __grid_constant__ oc_rotary_args a, int columns) {
+  constexpr int NT = INTER ? N / 2 : N;  // table entries of a vector
+  extern __shared__ __align__(128) char ring[];
+  __shared__ __align__(8) uint64_t bars[kStreamWarps][kStages];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t my_bar = smem_u32(bars[warp]), my_ring = smem_u32(ring) + warp * kStages * kStageBytes;
+  const char* const mine = ring + warp * kStages * kStageBytes;
+  if (lane == 0) {
+    for (int i = 0; i < kStages; ++i) mbar_init(my_bar + 8 * i, 1);
+    mbar_init_fence();
+  }
+  __syncwarp();
+  pdl_launch_dependents();
+  pdl_wait();
+
+  // a token's pieces: runs of `most` heads of q, of k, of v
+  const int row = a.head_dim * (int)sizeof(T), most = kStageBytes / row;
+  const int nq = (a.q_heads + most - 1) / most, nk = (a.kv_heads + most - 1) / most;
+  const int pieces = nq + nk * (a.v ? 2 : 1);
+  struct Piece {
+    int part, h0, heads;  // 0 q, 1 k, 2 v
+  };
+  auto piece_of = [&](int i) {
+    Piece p;
+    p.part = i < nq ? 0 : i < nq + nk ? 1 : 2;
+    p.h0 = (p.part == 0 ? i : p.part == 1 ? i - nq : i - nq - nk) * most;
+    p.heads = min(most, (p.part == 0 ? a.q_heads : a.kv_heads) - p.h0);
+    return p;
+  };
+  const int64_t warps = (int64_t)gridDim.x * kStreamWarps, me = (int64_t)blockIdx.x * kStreamWarps + warp;
+  const int64_t begin = a.tokens * pieces * me / warps, end = a.tokens * pieces * (me + 1) / warps;
+  if (begin >= end) return;
+  int64_t t = begin / pieces;
+  int i = (int)(begin - t * pieces);
+  int64_t ld_t = t, ld_left = end - begin;
+  int ld_piece = i, ld_stage = 0;
+  auto issue = [&]() {  // the next piece's copy
+    if (ld_left <= 0) return;
+    --ld_left;
+    if (lane == 0) {
+      const Piece p = piece_of(ld_piece);
+      const char* src = static_cast<const char*>(p.part == 0 ? a.q : p.part == 1 ? a.k : a.v);
+      const int64_t stride = p.part == 0 ? a.q_tok_stride : p.part == 1 ? a.k_tok_stride : a.v_tok_stride;
+      const uint32_t bar = my_bar + 8 * ld_stage, bytes = (uint32_t)(p.heads * row);
+      mbar_arrive_expect_tx(bar, bytes);
+      bulk_load(my_ring + ld_stage * kStageBytes, src + ld_t * stride * (int64_t)sizeof(T) + (int64_t)p.h0 * row, bytes, bar);
+    }
+    ld_stage = ld_stage + 1 == kStages ? 0 : ld_stage + 1;
+    if (++ld_piece == pieces) {
+      ld_piece = 0;
+      ++ld_t;
+    }
+  };
+
+  // this lane's column
+  const int half = a.rotary_dim / 2, turning = (INTER ? a.rotary_dim : half) / N;
+  const int col = lane % columns, hl = lane / columns, side = 32 / columns;
+  const bool active = hl < side, turn = col < turning, paired = !INTER && turn;
+  const int lo = turn ? col * N : a.rotary_dim + (col - turning) * N;
+  const int shift = a.k_cache ? __ffs(a.block_size) - 1 : 0;
+  const float sign = a.flags & OC_ROTARY_INVERSE ? -1.f : 1.f;
+  const float k_inv = 1.f / a.k_scale, v_inv = 1.f / a.v_scale;
+
+  struct Place {
+    int64_t pos, seq;
+  };
+  auto place_of = [&](int64_t t) {
+    Place p = {0, -1};  // beyond the last token: a place that exists and appends nothing
+    if (t < a.tokens) {
+      p.pos = a.positions_64 ? static_cast<const int64_t*>(a.positions)[t]
+                             : (int64_t) static_cast<const int32_t*>(a.positions)[t];
+      if (a.k_cache) p.seq = a.seq_ids ? a.seq_ids[t] : t;
+    }
+    return p;
+  };
+  struct Token {
+    float c[NT], s[NT];
+    int page, slot;  // page -2: no append
+  };
+  auto look = [&](Place p) {
+    Token k;
+    const bool inside = half == 0 || (p.pos >= 0 && p.pos < a.table_rows);
+    bool bad = !inside;
+    k.page = -2;
+    k.slot = 0;
+    if (p.seq >= 0) {
+      const int64_t column = p.pos >> shift;
+      if (inside && p.pos >= 0 && p.seq < a.num_seqs && column < a.max_blocks) {
+        k.page = a.block_tables[p.seq * a.block_table_stride + column];
+        k.page = k.page < 0 || k.page >= a.num_blocks ? -1 : k.page;
+        k.slot = (int)(p.pos & (a.block_size - 1));
+      } else {
+        bad = true;
+      }
+    }
+    if (bad && lane == 0) raise_status(a.status, OC_STATUS_POSITION);
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      k.c[j] = 1.f;
+      k.s[j] = 0.f;
+    }
+    if (turn) {
+      const float* ct = a.cos_tab + (inside ? p.pos : 0) * half + (INTER ? lo / 2 : lo);
+      const float* st = a.sin_tab + (inside ? p.pos : 0) * half + (INTER ? lo / 2 : lo);
+      constexpr int W = NT < 4 ? NT : 4;
+#pragma unroll
+      for (int j = 0; j < NT; j += W) {
+        const Vec<float, W> cv = *reinterpret_cast<const Vec<float, W>*>(ct + j);
+        const Vec<float, W> sv = *reinterpret_cast<const Vec<float, W>*>(st + j);
+#pragma unroll
+        for (int e = 0; e < W; ++e) {
+          k.c[j + e] = cv.e[e];
+          k.s[j + e] = sv.e[e] * sign;
+        }
+      }
+    }
+    return k;
+  };
+
+#pragma unroll
+  for (int s = 0; s < kStages; ++s) issue();
+  const Place p0 = place_of(t), p1 = place_of(t + 1);
+  Token now = look(p0), next = look(p1);
+  Place ahead = place_of(t + 2);
+  int stage = 0;
+  uint32_t parity = 0;
+  bool late = false;
+  for (int64_t left = end - begin; left > 0; --left) {
+      if (now.page == -1 && lane == 0) raise_status(a.status, OC_STATUS_BAD_PAGE);
+      const Piece p = piece_of(i);
+      late = !__all_sync(0xffffffffu, mbar_wait_bounded(my_bar + 8 * stage, parity >> stage & 1, kPolls));
+      if (late) break;
+      parity ^= 1u << stage;
+      const char* in = mine + stage * kStageBytes;
+      T* out = nullptr;
+      int64_t out_head = 0, cache_head = 0;
+      C* cache = nullptr;
+      float inv = 1.f;
+      if (p.part == 0) {
+        out = static_cast<T*>(a.q_out) + t * a.qo_tok_stride + lo;
+        out_head = a.qo_head_stride;
+      } else if (p.part == 1) {
+        if (a.k_out) out = static_cast<T*>(a.k_out) + t * a.ko_tok_stride + lo;
+        out_head = a.ko_head_stride;
+        if (now.page >= 0)
+          cache = static_cast<C*>(a.k_cache) + now.page * a.kc_block_stride + now.slot * a.kc_tok_stride + lo;
+        cache_head = a.kc_head_stride;
+        inv = k_inv;
+      } else {
+        if (now.page >= 0)
+          cache = static_cast<C*>(a.v_cache) + now.page * a.vc_block_stride + now.slot * a.vc_tok_stride + lo;
+        cache_head = a.vc_head_stride;
+        inv = v_inv;
+      }
+      const bool rotate = turn && p.part != 2;
+      if (active) {
+#pragma unroll 2
+        for (int h = hl; h < p.heads; h += side) {
+          const T* src = reinterpret_cast<const T*>(in + h * row) + lo;
+          const Vec<T, N> xv = *reinterpret_cast<const Vec<T, N>*>(src);
+          Vec<T, N> yv = {};
+          if (paired) yv = *reinterpret_cast<const Vec<T, N>*>(src + half);
+          float x[N], y[N];
+#pragma unroll
+          for (int j = 0; j < N; ++j) {
+            x[j] = to_f32(xv.e[j]);
+            y[j] = to_f32(yv.e[j]);
+          }
+          if (rotate) {
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+              float& u = INTER ? x[2 * j] : x[j];
+              float& w = INTER ? x[2 * j + 1] : y[j];
+              const float u0 = u, w0 = w;
+              u = u0 * now.c[j] - w0 * now.s[j];
+              w = w0 * now.c[j] + u0 * now.s[j];
+            }
+          }
+          if (out) {
+            T* dst = out + (p.h0 + h) * out_head;
+            store_vec<T, N, true>(dst, N, x);
+            if (paired) store_vec<T, N, true>(dst + half, N, y);
+          }
+          if (cache) {
+            C* dst = cache + (p.h0 + h) * cache_head;
+            store_cache<C, N, true>(dst, N, x, inv);
+            if (paired) store_cache<C, N, true>(dst + half, N, y, inv);
+          }
+        }
+      }
+      __syncwarp();  // every lane has read the stage before it is filled again
+      issue();
+      stage = stage + 1 == kStages ? 0 : stage + 1;
+      if (++i == pieces) {
+        i = 0;
+        ++t;
+        now = next;
+        next = look(ahead);
+        ahead = place_of(t + 2);
+      }
+  }
+  if (late) {  // report it, and let this warp's other copies land before the CTA's memory is reused
+    if (lane == 0) raise_status(a.status, OC_STATUS_TIMEOUT);
+#pragma unroll 1
+    for (int b = 0; b < kStages; ++b) mbar_wait_bounded(my_bar + 8 * b, parity >> b & 1, kPolls);
+  }
+}
+
+// The heads of a token side by side, whole vectors, 32 columns at most, and a token for every warp.
+template <typename T, int N, bool INTER>
+bool streams(const oc_rotary_args& a, int& columns) {
+  const int half = a.rotary_dim / 2;
+  columns = (INTER ? a.rotary_dim : half) / N + (a.head_dim - a.rotary_dim) / N;
+  auto dense = [&](const void* p, int64_t head_stride, int heads) { return !p || heads == 1 || head_stride == a.head_dim; };
+  return columns <= 32 && a.head_dim * (int)sizeof(T) <= kStageBytes && a.tokens >= (int64_t)a.num_sms * kStreamWarps &&
+         dense(a.q, a.q_head_stride, a.q_heads) && dense(a.k, a.k_head_stride, a.kv_heads) &&
+         dense(a.v, a.v_head_stride, a.kv_heads) && aligned_to(a.cos_tab, 16) && aligned_to(a.sin_tab, 16) && half % 4 == 0;
+}
+
+template <typename T, typename C, int N, bool INTER>
+int launch_aligned(const oc_rotary_args& a, void* stream) {
+  int columns;
+  if (!streams<T, N, INTER>(a, columns)) return launch<T, C, N, true, INTER>(a, stream);
+  constexpr int smem = kStreamWarps * kStages * kStageBytes;
+  auto kernel = rotary_stream_kernel<T, C, N, INTER>;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
+    cudaGetLastError();
+    return OC_ERR_CUDA;
+  }
+  const int64_t ctas = (a.tokens + kStreamWarps - 1) / kStreamWarps;
+  return launch_pdl(kernel, dim3((unsigned)(ctas < a.num_sms ? ctas : a.num_sms)), dim3(kStreamWarps * 32), smem, stream,
+                    a, columns);
+}
+
 // 16-byte vectors of T where every row starts at a multiple of 16 bytes and
 // the rotated part splits into whole vectors; else elements one by one.
 template <typename T, typename C>
@@ -214,7 +472,7 @@ int dispatch(const oc_rotary_args& a, void* stream) {
   ok(a.k_out, a.ko_tok_stride, a.ko_head_stride, 0, 16);
   ok(a.k_cache, a.kc_block_stride, a.kc_head_stride, a.kc_tok_stride, N * sizeof(C));
   ok(a.v_cache, a.vc_block_stride, a.vc_head_stride, a.vc_tok_stride, N * sizeof(C));
-  if (vec) return inter ? launch<T, C, N, true, true>(a, stream) : launch<T, C, N, true, false>(a, stream);
+  if (vec) return inter ? launch_aligned<T, C, N, true>(a, stream) : launch_aligned<T, C, N, false>(a, stream);
   return inter ? launch<T, C, 2, false, true>(a, stream) : launch<T, C, 1, false, false>(a, stream);
 }
 
@@ -230,7 +488,8 @@ extern "C" int oc_rotary_append_paged(const oc_rotary_args* args, void* stream) 
   if (!a.positions || (a.q_heads && (!a.q || !a.q_out)) || (a.kv_heads && (!a.k || (!a.k_out && !a.k_cache))) ||
       (a.rotary_dim && (!a.cos_tab || !a.sin_tab || a.table_rows < 1)))
     return OC_ERR_INVALID;
-  if (a.k_cache && (!a.v_cache || !a.v || !a.kv_heads || !a.block_tables || a.block_size < 1 || a.max_blocks < 0 ||
+  if (a.k_cache && (!a.v_cache || !a.v || !a.kv_heads || !a.block_tables || a.block_size < 1 || (a.block_size & (a.block_size - 1)) ||
+                    a.max_blocks < 0 ||
                     a.num_seqs < 0 || a.num_blocks < 0))
     return OC_ERR_INVALID;
   if (!a.k_cache && (a.v || a.v_cache)) return OC_ERR_INVALID;

@@ -456,8 +456,10 @@ struct CacheList {
       TORCH_CHECK_VALUE(c.dim() >= 2, "a cache must be (num_blocks, ...), got ", c.sizes());
       const int64_t es = c.element_size(), pages = c.size(0);
       const int64_t bytes = pages ? c.numel() / pages * es : 0;
-      TORCH_CHECK_VALUE(pages == 0 || (c.select(0, 0).is_contiguous() && c.stride(0) * es >= bytes && bytes > 0),
-                        "a page of a cache must be contiguous, got strides ", c.strides());
+      bool dense = bytes > 0 && c.stride(0) * es >= bytes;  // a page of contiguous elements
+      for (int64_t i = c.dim() - 1, run = 1; dense && i > 0; run *= c.size(i--))
+        dense = c.size(i) == 1 || c.stride(i) == run;
+      TORCH_CHECK_VALUE(pages == 0 || dense, "a page of a cache must be contiguous, got strides ", c.strides());
       if (!base.empty())
         TORCH_CHECK_VALUE(pages == num_pages && (pages == 0 || bytes == page_bytes),
                           "the caches must have pages of one size and number");
