@@ -8,6 +8,7 @@
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 
 #include "../../include/orthocache_b200.h"
@@ -78,6 +79,21 @@ inline int launch_pdl(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, 
     return OC_ERR_CUDA;
   }
   return OC_OK;
+}
+
+// Lets a kernel use `bytes` of dynamic shared memory on the current device.
+// The attribute outlives the call: `done` (one per kernel) remembers the
+// devices that have it.
+inline bool allow_smem(const void* kernel, std::atomic<uint64_t>& done, int bytes) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  if (dev < 64 && (done.load(std::memory_order_relaxed) >> dev & 1)) return true;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
+    cudaGetLastError();
+    return false;
+  }
+  if (dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
+  return true;
 }
 
 __device__ __forceinline__ void raise_status(uint32_t* status, uint32_t bits) {

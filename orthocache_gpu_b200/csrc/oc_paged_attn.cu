@@ -882,10 +882,8 @@ int launch_tiled(const oc_paged_decode_args& a, const Plan& p, void* stream) {
       !encode(&maps.v, maps.v_role, a.v_cache, a, a.vc_tok_stride, a.vc_head_stride, a.vc_block_stride, S::PANEL, rows))
     return launch_rows<T, C>(a, stream);
   auto kernel = p.direct ? decode_kernel<T, C, DP, NT, true> : decode_kernel<T, C, DP, NT, false>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM) != cudaSuccess) {
-    cudaGetLastError();
-    return OC_ERR_CUDA;
-  }
+  static std::atomic<uint64_t> ready[2];
+  if (!allow_smem(reinterpret_cast<const void*>(kernel), ready[p.direct], S::SMEM)) return OC_ERR_CUDA;
   int rc = launch_pdl(kernel, dim3((unsigned)p.grid), dim3(kWarps * 32), S::SMEM, stream, a, maps);
   if (rc != OC_OK || p.direct) return rc;
   return launch_pdl(join_kernel<T, DP, NT>, dim3((unsigned)(a.kv_heads * a.group), (unsigned)a.num_seqs), dim3(256), 0,

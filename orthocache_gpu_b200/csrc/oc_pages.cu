@@ -27,33 +27,44 @@ struct Caches {
 };
 
 // ------------------------------------------------------------------ block scan
-// Exclusive prefix sum of v over the CTA; total returns the sum.
-__device__ __forceinline__ int block_scan(int v, int& total) {
-  __shared__ int part[33];
+struct Two {
+  int a, b;
+};
+// Exclusive prefix sums of two counts over the CTA; total returns their sums.
+__device__ __forceinline__ Two block_scan(Two v, Two& total) {
+  __shared__ long long part[33];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  int x = v;
+  const long long own = (long long)v.a << 32 | (unsigned)v.b;  // no sum reaches 2^31
+  long long x = own;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    const long long y = __shfl_up_sync(0xffffffffu, x, o);
     if (lane >= o) x += y;
   }
   __syncthreads();  // part may still be read by an earlier call
   if (lane == 31) part[w] = x;
   __syncthreads();
   if (w == 0) {
-    int p = lane < (int)(blockDim.x >> 5) ? part[lane] : 0;
-    const int own = p;
+    const long long mine = lane < (int)(blockDim.x >> 5) ? part[lane] : 0;
+    long long p = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, p, o);
+      const long long y = __shfl_up_sync(0xffffffffu, p, o);
       if (lane >= o) p += y;
     }
-    part[lane] = p - own;
+    part[lane] = p - mine;
     if (lane == 31) part[32] = p;
   }
   __syncthreads();
-  total = part[32];
-  return part[w] + x - v;
+  total = Two{(int)(part[32] >> 32), (int)(part[32] & 0xffffffff)};
+  const long long before = part[w] + x - own;
+  return Two{(int)(before >> 32), (int)(before & 0xffffffff)};
+}
+
+// Four counts from index i on; beyond n: `fill`.
+__device__ __forceinline__ int4 four_at(const int32_t* p, int64_t i, int64_t n, int fill) {
+  if (i + 4 <= n && (reinterpret_cast<uintptr_t>(p + i) & 15) == 0) return *reinterpret_cast<const int4*>(p + i);
+  return int4{i < n ? p[i] : fill, i + 1 < n ? p[i + 1] : fill, i + 2 < n ? p[i + 2] : fill, i + 3 < n ? p[i + 3] : fill};
 }
 
 // ------------------------------------------------------------------ page copies
@@ -216,10 +227,8 @@ int copy_all(void* const* caches, const int64_t* strides, int num_caches, int64_
       int64_t ctas = (pieces + kCopyWarps - 1) / kCopyWarps;
       if (table.out && ctas < entries / (kCopyWarps * 32) + 1) ctas = entries / (kCopyWarps * 32) + 1;
       ctas = ctas < 1 ? 1 : ctas < num_sms ? ctas : num_sms;
-      if (cudaFuncSetAttribute(copy_bulk_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
-        cudaGetLastError();
-        return OC_ERR_CUDA;
-      }
+      static std::atomic<uint64_t> ready;
+      if (!allow_smem(reinterpret_cast<const void*>(copy_bulk_kernel), ready, smem)) return OC_ERR_CUDA;
       rc = launch_pdl(copy_bulk_kernel, (unsigned)ctas, kCopyWarps * 32, smem, stream, c, job, table, status);
     } else {
       rc = launch_pdl(copy_bytes_kernel, (unsigned)num_sms * 8, 256, 0, stream, c, job, table, status);
@@ -231,9 +240,9 @@ int copy_all(void* const* caches, const int64_t* strides, int num_caches, int64_
 }
 
 // ------------------------------------------------------------------ fork
-// One cluster.  Phase 1 copies the counts; after the cluster's barrier, phase
-// 2 writes the rows and adds what came and went (integer atomics: any order
-// gives the same counts).
+// One cluster.  The counts are copied and the first entries of both tables
+// read; after the cluster's barrier, what came and went is added (integer
+// atomics: any order gives the same counts).
 __global__ void __launch_bounds__(kThreads) fork_kernel(const int32_t* table_in, int64_t in_stride, int32_t* table_out,
                                                         int64_t out_stride, const int32_t* lens_in, int32_t* lens_out,
                                                         const int32_t* refs_in, int32_t* refs_out,
@@ -241,134 +250,140 @@ __global__ void __launch_bounds__(kThreads) fork_kernel(const int32_t* table_in,
                                                         int64_t num_pages, int block_size, uint32_t* status) {
   pdl_launch_dependents();
   pdl_wait();
+  constexpr int kEntries = 4;  // of a thread at a time
   const int64_t me = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, all = (int64_t)gridDim.x * blockDim.x;
+  const int64_t entries = (int64_t)num_seqs * max_blocks;
+  auto source_of = [&](int row) {
+    const int from = source[row];
+    if (from < num_seqs) return from;
+    raise_status(status, OC_STATUS_POSITION);
+    return row;
+  };
   for (int64_t i = me; i < num_pages; i += all) refs_out[i] = refs_in[i];
-  cooperative_groups::this_cluster().sync();
-  // a warp per row
-  const int lane = threadIdx.x & 31;
-  for (int64_t row = me >> 5; row < num_seqs; row += all >> 5) {
-    int from = source[row];
-    if (from >= num_seqs) {
-      if (lane == 0) raise_status(status, OC_STATUS_POSITION);
-      from = (int)row;
-    }
-    const bool stays = from == row;
-    const int len = from >= 0 ? lens_in[from] : 0;
-    const int used = stays ? max_blocks : min(max_blocks, (len + block_size - 1) / block_size);
-    if (lane == 0) lens_out[row] = len;
-    for (int c = lane; c < max_blocks; c += 32) {
-      const int old = table_in[row * in_stride + c];
-      const int now = stays ? old : from >= 0 && c < used ? table_in[(int64_t)from * in_stride + c] : -1;
-      table_out[row * out_stride + c] = now;
-      if (stays) continue;
-      if (old >= num_pages || now >= num_pages) {
-        raise_status(status, OC_STATUS_BAD_PAGE);
-        continue;
+  for (int64_t r = me; r < num_seqs; r += all) {
+    const int from = source_of((int)r);
+    lens_out[r] = from >= 0 ? lens_in[from] : 0;
+  }
+  for (int64_t base = 0; base < entries; base += all * kEntries) {
+    int old[kEntries], now[kEntries];
+#pragma unroll
+    for (int i = 0; i < kEntries; ++i) {
+      const int64_t e = base + i * all + me;
+      old[i] = now[i] = -1;
+      if (e >= entries) continue;
+      const int row = (int)(e / max_blocks), c = (int)(e - (int64_t)row * max_blocks);
+      const int from = source_of(row);
+      old[i] = now[i] = table_in[row * in_stride + c];
+      if (from != row) {
+        now[i] = -1;
+        if (from >= 0) {
+          const int page = table_in[from * in_stride + c], len = lens_in[from];
+          if ((int64_t)c * block_size < len) now[i] = page;
+        }
       }
-      if (old == now) continue;
-      if (old >= 0) atomicSub(refs_out + old, 1);
-      if (now >= 0) atomicAdd(refs_out + now, 1);
+      table_out[row * out_stride + c] = now[i];
+      if (from != row && (old[i] >= num_pages || now[i] >= num_pages)) {
+        raise_status(status, OC_STATUS_BAD_PAGE);
+        old[i] = now[i] = -1;
+      }
+    }
+    if (base == 0) cooperative_groups::this_cluster().sync();  // refs_out holds the old counts
+#pragma unroll
+    for (int i = 0; i < kEntries; ++i) {
+      if (old[i] == now[i]) continue;
+      if (old[i] >= 0) atomicSub(refs_out + old[i], 1);
+      if (now[i] >= 0) atomicAdd(refs_out + now[i], 1);
     }
   }
 }
 
 // ------------------------------------------------------------------ reserve
-// Workspace: [0] copies, [1] unused, then src[num_seqs], dst[num_seqs], and
-// the free pages handed out, free[num_pages].
+// Workspace: [0] copies, then src[num_seqs], dst[num_seqs], and the free pages
+// handed out, free[num_pages].
 struct ReserveSpace {
   int32_t *count, *src, *dst, *free;
   __host__ __device__ ReserveSpace(void* p, int num_seqs)
       : count(static_cast<int32_t*>(p)), src(count + 4), dst(src + num_seqs), free(dst + num_seqs) {}
 };
 
-// One CTA.  Rows are taken in runs, one run per thread, so that the prefix sum
-// over threads is the prefix sum over rows.  Shared memory: per row the page
-// it shares and would write to (or -1), and whether it copies it.
+// One CTA.  What a row needs is worked out with rows spread over the threads
+// and kept in shared memory; they are then taken in runs, one run per thread,
+// so that the prefix sum over threads is the prefix sum over rows.
 __global__ void __launch_bounds__(kThreads) reserve_kernel(int32_t* table, int64_t stride, const int32_t* lens,
                                                            int32_t* refs, const int32_t* wanted, int num_seqs,
                                                            int max_blocks, int64_t num_pages, int block_size,
                                                            void* workspace, uint32_t* status) {
-  extern __shared__ int32_t shared_page[];  // num_seqs
+  extern __shared__ int2 rows[];  // x: the page that the row shares and would write to, or -1; y: pages that it holds
   __shared__ int32_t short_list[kShortList];
   __shared__ int bad;
   pdl_launch_dependents();
   pdl_wait();
   const ReserveSpace ws(workspace, num_seqs);
-  if (threadIdx.x == 0) bad = 0;
   // the counts of the first pages, read ahead of the rows that will ask for them
-  const bool quads = (reinterpret_cast<uintptr_t>(refs) & 15) == 0;
-  auto counts_at = [&](int64_t i) {
-    if (quads && i + 4 <= num_pages) return *reinterpret_cast<const int4*>(refs + i);
-    int4 r = {1, 1, 1, 1};
-    if (i < num_pages) r.x = refs[i];
-    if (i + 1 < num_pages) r.y = refs[i + 1];
-    if (i + 2 < num_pages) r.z = refs[i + 2];
-    if (i + 3 < num_pages) r.w = refs[i + 3];
-    return r;
-  };
-  const int4 first_counts = counts_at((int64_t)threadIdx.x * 4);
-  // 1: the page that a growing sequence would write to and others hold too
+  const int4 first_counts = four_at(refs, (int64_t)threadIdx.x * 4, num_pages, 1);
+  if (threadIdx.x == 0) bad = 0;
+  __syncthreads();
+  // 1: the page that a growing sequence would write to and others hold too; the pages that it has
   for (int r = threadIdx.x; r < num_seqs; r += blockDim.x) {
     const int len = lens[r], part = len / block_size;
-    int page = -1;
-    if (wanted[r] > len && len > 0 && len % block_size != 0 && part < max_blocks) {
-      const int p = table[r * stride + part];
+    const int64_t goal = ((int64_t)wanted[r] + block_size - 1) / block_size;
+    int page = -1, held = (int)(((int64_t)len + block_size - 1) / block_size);
+    if (len < 0 || goal > max_blocks) {
+      bad = 1;
+    } else {
+      const bool inside = wanted[r] > len && len % block_size != 0 && part < max_blocks;
+      const int p = inside ? table[r * stride + part] : -1;
+      while (held < goal && table[r * stride + held] >= 0) ++held;
       if (p >= 0 && p < num_pages && refs[p] > 1) page = p;
     }
-    shared_page[r] = page;
+    rows[r] = int2{page, held};
   }
   __syncthreads();
   // 2: what each row needs
   const int per = (num_seqs + blockDim.x - 1) / blockDim.x, r0 = threadIdx.x * per, r1 = min(num_seqs, r0 + per);
-  int need = 0;
-  unsigned long long copies = 0;  // one bit per row of the run (per <= 64)
+  Two need = {0, 0};  // pages, and copies among them
+  unsigned copies = 0;  // one bit per row of the run
   for (int r = r0; r < r1; ++r) {
-    const int p = shared_page[r];
+    const int p = rows[r].x;
     if (p >= 0) {
       int writers = 0, last = -1;
       for (int o = 0; o < num_seqs; ++o)
-        if (shared_page[o] == p) {
+        if (rows[o].x == p) {
           ++writers;
           last = o;
         }
       // if every holder writes, the last of them keeps the page
       if (!(writers == refs[p] && last == r)) {
-        copies |= 1ull << (r - r0);
-        ++need;
+        copies |= 1u << (r - r0);
+        ++need.a;
+        ++need.b;
       }
     }
-    const int len = lens[r], goal = (int)(((int64_t)wanted[r] + block_size - 1) / block_size);
-    if (len < 0 || goal > max_blocks) {
-      bad = 1;
-      continue;
-    }
-    int held = (len + block_size - 1) / block_size;
-    while (held < goal && table[r * stride + held] >= 0) ++held;
-    need += goal > held ? goal - held : 0;
+    const int goal = (int)(((int64_t)wanted[r] + block_size - 1) / block_size);
+    need.a += !bad && goal > rows[r].y ? goal - rows[r].y : 0;
   }
-  int total;
-  int rank = block_scan(need, total);
+  Two total;
+  const Two before = block_scan(need, total);
+  int rank = before.a, copied = before.b;
   // 3: the lowest free pages
-  int32_t* const list = total <= kShortList ? short_list : ws.free;
+  int32_t* const list = total.a <= kShortList ? short_list : ws.free;
   int found = 0;
-  for (int64_t base = 0; base < num_pages && found < total; base += (int64_t)blockDim.x * 4) {
+  for (int64_t base = 0; base < num_pages && found < total.a; base += (int64_t)blockDim.x * 4) {
     const int64_t i = base + threadIdx.x * 4;
-    const int4 r = base == 0 ? first_counts : counts_at(i);
+    const int4 r = base == 0 ? first_counts : four_at(refs, i, num_pages, 1);
     const int f[4] = {r.x == 0, r.y == 0, r.z == 0, r.w == 0};
-    int sum;
-    int at = found + block_scan(f[0] + f[1] + f[2] + f[3], sum);
+    Two sum;
+    int at = found + block_scan(Two{f[0] + f[1] + f[2] + f[3], 0}, sum).a;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       if (f[j]) {
-        if (at < total) list[at] = (int32_t)(i + j);
+        if (at < total.a) list[at] = (int32_t)(i + j);
         ++at;
       }
-    found += sum;
+    found += sum.a;
   }
-  __syncthreads();  // the list and bad are complete
-  int copied_before, all_copies;
-  copied_before = block_scan(__popcll(copies), all_copies);
-  if (bad || found < total) {
+  __syncthreads();  // the list is complete
+  if (bad || found < total.a) {
     if (threadIdx.x == 0) {
       raise_status(status, OC_STATUS_PAGES);
       *ws.count = 0;
@@ -377,24 +392,22 @@ __global__ void __launch_bounds__(kThreads) reserve_kernel(int32_t* table, int64
   }
   // 4: hand them out (pages that are handed out were free: no count below is read above)
   for (int r = r0; r < r1; ++r) {
-    const int len = lens[r], goal = (int)(((int64_t)wanted[r] + block_size - 1) / block_size);
     if (copies >> (r - r0) & 1) {
-      const int p = shared_page[r], q = list[rank++];
-      table[r * stride + len / block_size] = q;
+      const int p = rows[r].x, q = list[rank++];
+      table[r * stride + lens[r] / block_size] = q;
       refs[q] = 1;
       atomicSub(refs + p, 1);
-      ws.src[copied_before] = p;
-      ws.dst[copied_before++] = q;
+      ws.src[copied] = p;
+      ws.dst[copied++] = q;
     }
-    int held = (len + block_size - 1) / block_size;
-    while (held < goal && table[r * stride + held] >= 0) ++held;
-    for (; held < goal; ++held) {
+    const int goal = (int)(((int64_t)wanted[r] + block_size - 1) / block_size);
+    for (int c = rows[r].y; c < goal; ++c) {
       const int q = list[rank++];
-      table[r * stride + held] = q;
+      table[r * stride + c] = q;
       refs[q] = 1;
     }
   }
-  if (threadIdx.x == 0) *ws.count = all_copies;
+  if (threadIdx.x == 0) *ws.count = total.b;
 }
 
 // ------------------------------------------------------------------ compact
@@ -410,24 +423,29 @@ __global__ void __launch_bounds__(kThreads) compact_plan_kernel(const int32_t* r
   pdl_launch_dependents();
   pdl_wait();
   const CompactSpace ws(workspace, num_pages);
-  int live = 0;
-  for (int64_t i = threadIdx.x; i < num_pages; i += blockDim.x) live += refs_in[i] > 0;
-  int n;
-  block_scan(live, n);
+  const int64_t chunk = (int64_t)blockDim.x * 4;
+  const int4 first = four_at(refs_in, (int64_t)threadIdx.x * 4, num_pages, 0);
+  int live = (first.x > 0) + (first.y > 0) + (first.z > 0) + (first.w > 0);
+  for (int64_t i = chunk + threadIdx.x * 4; i < num_pages; i += chunk) {
+    const int4 r = four_at(refs_in, i, num_pages, 0);
+    live += (r.x > 0) + (r.y > 0) + (r.z > 0) + (r.w > 0);
+  }
+  Two sum;
+  block_scan(Two{live, 0}, sum);
+  const int n = sum.a;
   int holes = 0, movers = 0;
-  for (int64_t base = 0; base < num_pages; base += (int64_t)blockDim.x * 4) {
+  for (int64_t base = 0; base < num_pages; base += chunk) {
     const int64_t i0 = base + threadIdx.x * 4;
-    int h = 0, m = 0;
-    int32_t ref[4];
+    const int4 r = base == 0 ? first : four_at(refs_in, i0, num_pages, 0);
+    const int ref[4] = {r.x, r.y, r.z, r.w};
+    Two c = {0, 0};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int64_t i = i0 + j;
-      ref[j] = i < num_pages ? refs_in[i] : 0;
-      h += i < n && ref[j] <= 0;
-      m += i >= n && ref[j] > 0;
+      c.a += i0 + j < n && ref[j] <= 0;
+      c.b += i0 + j >= n && ref[j] > 0;
     }
-    int hs, ms;
-    int hat = holes + block_scan(h, hs), mat = movers + block_scan(m, ms);
+    const Two before = block_scan(c, sum);
+    int hat = holes + before.a, mat = movers + before.b;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int64_t i = i0 + j;
@@ -438,8 +456,8 @@ __global__ void __launch_bounds__(kThreads) compact_plan_kernel(const int32_t* r
       else ws.to[i] = (int32_t)i;
       refs_out[i] = i < n && used ? ref[j] : 0;
     }
-    holes += hs;
-    movers += ms;
+    holes += sum.a;
+    movers += sum.b;
   }
   __syncthreads();
   for (int i = threadIdx.x; i < movers; i += blockDim.x) {  // as many holes as movers
@@ -457,7 +475,7 @@ bool bad_caches(void* const* caches, const int64_t* strides, int num_caches, int
   return false;
 }
 
-constexpr int kMaxSeqs = 8192;  // rows of one reserve call (their shared pages are held in shared memory)
+constexpr int kMaxSeqs = 4096;  // rows of one reserve call (their needs are held in shared memory)
 
 }  // namespace
 
@@ -483,14 +501,16 @@ extern "C" int oc_fork_sequences(const int32_t* table_in, int64_t table_in_strid
     return OC_ERR_INVALID;
   if (num_seqs == 0 && num_pages == 0) return OC_OK;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(8);
+  // small tables: one CTA, whose barrier is cheaper than a cluster's; one entry per thread and round else
+  const unsigned ctas = (int64_t)num_seqs * max_blocks + num_pages <= 16 * kThreads ? 1 : 8;
+  cfg.gridDim = dim3(ctas);
   cfg.blockDim = dim3(kThreads);
   cfg.stream = static_cast<cudaStream_t>(stream);
   cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
   at[1].id = cudaLaunchAttributeClusterDimension;
-  at[1].val.clusterDim.x = 8;
+  at[1].val.clusterDim.x = ctas;
   at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 2;
@@ -521,7 +541,7 @@ extern "C" int oc_reserve_pages(void* const* caches, const int64_t* page_strides
   if (num_seqs == 0) return OC_OK;
   if (!workspace || !aligned_to(workspace, 4) || workspace_bytes < oc_reserve_workspace_bytes(num_seqs, num_pages))
     return OC_ERR_WORKSPACE;
-  const int rc = launch_pdl(reserve_kernel, 1, kThreads, num_seqs * sizeof(int32_t), stream, table, table_stride, lens,
+  const int rc = launch_pdl(reserve_kernel, 1, kThreads, num_seqs * sizeof(int2), stream, table, table_stride, lens,
                             refs, wanted, num_seqs, max_blocks, num_pages, block_size, workspace, status);
   if (rc != OC_OK || num_caches == 0) return rc;
   const ReserveSpace ws(workspace, num_seqs);

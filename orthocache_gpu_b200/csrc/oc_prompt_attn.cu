@@ -671,10 +671,8 @@ bool encode(CUtensorMap* map, int& swap, const void* base, int dtype, int head_d
 template <typename T, int DP, bool GENERAL>
 int launch_tiled(const oc_prompt_args& a, const Maps& maps, unsigned tiles, void* stream) {
   auto kernel = prompt_kernel<T, DP, GENERAL>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<DP>::SMEM) != cudaSuccess) {
-    cudaGetLastError();
-    return OC_ERR_CUDA;
-  }
+  static std::atomic<uint64_t> ready;
+  if (!allow_smem(reinterpret_cast<const void*>(kernel), ready, Tile<DP>::SMEM)) return OC_ERR_CUDA;
   return launch_pdl(kernel, dim3((unsigned)(a.kv_heads * a.group), tiles), dim3(kThreads), Tile<DP>::SMEM, stream, a,
                     maps);
 }

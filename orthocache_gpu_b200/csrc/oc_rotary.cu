@@ -445,10 +445,8 @@ int launch_aligned(const oc_rotary_args& a, void* stream) {
   if (!streams<T, N, INTER>(a, columns)) return launch<T, C, N, true, INTER>(a, stream);
   constexpr int smem = kStreamWarps * kStages * kStageBytes;
   auto kernel = rotary_stream_kernel<T, C, N, INTER>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
-    cudaGetLastError();
-    return OC_ERR_CUDA;
-  }
+  static std::atomic<uint64_t> ready;
+  if (!allow_smem(reinterpret_cast<const void*>(kernel), ready, smem)) return OC_ERR_CUDA;
   const int64_t ctas = (a.tokens + kStreamWarps - 1) / kStreamWarps;
   return launch_pdl(kernel, dim3((unsigned)(ctas < a.num_sms ? ctas : a.num_sms)), dim3(kStreamWarps * 32), smem, stream,
                     a, columns);

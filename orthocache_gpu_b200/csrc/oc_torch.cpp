@@ -8,6 +8,7 @@
 // (include/orthocache_b200.h) directly; it adds no GPU code.  The serving
 // operators check their arguments here too: ValueError for shapes and sizes,
 // TypeError for dtypes, RuntimeError for devices.
+#include <torch/csrc/autograd/python_variable.h>
 #include <torch/extension.h>
 
 #include <cstdint>
@@ -450,23 +451,36 @@ struct CacheList {
   std::vector<int64_t> stride;
   int64_t page_bytes = 1, num_pages = 0;
 
-  CacheList(const std::vector<Tensor>& caches, const Tensor& like) {
-    for (const Tensor& c : caches) {
+  // a list or tuple of tensors, looked at without a conversion: a model has tens of caches, a call a few us
+  CacheList(py::handle caches, const Tensor& like) {
+    const bool list = PyList_Check(caches.ptr());
+    TORCH_CHECK_TYPE(list || PyTuple_Check(caches.ptr()), "caches must be a list or tuple of tensors");
+    const Py_ssize_t n = list ? PyList_GET_SIZE(caches.ptr()) : PyTuple_GET_SIZE(caches.ptr());
+    base.reserve(n);
+    stride.reserve(n);
+    const Tensor* first = nullptr;
+    for (Py_ssize_t i = 0; i < n; ++i) {
+      PyObject* o = list ? PyList_GET_ITEM(caches.ptr(), i) : PyTuple_GET_ITEM(caches.ptr(), i);
+      TORCH_CHECK_TYPE(THPVariable_Check(o), "caches must be a list or tuple of tensors");
+      const Tensor& c = THPVariable_Unpack(o);
       need_cuda(c, like);
-      TORCH_CHECK_VALUE(c.dim() >= 2, "a cache must be (num_blocks, ...), got ", c.sizes());
-      const int64_t es = c.element_size(), pages = c.size(0);
-      const int64_t bytes = pages ? c.numel() / pages * es : 0;
-      bool dense = bytes > 0 && c.stride(0) * es >= bytes;  // a page of contiguous elements
-      for (int64_t i = c.dim() - 1, run = 1; dense && i > 0; run *= c.size(i--))
-        dense = c.size(i) == 1 || c.stride(i) == run;
-      TORCH_CHECK_VALUE(pages == 0 || dense, "a page of a cache must be contiguous, got strides ", c.strides());
-      if (!base.empty())
-        TORCH_CHECK_VALUE(pages == num_pages && (pages == 0 || bytes == page_bytes),
+      if (!first || c.scalar_type() != first->scalar_type() || c.sizes() != first->sizes() ||
+          c.strides() != first->strides()) {
+        TORCH_CHECK_VALUE(c.dim() >= 2, "a cache must be (num_blocks, ...), got ", c.sizes());
+        const int64_t es = c.element_size(), pages = c.size(0);
+        const int64_t bytes = pages ? c.numel() / pages * es : 0;
+        bool dense = bytes > 0 && c.stride(0) * es >= bytes;  // a page of contiguous elements
+        for (int64_t d = c.dim() - 1, run = 1; dense && d > 0; run *= c.size(d--))
+          dense = c.size(d) == 1 || c.stride(d) == run;
+        TORCH_CHECK_VALUE(pages == 0 || dense, "a page of a cache must be contiguous, got strides ", c.strides());
+        TORCH_CHECK_VALUE(!first || (pages == num_pages && (pages == 0 || bytes == page_bytes)),
                           "the caches must have pages of one size and number");
-      num_pages = pages;
-      if (pages) page_bytes = bytes;
+        num_pages = pages;
+        if (pages) page_bytes = bytes;
+        first = &c;
+      }
       base.push_back(c.data_ptr());
-      stride.push_back(c.stride(0) * es);
+      stride.push_back(c.stride(0) * (int64_t)c.element_size());
     }
     if (num_pages == 0) base.clear();  // nothing to move
   }
@@ -485,7 +499,7 @@ void need_len(const Tensor& t, int64_t n, const char* name) {
   TORCH_CHECK_VALUE(t.size(0) == n, name, " must be (", n, ",), got ", t.sizes());
 }
 
-void copy_pages(const std::vector<Tensor>& caches, const Tensor& src_, const Tensor& dst_, int64_t num_sms,
+void copy_pages(py::handle caches, const Tensor& src_, const Tensor& dst_, int64_t num_sms,
                 int64_t status, int64_t stream) {
   need_cuda(src_, src_);
   const c10::DeviceGuard guard(src_.device());
@@ -523,7 +537,7 @@ std::tuple<Tensor, Tensor, Tensor> fork_sequences(const Tensor& tables, const Te
   return {t, l, r};
 }
 
-void reserve_pages(const std::vector<Tensor>& caches, const Tensor& tables, const Tensor& lens, const Tensor& refs,
+void reserve_pages(py::handle caches, const Tensor& tables, const Tensor& lens, const Tensor& refs,
                    const Tensor& wanted_, int64_t block_size, int64_t num_sms, int64_t status, int64_t stream) {
   need_int32(tables, tables, "block_tables", 2);
   const c10::DeviceGuard guard(tables.device());
@@ -549,7 +563,7 @@ void reserve_pages(const std::vector<Tensor>& caches, const Tensor& tables, cons
         "reserve_pages");
 }
 
-std::tuple<Tensor, Tensor> compact_pages(const std::vector<Tensor>& caches, const Tensor& tables, const Tensor& refs,
+std::tuple<Tensor, Tensor> compact_pages(py::handle caches, const Tensor& tables, const Tensor& refs,
                                          int64_t num_sms, int64_t status, int64_t stream) {
   need_int32(tables, tables, "block_tables", 2);
   const c10::DeviceGuard guard(tables.device());

@@ -23,7 +23,7 @@ def copy_pages(caches: Sequence[torch.Tensor], src: torch.Tensor, dst: torch.Ten
 
     A negative id skips the pair; no dst may be the src or dst of another pair.
     """
-    _lib.require_binding().copy_pages(list(caches), src, dst, *_lib.call_context(src))
+    _lib.require_binding().copy_pages(caches, src, dst, *_lib.call_context(src))
 
 
 def fork_sequences(block_tables: torch.Tensor, seq_lens: torch.Tensor, refcounts: torch.Tensor, source: torch.Tensor,
@@ -49,7 +49,7 @@ def reserve_pages(caches: Sequence[torch.Tensor], block_tables: torch.Tensor, se
     and the stream's status word is set, so check it (:func:`check_status`) before the rows are written to.
     ``seq_lens`` does not change.
     """
-    _lib.require_binding().reserve_pages(list(caches), block_tables, seq_lens, refcounts, wanted, block_size,
+    _lib.require_binding().reserve_pages(caches, block_tables, seq_lens, refcounts, wanted, block_size,
                                          *_lib.call_context(block_tables))
 
 
@@ -60,7 +60,7 @@ def compact_pages(caches: Sequence[torch.Tensor], block_tables: torch.Tensor,
     Cache contents move in place: the k-th used page at or above n goes to the k-th free one below it, so
     pages already below n stay.
     """
-    return _lib.require_binding().compact_pages(list(caches), block_tables, refcounts,
+    return _lib.require_binding().compact_pages(caches, block_tables, refcounts,
                                                 *_lib.call_context(block_tables))
 
 
