@@ -61,6 +61,10 @@ __device__ __forceinline__ Two block_scan(Two v, Two& total) {
   return Two{(int)(before >> 32), (int)(before & 0xffffffff)};
 }
 
+__device__ __forceinline__ int pages_for(int tokens, int block_size) {  // 32-bit arithmetic, for any tokens >= 0
+  return (int)(((unsigned)tokens + (unsigned)block_size - 1u) / (unsigned)block_size);
+}
+
 // Four counts from index i on; beyond n: `fill`.
 __device__ __forceinline__ int4 four_at(const int32_t* p, int64_t i, int64_t n, int fill) {
   if (i + 4 <= n && (reinterpret_cast<uintptr_t>(p + i) & 15) == 0) return *reinterpret_cast<const int4*>(p + i);
@@ -251,8 +255,8 @@ __global__ void __launch_bounds__(kThreads) fork_kernel(const int32_t* table_in,
   pdl_launch_dependents();
   pdl_wait();
   constexpr int kEntries = 4;  // of a thread at a time
-  const int64_t me = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, all = (int64_t)gridDim.x * blockDim.x;
-  const int64_t entries = (int64_t)num_seqs * max_blocks;
+  const unsigned me = blockIdx.x * blockDim.x + threadIdx.x, all = gridDim.x * blockDim.x;
+  const unsigned entries = (unsigned)num_seqs * (unsigned)max_blocks;
   auto source_of = [&](int row) {
     const int from = source[row];
     if (from < num_seqs) return from;
@@ -260,18 +264,18 @@ __global__ void __launch_bounds__(kThreads) fork_kernel(const int32_t* table_in,
     return row;
   };
   for (int64_t i = me; i < num_pages; i += all) refs_out[i] = refs_in[i];
-  for (int64_t r = me; r < num_seqs; r += all) {
+  for (unsigned r = me; r < (unsigned)num_seqs; r += all) {
     const int from = source_of((int)r);
     lens_out[r] = from >= 0 ? lens_in[from] : 0;
   }
-  for (int64_t base = 0; base < entries; base += all * kEntries) {
+  for (unsigned base = 0; base < entries; base += all * kEntries) {
     int old[kEntries], now[kEntries];
 #pragma unroll
     for (int i = 0; i < kEntries; ++i) {
-      const int64_t e = base + i * all + me;
+      const unsigned e = base + i * all + me;
       old[i] = now[i] = -1;
       if (e >= entries) continue;
-      const int row = (int)(e / max_blocks), c = (int)(e - (int64_t)row * max_blocks);
+      const int row = (int)(e / (unsigned)max_blocks), c = (int)(e - (unsigned)row * (unsigned)max_blocks);
       const int from = source_of(row);
       old[i] = now[i] = table_in[row * in_stride + c];
       if (from != row) {
@@ -326,8 +330,8 @@ __global__ void __launch_bounds__(kThreads) reserve_kernel(int32_t* table, int64
   // 1: the page that a growing sequence would write to and others hold too; the pages that it has
   for (int r = threadIdx.x; r < num_seqs; r += blockDim.x) {
     const int len = lens[r], part = len / block_size;
-    const int64_t goal = ((int64_t)wanted[r] + block_size - 1) / block_size;
-    int page = -1, held = (int)(((int64_t)len + block_size - 1) / block_size);
+    const int goal = pages_for(max(wanted[r], 0), block_size);
+    int page = -1, held = pages_for(max(len, 0), block_size);
     if (len < 0 || goal > max_blocks) {
       bad = 1;
     } else {
@@ -359,7 +363,7 @@ __global__ void __launch_bounds__(kThreads) reserve_kernel(int32_t* table, int64
         ++need.b;
       }
     }
-    const int goal = (int)(((int64_t)wanted[r] + block_size - 1) / block_size);
+    const int goal = pages_for(max(wanted[r], 0), block_size);
     need.a += !bad && goal > rows[r].y ? goal - rows[r].y : 0;
   }
   Two total;
@@ -400,7 +404,7 @@ __global__ void __launch_bounds__(kThreads) reserve_kernel(int32_t* table, int64
       ws.src[copied] = p;
       ws.dst[copied++] = q;
     }
-    const int goal = (int)(((int64_t)wanted[r] + block_size - 1) / block_size);
+    const int goal = pages_for(max(wanted[r], 0), block_size);
     for (int c = rows[r].y; c < goal; ++c) {
       const int q = list[rank++];
       table[r * stride + c] = q;
@@ -499,10 +503,10 @@ extern "C" int oc_fork_sequences(const int32_t* table_in, int64_t table_in_strid
       (num_seqs && max_blocks && (!table_in || !table_out || table_in == table_out)) ||
       (num_pages && (!refs_in || !refs_out || refs_in == refs_out)))
     return OC_ERR_INVALID;
+  if ((int64_t)num_seqs * max_blocks > 0x3fffffff) return OC_ERR_TOO_LARGE;
   if (num_seqs == 0 && num_pages == 0) return OC_OK;
   cudaLaunchConfig_t cfg = {};
-  // small tables: one CTA, whose barrier is cheaper than a cluster's; one entry per thread and round else
-  const unsigned ctas = (int64_t)num_seqs * max_blocks + num_pages <= 16 * kThreads ? 1 : 8;
+  constexpr unsigned ctas = 8;  // one CTA alone is slower even for small tables (10.6 against 6.9 us at 64 x 59 entries)
   cfg.gridDim = dim3(ctas);
   cfg.blockDim = dim3(kThreads);
   cfg.stream = static_cast<cudaStream_t>(stream);
