@@ -24,6 +24,7 @@
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
+#include <climits>
 #include <mutex>
 #include <utility>
 
@@ -36,7 +37,9 @@ using namespace oc;
 
 constexpr int kWarps = 4;
 constexpr int kBufs = 3;         // buffers of a warp's ring
-constexpr int kMinShare = 4;     // tiles that a CTA takes at least before a unit is split
+constexpr int kMinShare = 2;     // tiles that a CTA takes at least before a unit is split
+constexpr int kLongRun = 24;     // places per CTA from which runs have a finer tail
+constexpr int kTailPart = 4;     // which is one kTailPart-th of all places
 constexpr int kUnitCost = 3;     // what beginning and ending a unit costs, in tiles, when shares are equalised
 constexpr int kDirectTiles = 8;  // units of at most so many tiles get a CTA each and no joining launch
 constexpr uint32_t kPolls = 1u << 22;  // bound of a wait for a copy
@@ -168,12 +171,35 @@ struct Walk {
   }
 };
 
-// Workspace: header (the place before each sequence, and after all, then the
-// run length), then per CTA two states of 8 NT heads: acc, m, l.
+// How the places [0, total) are cut into runs, one per CTA.  The first `wave`
+// CTAs, those that are resident from the start, take equal runs.  SMs do not
+// stream equally fast (on this part some take 15% longer than the mean), so
+// where runs are long the last quarter of all places is cut finer and left to
+// `late` CTAs that start as others leave (16 ragged sequences of fp16: 110 to
+// 99 us).  Not with 8-bit caches, whose tiles are bound by their conversion,
+// the same on every SM (64 x 8192: 98 us without, 103 with).
+struct Runs {
+  int wave, big, small;
+  __device__ __forceinline__ Runs(int total, int wave, int late) : wave(wave) {
+    const bool tail = late > 0 && total >= kLongRun * wave;
+    big = tail ? (total - total / kTailPart) / wave : (total + wave - 1) / wave;
+    big = big < kMinShare ? kMinShare : big;
+    small = tail ? (total - big * wave + late - 1) / late : 1;
+  }
+  __device__ __forceinline__ int64_t start(int c) const {
+    return c < wave ? (int64_t)c * big : (int64_t)wave * big + (int64_t)(c - wave) * small;
+  }
+  __device__ __forceinline__ int owner(int place) const {
+    const int64_t first = (int64_t)wave * big;
+    return place < first ? place / big : wave + (int)(place - first) / small;
+  }
+};
+
+// Workspace: header (the place before each sequence, and after all), then per CTA two states of 8 NT heads: acc, m, l.
 struct Space {
-  int32_t* before;  // num_seqs + 1, then the run length
+  int32_t* before;  // num_seqs + 1
   float* states;
-  __host__ __device__ static size_t header(int num_seqs) { return (((size_t)num_seqs + 2) * 4 + 15) / 16 * 16; }
+  __host__ __device__ static size_t header(int num_seqs) { return (((size_t)num_seqs + 1) * 4 + 15) / 16 * 16; }
   __host__ __device__ Space(void* p, int num_seqs)
       : before(static_cast<int32_t*>(p)), states(reinterpret_cast<float*>(static_cast<char*>(p) + header(num_seqs))) {}
 };
@@ -189,7 +215,7 @@ struct Maps {
 
 template <typename T, typename C, int DP, int NT, bool DIRECT>
 __global__ void __launch_bounds__(kWarps * 32, Shape<sizeof(C), DP, NT>::PER_SM)
-    decode_kernel(const __grid_constant__ oc_paged_decode_args a, const __grid_constant__ Maps maps) {
+    decode_kernel(const __grid_constant__ oc_paged_decode_args a, const __grid_constant__ Maps maps, int late_ctas) {
   using S = Shape<sizeof(C), DP, NT>;
   constexpr bool F8 = sizeof(C) == 1;
   constexpr bool BF16 = !F8 && std::is_same<T, __nv_bfloat16>::value;  // 8-bit caches multiply in float16
@@ -227,46 +253,72 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<sizeof(C), DP, NT>::PER_SM)
     end = cs.tiles;
   } else {
     const Space ws(a.workspace, a.num_seqs);
-    int mine = 0, own = 0;  // own: of sequence threadIdx.x
-    for (int s = threadIdx.x; s < a.num_seqs; s += kWarps * 32) {
-      const int n = (tiles_of<S>(span_of(a, s)) + kUnitCost) * subs;
-      if (s == (int)threadIdx.x) own = n;
-      mine += n;
-    }
-    int total;
-    scan128(mine, total, part);
-    int share = (total + gridDim.x - 1) / gridDim.x;
-    share = share < kMinShare ? kMinShare : share;
-    const int64_t start = (int64_t)blockIdx.x * share;
-    if (start >= total && blockIdx.x != 0) return;
-    end = (int)min(start + share, (int64_t)total);
-    // the sequence that holds `start` (CTA 0 also leaves the prefix sums for the joining launch)
-    int base = 0;
-    for (int s0 = 0; s0 < a.num_seqs; s0 += kWarps * 32) {
-      const int s = s0 + threadIdx.x;
-      const int n = s >= a.num_seqs ? 0 : s0 == 0 ? own : (tiles_of<S>(span_of(a, s)) + kUnitCost) * subs;
-      int sum;
-      const int at = base + scan128(n, sum, part);
-      if (s < a.num_seqs && start >= at && start < at + n) {
-        const int unit = n / subs, off = (int)(start - at);
-        found[0] = s;
-        found[1] = off / unit;
-        found[2] = off % unit;
+    const int wave = (int)gridDim.x - late_ctas;
+    if (a.num_seqs <= 32) {  // each warp for itself, without a barrier
+      const Span sp = lane < a.num_seqs ? span_of(a, lane) : Span{0, 0};
+      const int n = lane < a.num_seqs ? (tiles_of<S>(sp) + kUnitCost) * subs : 0;
+      int up = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, up, o);
+        if (lane >= o) up += y;
       }
-      if (blockIdx.x == 0 && s < a.num_seqs) ws.before[s] = at;
-      base += sum;
-      if (blockIdx.x != 0 && start < base) break;
+      const int total = __shfl_sync(0xffffffffu, up, 31), at = up - n;
+      const Runs runs(total, wave, late_ctas);
+      const int64_t start = runs.start(blockIdx.x);
+      if (blockIdx.x == 0 && warp == 0) {  // for the joining launch
+        if (lane < a.num_seqs) ws.before[lane] = at;
+        if (lane == 0) ws.before[a.num_seqs] = total;
+      }
+      if (start >= total) return;
+      end = (int)min(runs.start(blockIdx.x + 1), (int64_t)total);
+      const int who = __ffs(__ballot_sync(0xffffffffu, start >= at && start < up)) - 1;
+      const int unit = __shfl_sync(0xffffffffu, n, who) / subs, off = (int)start - __shfl_sync(0xffffffffu, at, who);
+      cs.seq = who;
+      cs.sub = off / unit;
+      cs.tile = off % unit;
+      cs.at = (int)start;
+      cs.span.lo = __shfl_sync(0xffffffffu, sp.lo, who);
+      cs.span.n = __shfl_sync(0xffffffffu, sp.n, who);
+      cs.tiles = unit - kUnitCost;
+    } else {
+      int mine = 0, own = 0;  // own: of sequence threadIdx.x
+      for (int s = threadIdx.x; s < a.num_seqs; s += kWarps * 32) {
+        const int n = (tiles_of<S>(span_of(a, s)) + kUnitCost) * subs;
+        if (s == (int)threadIdx.x) own = n;
+        mine += n;
+      }
+      int total;
+      scan128(mine, total, part);
+      const Runs runs(total, wave, late_ctas);
+      const int64_t start = runs.start(blockIdx.x);
+      if (start >= total && blockIdx.x != 0) return;
+      end = (int)min(runs.start(blockIdx.x + 1), (int64_t)total);
+      // the sequence that holds `start` (CTA 0 also leaves the prefix sums for the joining launch)
+      int base = 0;
+      for (int s0 = 0; s0 < a.num_seqs; s0 += kWarps * 32) {
+        const int s = s0 + threadIdx.x;
+        const int n = s >= a.num_seqs ? 0 : s0 == 0 ? own : (tiles_of<S>(span_of(a, s)) + kUnitCost) * subs;
+        int sum;
+        const int at = base + scan128(n, sum, part);
+        if (s < a.num_seqs && start >= at && start < at + n) {
+          const int unit = n / subs, off = (int)(start - at);
+          found[0] = s;
+          found[1] = off / unit;
+          found[2] = off % unit;
+        }
+        if (blockIdx.x == 0 && s < a.num_seqs) ws.before[s] = at;
+        base += sum;
+        if (blockIdx.x != 0 && start < base) break;
+      }
+      if (blockIdx.x == 0 && threadIdx.x == 0) ws.before[a.num_seqs] = total;
+      __syncthreads();
+      cs.seq = found[0];
+      cs.sub = found[1];
+      cs.tile = found[2];
+      cs.at = (int)start;
+      cs.enter(a);
     }
-    if (blockIdx.x == 0 && threadIdx.x == 0) {
-      ws.before[a.num_seqs] = total;
-      ws.before[a.num_seqs + 1] = share;
-    }
-    __syncthreads();
-    cs.seq = found[0];
-    cs.sub = found[1];
-    cs.tile = found[2];
-    cs.at = (int)start;
-    cs.enter(a);
     if (cs.tile >= cs.tiles) {  // in the cost of a unit that others have done
       cs.at += cs.tiles + kUnitCost - cs.tile;
       cs.next_unit(a, subs);
@@ -280,31 +332,33 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<sizeof(C), DP, NT>::PER_SM)
   const int block_shift = __ffs(a.block_size) - 1;
   const int run_rows = a.block_size < S::KW ? a.block_size : S::KW, runs = S::KW / run_rows;
   Walk<S> ld = cs;
+  constexpr int kNoRun = INT_MIN;
   struct Source {
     bool on;             // there is such a tile
-    int page, slot, hk;  // of run `lane` (+ 32 where pages are single slots); page -1: nothing to copy
+    int page, slot, hk;  // of run `lane` (+ 32 where pages are single slots); kNoRun: nothing to copy
     int page2;
   };
-  // the pages of the next tile
+  // the pages of the next tile, as the table has them: nothing waits for them here
   auto look = [&]() {
-    Source p = {ld.at < end, -1, 0, 0, -1};
+    Source p = {ld.at < end, kNoRun, 0, 0, kNoRun};
     if (!p.on) return p;
     const int key0 = (ld.span.lo & -S::KW) + ld.tile * S::CT + warp * S::KW;
     p.hk = ld.sub / gtiles;
     const int32_t* table = a.block_tables + (int64_t)ld.seq * a.block_table_stride;
     auto page_of = [&](int r) {
       const int j = key0 + r * run_rows;
-      if (r >= runs || j >= ld.span.n || j + run_rows <= ld.span.lo) return -1;
-      const int page = table[j >> block_shift];
-      if (page >= 0 && page < a.num_blocks) return page;
-      raise_status(a.status, OC_STATUS_BAD_PAGE);
-      return -1;
+      return r >= runs || j >= ld.span.n || j + run_rows <= ld.span.lo ? kNoRun : table[j >> block_shift];
     };
     p.slot = key0 & (a.block_size - 1);  // 0 where a tile has several runs
     p.page = page_of(lane);
     if (S::KW > 32 && runs > 32) p.page2 = page_of(lane + 32);
     ld.next(a, subs);
     return p;
+  };
+  auto usable = [&](int page) {
+    if (page >= 0 && page < a.num_blocks) return true;
+    if (page != kNoRun) raise_status(a.status, OC_STATUS_BAD_PAGE);
+    return false;
   };
   const uint64_t policy = policy_evict_first();
   auto copy_run = [&](const CUtensorMap* map, const int* role, const Source& p, int page, int r, uint32_t buf,
@@ -318,13 +372,33 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<sizeof(C), DP, NT>::PER_SM)
   // fills buffer b with K (or V) of a tile
   auto issue = [&](const CUtensorMap* map, const int* role, const Source& p, int b) {
     const uint32_t buf = my_ring + b * S::BUF, bar = my_bar + 8 * b;
-    int n = __popc(__ballot_sync(0xffffffffu, p.page >= 0));
-    if (S::KW > 32) n += __popc(__ballot_sync(0xffffffffu, p.page2 >= 0));
+    const bool first = usable(p.page), second = S::KW > 32 && usable(p.page2);
+    int n = __popc(__ballot_sync(0xffffffffu, first));
+    if (S::KW > 32) n += __popc(__ballot_sync(0xffffffffu, second));
     if (lane == 0) mbar_arrive_expect_tx(bar, n * S::PANELS * run_rows * S::PANEL);
     __syncwarp();
-    if (p.page >= 0) copy_run(map, role, p, p.page, lane, buf, bar);
-    if (S::KW > 32 && p.page2 >= 0) copy_run(map, role, p, p.page2, lane + 32, buf, bar);
+    if (first) copy_run(map, role, p, p.page, lane, buf, bar);
+    if (second) copy_run(map, role, p, p.page2, lane + 32, buf, bar);
   };
+  // The unit's queries: head g, the columns of this lane's operand (8-bit keys come out of their conversion in
+  // another order: 4t, 4t + 1 | 4t + 2, 4t + 3).  Loads without branches, of a head and column that exist, so that
+  // all are on their way at once.
+  Vec<T, 4> query[NT][KS];
+  auto column = [&](int k, int e) { return k * 16 + (F8 ? 4 * t + e : 2 * t + (e & 1) + (e >> 1) * 8); };
+  auto load_query = [&]() {
+    const int first = (cs.sub % gtiles) * HT, heads = min(HT, a.group - first);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int hr = n * 8 + g;
+      const T* q = static_cast<const T*>(a.q) + (int64_t)cs.seq * a.q_seq_stride +
+                   (int64_t)(cs.sub / gtiles * a.group + first + (hr < heads ? hr : 0)) * a.q_head_stride;
+#pragma unroll
+      for (int k = 0; k < KS; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) query[n][k].e[e] = q[column(k, e) < a.head_dim ? column(k, e) : 0];
+    }
+  };
+  load_query();
   Source for_v, for_k;  // the tile whose values, and the one whose keys, are copied next
   {
     const Source s0 = look(), s1 = look();
@@ -354,8 +428,12 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<sizeof(C), DP, NT>::PER_SM)
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const int hr = n * 8 + g;
-      const T* q = static_cast<const T*>(a.q) + (int64_t)cs.seq * a.q_seq_stride + (int64_t)(h0 + hr) * a.q_head_stride;
-      auto at = [&](int d) { return hr < heads && d < a.head_dim ? to_f32(q[d]) : 0.f; };
+      float x[KS][4];
+#pragma unroll
+      for (int k = 0; k < KS; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          x[k][e] = hr < heads && column(k, e) < a.head_dim ? to_f32(query[n][k].e[e]) : 0.f;
       qscale[n] = 1.f;
       if constexpr (F8 && std::is_same<T, __nv_bfloat16>::value) {
         // bfloat16 queries go through float16 times a power of two that puts their largest below 2^8
@@ -363,7 +441,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<sizeof(C), DP, NT>::PER_SM)
 #pragma unroll
         for (int k = 0; k < KS; ++k)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(at(k * 16 + 4 * t + e)));
+          for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(x[k][e]));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         if (top > 0.f && top < INFINITY) {
@@ -374,15 +452,8 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<sizeof(C), DP, NT>::PER_SM)
       }
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
-        if constexpr (F8) {  // column order of the converted keys: 4t, 4t + 1 | 4t + 2, 4t + 3
-          const int d = k * 16 + 4 * t;
-          qf[k][n][0] = pack16<BF16>(at(d) * qscale[n], at(d + 1) * qscale[n]);
-          qf[k][n][1] = pack16<BF16>(at(d + 2) * qscale[n], at(d + 3) * qscale[n]);
-        } else {
-          const int d = k * 16 + 2 * t;
-          qf[k][n][0] = pack16<BF16>(at(d), at(d + 1));
-          qf[k][n][1] = pack16<BF16>(at(d + 8), at(d + 9));
-        }
+        qf[k][n][0] = pack16<BF16>(x[k][0] * qscale[n], x[k][1] * qscale[n]);
+        qf[k][n][1] = pack16<BF16>(x[k][2] * qscale[n], x[k][3] * qscale[n]);
       }
     }
 #pragma unroll
@@ -663,6 +734,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<sizeof(C), DP, NT>::PER_SM)
     kb = vb + 1 == kBufs ? 0 : vb + 1;
     cs.next(a, subs);
     if (cs.tile == 0) {
+      load_query();
       begin_unit();
       from_start = true;
     }
@@ -675,13 +747,14 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<sizeof(C), DP, NT>::PER_SM)
 }
 
 // Joins the partial states of the units that were split: one CTA per
-// (unit, head), its warps take the parts in turn, and their sums are added in
-// a fixed order.
+// (sequence, head); its warps take the parts in turn, and their states are
+// joined in a fixed order.
 template <typename T, int DP, int NT>
-__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ oc_paged_decode_args a) {
-  constexpr int HT = 8 * NT, W = 8;
-  __shared__ float sm[W][2];
-  __shared__ float so[W][DP];
+__global__ void __launch_bounds__(512) join_kernel(const __grid_constant__ oc_paged_decode_args a, int wave, int late_ctas) {
+  constexpr int HT = 8 * NT, MOST = 16;
+  const int W = blockDim.x >> 5;
+  __shared__ float sm[MOST][2];
+  __shared__ float so[MOST][DP];
   pdl_launch_dependents();
   pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -689,43 +762,69 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ oc_pa
   const int h = blockIdx.x, seq = blockIdx.y, hk = h / a.group, hg = h - hk * a.group;
   const int sub = hk * gtiles + hg / HT, hr = hg % HT;
   const Space ws(a.workspace, a.num_seqs);
-  const int before = ws.before[seq], tiles = (ws.before[seq + 1] - before) / subs - kUnitCost, share = ws.before[a.num_seqs + 1];
-  const int t0 = before + sub * (tiles + kUnitCost), t1 = t0 + tiles, c0 = t0 / share, c1 = (t1 - 1) / share;
+  const int before = ws.before[seq], tiles = (ws.before[seq + 1] - before) / subs - kUnitCost;
+  const Runs runs(ws.before[a.num_seqs], wave, late_ctas);
+  const int t0 = before + sub * (tiles + kUnitCost), c0 = runs.owner(t0), c1 = runs.owner(t0 + tiles - 1);
   if (c0 == c1) return;  // one CTA had it all and wrote the output
   auto state = [&](int c) {
     // the unit is the CTA's first unless it starts inside the CTA's run
-    const int slot = t0 >= c * share ? 1 : 0;
+    const int slot = t0 >= runs.start(c) ? 1 : 0;
     return ws.states + (int64_t)(2 * c + slot) * state_floats(HT, DP);
   };
-  float top = -INFINITY;
-  for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, state(c)[HT * DP + 2 * hr]);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  float sum = 0.f, x[DP / 32];
+  // each warp joins every W-th part by itself, then the warps' states are joined
+  float top = -INFINITY, sum = 0.f, x[DP / 32];
 #pragma unroll
   for (int i = 0; i < DP / 32; ++i) x[i] = 0.f;
-#pragma unroll 4
-  for (int c = c0 + warp; c <= c1; c += W) {
-    const float* s = state(c);
-    const float mc = s[HT * DP + 2 * hr], lc = s[HT * DP + 2 * hr + 1];
-    const float f = mc == -INFINITY ? (lc == 0.f ? 0.f : 1.f) : exp2f(mc - top);
-    sum = fmaf(lc, f, sum);
+  constexpr int U = 5;  // parts whose loads go out together
+  for (int c = c0 + warp; c <= c1; c += U * W) {
+    float mc[U], lc[U], v[U][DP / 32];
 #pragma unroll
-    for (int i = 0; i < DP / 32; ++i) x[i] = fmaf(s[hr * DP + lane + 32 * i], f, x[i]);
+    for (int u = 0; u < U; ++u) {
+      const bool on = c + u * W <= c1;
+      const float* s = state(on ? c + u * W : c);
+      mc[u] = s[HT * DP + 2 * hr];
+      lc[u] = s[HT * DP + 2 * hr + 1];
+#pragma unroll
+      for (int i = 0; i < DP / 32; ++i) v[u][i] = s[hr * DP + lane + 32 * i];
+      if (!on) {
+        mc[u] = -INFINITY;
+        lc[u] = 0.f;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      // a maximum of -inf with a sum that is not 0 is a NaN score: it stays
+      if (mc[u] == -INFINITY && lc[u] == 0.f) continue;
+      const float m = fmaxf(top, mc[u]);
+      const float back = top == -INFINITY ? 1.f : exp2f(top - m), f = mc[u] == -INFINITY ? 1.f : exp2f(mc[u] - m);
+      top = m;
+      sum = fmaf(lc[u], f, sum * back);
+#pragma unroll
+      for (int i = 0; i < DP / 32; ++i) x[i] = fmaf(v[u][i], f, x[i] * back);
+    }
   }
 #pragma unroll
   for (int i = 0; i < DP / 32; ++i) so[warp][lane + 32 * i] = x[i];
-  if (lane == 0) sm[warp][0] = sum;
+  if (lane == 0) {
+    sm[warp][0] = top;
+    sm[warp][1] = sum;
+  }
   __syncthreads();
-  float all = 0.f;
+  top = -INFINITY;
+  for (int w = 0; w < W; ++w) top = fmaxf(top, sm[w][0]);
+  float all = 0.f, f[MOST];
 #pragma unroll
-  for (int w = 0; w < W; ++w) all += sm[w][0];
+  for (int w = 0; w < MOST; ++w) {
+    f[w] = w >= W ? 0.f : sm[w][0] == -INFINITY ? (sm[w][1] == 0.f ? 0.f : 1.f) : exp2f(sm[w][0] - top);
+    if (w < W) all = fmaf(sm[w][1], f[w], all);
+  }
   const float inv = all == 0.f ? 0.f : a.v_scale / all;
   T* out = static_cast<T*>(a.out) + (int64_t)seq * a.out_seq_stride + (int64_t)h * a.out_head_stride;
   for (int d = threadIdx.x; d < a.head_dim; d += blockDim.x) {
     float y = 0.f;
 #pragma unroll
-    for (int w = 0; w < W; ++w) y += so[w][d];
+    for (int w = 0; w < MOST; ++w)
+      if (w < W) y = fmaf(so[w][d], f[w], y);
     out[d] = from_f32<T>(y * inv);
   }
   if (a.lse && threadIdx.x == 0)
@@ -787,7 +886,7 @@ bool tiled(const oc_paged_decode_args& a) {
 
 struct Plan {
   bool direct;
-  int64_t grid;
+  int64_t grid, late;  // CTAs, and those of them that wait for others to leave
   int nt;
 };
 
@@ -801,7 +900,8 @@ void plan_nt(const oc_paged_decode_args& a, Plan& p) {
   const int64_t useful = (units * (tiles + kUnitCost) + kMinShare - 1) / kMinShare;
   p.nt = NT;
   p.direct = tiles <= kDirectTiles;
-  p.grid = p.direct ? units : useful < wave ? useful : wave;
+  p.late = ES > 1 && !p.direct && units * (tiles + kUnitCost) >= kLongRun * wave ? wave : 0;
+  p.grid = p.direct ? units : useful < wave ? useful : wave + p.late;
 }
 template <int ES, int DP>
 Plan plan_of(const oc_paged_decode_args& a) {
@@ -884,10 +984,12 @@ int launch_tiled(const oc_paged_decode_args& a, const Plan& p, void* stream) {
   auto kernel = p.direct ? decode_kernel<T, C, DP, NT, true> : decode_kernel<T, C, DP, NT, false>;
   static std::atomic<uint64_t> ready[2];
   if (!allow_smem(reinterpret_cast<const void*>(kernel), ready[p.direct], S::SMEM)) return OC_ERR_CUDA;
-  int rc = launch_pdl(kernel, dim3((unsigned)p.grid), dim3(kWarps * 32), S::SMEM, stream, a, maps);
+  int rc = launch_pdl(kernel, dim3((unsigned)p.grid), dim3(kWarps * 32), S::SMEM, stream, a, maps, (int)p.late);
   if (rc != OC_OK || p.direct) return rc;
-  return launch_pdl(join_kernel<T, DP, NT>, dim3((unsigned)(a.kv_heads * a.group), (unsigned)a.num_seqs), dim3(256), 0,
-                    stream, a);
+  // few outputs have many parts each, many outputs two or three
+  const int64_t outputs = (int64_t)a.num_seqs * a.kv_heads * a.group;
+  return launch_pdl(join_kernel<T, DP, NT>, dim3((unsigned)(a.kv_heads * a.group), (unsigned)a.num_seqs),
+                    dim3(outputs <= a.num_sms ? 512 : 128), 0, stream, a, (int)(p.grid - p.late), (int)p.late);
 }
 
 template <typename T, typename C, int DP>
