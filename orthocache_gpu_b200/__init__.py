@@ -34,6 +34,7 @@ from .pages import PagedKVCache, compact_pages, copy_pages, fork_sequences, rese
 from .rotary import rotary_append_paged, rotary_embedding, rotary_tables
 from .pipeline import BypassFlag, GPUProfile, TelemetryLevel, format_bypass_reason, orthocache_forward
 
+# PagedLlama (paged_model.py) and GatedLlama (model.py) are imported from their modules.
 __version__ = "0.1.0"
 
 __all__ = [

@@ -833,16 +833,21 @@ __global__ void __launch_bounds__(512) join_kernel(const __grid_constant__ oc_pa
 }
 
 // ------------------------------------------------------------------ any type, any alignment
-// One warp per (sequence, query head).
+// One CTA per (sequence, query head): each warp attends to a stretch of the
+// keys, and the warps' results are weighted by their sums.
+constexpr int kRowWarps = 8;
+
 template <typename T, typename C>
-__global__ void __launch_bounds__(32) decode_row_kernel(const oc_paged_decode_args a) {
+__global__ void __launch_bounds__(kRowWarps * 32) decode_row_kernel(const __grid_constant__ oc_paged_decode_args a) {
   __shared__ float qs[kRowMaxDim];
+  __shared__ float part[kRowWarps][kRowMaxDim];
+  __shared__ float sums[kRowWarps];
   pdl_launch_dependents();
   pdl_wait();
-  const int seq = blockIdx.y, h = blockIdx.x, hk = h / a.group, lane = threadIdx.x;
+  const int seq = blockIdx.y, h = blockIdx.x, hk = h / a.group, warp = threadIdx.x >> 5;
   const T* q = static_cast<const T*>(a.q) + seq * a.q_seq_stride + h * a.q_head_stride;
-  for (int d = lane; d < a.head_dim; d += 32) qs[d] = to_f32(q[d]);
-  __syncwarp();
+  for (int d = threadIdx.x; d < a.head_dim; d += blockDim.x) qs[d] = to_f32(q[d]);
+  __syncthreads();
   const Span span = span_of(a, seq);
   const int32_t* table = a.block_tables + seq * a.block_table_stride;
   auto row = [&](const void* cache, int64_t bs, int64_t hs, int64_t ts, int j) -> const C* {
@@ -853,20 +858,42 @@ __global__ void __launch_bounds__(32) decode_row_kernel(const oc_paged_decode_ar
     }
     return static_cast<const C*>(cache) + page * bs + hk * hs + (j % a.block_size) * ts;
   };
-  T* out = static_cast<T*>(a.out) + seq * a.out_seq_stride + h * a.out_head_stride;
+  const int each = ((span.n - span.lo + kRowWarps - 1) / kRowWarps + 31) & ~31;  // keys of a warp
+  const int first = min(span.n, span.lo + warp * each), last = min(span.n, first + each);
   const float lse = attend_row<C>(
-      qs, a.head_dim, RowScore{a.scale * a.k_scale, a.softcap, a.slopes ? a.slopes[h] : 0.f}, a.v_scale, span.lo,
-      span.n, [](int) { return false; },
+      qs, a.head_dim, RowScore{a.scale * a.k_scale, a.softcap, a.slopes ? a.slopes[h] : 0.f}, a.v_scale, first, last,
+      [](int) { return false; },
       [&](int j) { return row(a.k_cache, a.kc_block_stride, a.kc_head_stride, a.kc_tok_stride, j); },
       [&](int j) { return row(a.v_cache, a.vc_block_stride, a.vc_head_stride, a.vc_tok_stride, j); },
-      [&](int j) { return (float)(j - (span.n - 1)); }, [&](int d, float x) { out[d] = from_f32<T>(x); });
-  if (a.lse && lane == 0) a.lse[(int64_t)seq * a.kv_heads * a.group + h] = lse;
+      [&](int j) { return (float)(j - (span.n - 1)); }, [&](int d, float x) { part[warp][d] = x; });
+  if ((threadIdx.x & 31) == 0) sums[warp] = lse;
+  __syncthreads();
+  float top = -INFINITY, all = 0.f, f[kRowWarps];
+#pragma unroll
+  for (int w = 0; w < kRowWarps; ++w) top = fmaxf(top, sums[w]);
+#pragma unroll
+  for (int w = 0; w < kRowWarps; ++w) {
+    f[w] = sums[w] == -INFINITY ? 0.f : exp2f((sums[w] - (top == -INFINITY ? 0.f : top)) * kLog2e);  // NaN stays
+    all += f[w];
+  }
+  const float inv = all == 0.f ? 0.f : 1.f / all;
+  T* out = static_cast<T*>(a.out) + seq * a.out_seq_stride + h * a.out_head_stride;
+  for (int d = threadIdx.x; d < a.head_dim; d += blockDim.x) {
+    float x = 0.f;
+#pragma unroll
+    for (int w = 0; w < kRowWarps; ++w)
+      if (sums[w] != -INFINITY) x = fmaf(part[w][d], f[w], x);
+    out[d] = from_f32<T>(x * inv);
+  }
+  if (a.lse && threadIdx.x == 0)
+    a.lse[(int64_t)seq * a.kv_heads * a.group + h] =
+        all == 0.f ? -INFINITY : (top == -INFINITY ? 0.f : top) + log2f(all) * kLn2;
 }
 
 template <typename T, typename C>
 int launch_rows(const oc_paged_decode_args& a, void* stream) {
-  return launch_pdl(decode_row_kernel<T, C>, dim3((unsigned)(a.kv_heads * a.group), (unsigned)a.num_seqs), 32, 0,
-                    stream, a);
+  return launch_pdl(decode_row_kernel<T, C>, dim3((unsigned)(a.kv_heads * a.group), (unsigned)a.num_seqs),
+                    kRowWarps * 32, 0, stream, a);
 }
 
 // ------------------------------------------------------------------ host side

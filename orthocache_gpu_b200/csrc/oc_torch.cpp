@@ -13,11 +13,36 @@
 
 #include <cstdint>
 #include <limits>
+#include <string>
 #include <vector>
 
 #include "../../include/orthocache_b200.h"
 
+// Messages are put together without streams: the C++ compiler that builds
+// this module may bring a standard library of its own, whose number formatting
+// does not work inside a process that has another one loaded.
+#define OC_VALUE(cond, ...) TORCH_CHECK_VALUE(cond, text(__VA_ARGS__))
+#define OC_TYPE(cond, ...) TORCH_CHECK_TYPE(cond, text(__VA_ARGS__))
+#define OC_RUNTIME(cond, ...) TORCH_CHECK(cond, text(__VA_ARGS__))
+
 namespace {
+
+std::string word_of(const char* s) { return s; }
+std::string word_of(int64_t x) { return std::to_string(x); }
+std::string word_of(int x) { return std::to_string(x); }
+std::string word_of(at::ScalarType t) { return c10::toString(t); }
+std::string word_of(const at::Device& d) { return d.str(); }
+std::string word_of(at::IntArrayRef sizes) {
+  std::string s = "[";
+  for (size_t i = 0; i < sizes.size(); ++i) s += (i ? ", " : "") + std::to_string(sizes[i]);
+  return s + "]";
+}
+template <typename... A>
+std::string text(const A&... a) {
+  std::string s;
+  (s.append(word_of(a)), ...);
+  return s;
+}
 
 int code_of(const at::Tensor& t) {
   switch (t.scalar_type()) {
@@ -25,13 +50,13 @@ int code_of(const at::Tensor& t) {
     case at::kHalf: return OC_F16;
     case at::kBFloat16: return OC_BF16;
     case at::kFloat8_e4m3fn: return OC_F8E4M3;
-    default: TORCH_CHECK(false, "unsupported dtype ", t.scalar_type());
+    default: OC_RUNTIME(false, "unsupported dtype ", t.scalar_type());
   }
   return -1;
 }
 
 void check(int rc, const char* what) {
-  TORCH_CHECK(rc == OC_OK, what, ": ", oc_status_string(rc), " (code ", rc, ")");
+  OC_RUNTIME(rc == OC_OK, what, ": ", oc_status_string(rc), " (code ", rc, ")");
 }
 
 void* ptr_or_null(const c10::optional<at::Tensor>& t) { return t.has_value() ? t->data_ptr() : nullptr; }
@@ -74,30 +99,30 @@ using at::Tensor;
 using OptTensor = c10::optional<Tensor>;
 
 void need_cuda(const Tensor& t, const Tensor& like) {
-  TORCH_CHECK(t.is_cuda(), "orthocache_gpu_b200 runs on CUDA tensors only (no CPU fallback); got a tensor on ",
+  OC_RUNTIME(t.is_cuda(), "orthocache_gpu_b200 runs on CUDA tensors only (no CPU fallback); got a tensor on ",
               t.device());
-  TORCH_CHECK(t.device() == like.device(), "tensors on different devices: ", like.device(), " and ", t.device());
+  OC_RUNTIME(t.device() == like.device(), "tensors on different devices: ", like.device(), " and ", t.device());
 }
 
 // An input of an operator that has no backward pass.
 void need_input(const Tensor& t, const Tensor& like, const char* name) {
   need_cuda(t, like);
-  TORCH_CHECK(!(t.requires_grad() && at::GradMode::is_enabled()), name,
+  OC_RUNTIME(!(t.requires_grad() && at::GradMode::is_enabled()), name,
               " requires grad, and this operator has no backward pass; call it under torch.no_grad()");
 }
 
 int float_code(const Tensor& t, const char* name) {
   const auto s = t.scalar_type();
-  TORCH_CHECK_TYPE(s == at::kFloat || s == at::kHalf || s == at::kBFloat16, name,
+  OC_TYPE(s == at::kFloat || s == at::kHalf || s == at::kBFloat16, name,
                    " must be float32, float16 or bfloat16, got ", s);
   return code_of(t);
 }
 
 // The dtype code of a cache pair: that of the inputs, or float8_e4m3fn for both.
 int cache_code(const Tensor& k, const Tensor& v, const Tensor& in) {
-  TORCH_CHECK_TYPE(k.scalar_type() == v.scalar_type(), "k_cache and v_cache must share a dtype, got ",
+  OC_TYPE(k.scalar_type() == v.scalar_type(), "k_cache and v_cache must share a dtype, got ",
                    k.scalar_type(), " and ", v.scalar_type());
-  TORCH_CHECK_TYPE(k.scalar_type() == in.scalar_type() || k.scalar_type() == at::kFloat8_e4m3fn,
+  OC_TYPE(k.scalar_type() == in.scalar_type() || k.scalar_type() == at::kFloat8_e4m3fn,
                    "the caches must be of the inputs' dtype (", in.scalar_type(), ") or float8_e4m3fn, got ",
                    k.scalar_type());
   return code_of(k);
@@ -107,19 +132,19 @@ Tensor rows(const Tensor& t) { return t.dim() == 0 || t.stride(-1) == 1 || t.siz
 
 Tensor ints(const Tensor& t, const Tensor& like, const char* name) {
   need_cuda(t, like);
-  TORCH_CHECK_TYPE(t.scalar_type() == at::kInt || t.scalar_type() == at::kLong, name, " must be int32 or int64, got ",
+  OC_TYPE(t.scalar_type() == at::kInt || t.scalar_type() == at::kLong, name, " must be int32 or int64, got ",
                    t.scalar_type());
   return rows(t.scalar_type() == at::kInt ? t : t.to(at::kInt));
 }
 
 Tensor floats(const Tensor& t, const Tensor& like, const char* name) {
   need_cuda(t, like);
-  TORCH_CHECK_TYPE(t.scalar_type() == at::kFloat, name, " must be float32, got ", t.scalar_type());
+  OC_TYPE(t.scalar_type() == at::kFloat, name, " must be float32, got ", t.scalar_type());
   return t.contiguous();
 }
 
 int as_int(int64_t x, const char* name) {
-  TORCH_CHECK_VALUE(x >= 0 && x <= std::numeric_limits<int>::max(), name, " (", x, ") is out of range");
+  OC_VALUE(x >= 0 && x <= std::numeric_limits<int>::max(), name, " (", x, ") is out of range");
   return static_cast<int>(x);
 }
 
@@ -127,19 +152,19 @@ int as_int(int64_t x, const char* name) {
 void need_cache(const Tensor& k, const Tensor& v, const Tensor& like, int64_t kv_heads, int64_t head_dim) {
   need_cuda(k, like);
   need_cuda(v, like);
-  TORCH_CHECK_VALUE(k.dim() == 4 && k.sizes() == v.sizes(),
+  OC_VALUE(k.dim() == 4 && k.sizes() == v.sizes(),
                     "k_cache and v_cache must be (num_blocks, kv_heads, block_size, head_dim) alike, got ", k.sizes(),
                     " and ", v.sizes());
-  TORCH_CHECK_VALUE(k.size(3) == head_dim, "the caches' head_dim (", k.size(3), ") is not the inputs' (", head_dim, ")");
-  TORCH_CHECK_VALUE(kv_heads < 0 || k.size(1) == kv_heads, "the caches' kv_heads (", k.size(1),
+  OC_VALUE(k.size(3) == head_dim, "the caches' head_dim (", k.size(3), ") is not the inputs' (", head_dim, ")");
+  OC_VALUE(kv_heads < 0 || k.size(1) == kv_heads, "the caches' kv_heads (", k.size(1),
                     ") is not that of k (", kv_heads, ")");
-  TORCH_CHECK_VALUE(k.stride(3) == 1 && v.stride(3) == 1, "the caches' last dimension must be contiguous");
+  OC_VALUE(k.stride(3) == 1 && v.stride(3) == 1, "the caches' last dimension must be contiguous");
   const int64_t bs = k.size(2);
-  TORCH_CHECK_VALUE(bs > 0 && (bs & (bs - 1)) == 0, "block_size (", bs, ") must be a power of 2");
+  OC_VALUE(bs > 0 && (bs & (bs - 1)) == 0, "block_size (", bs, ") must be a power of 2");
 }
 
 Tensor need_tables(const Tensor& t, const Tensor& like) {
-  TORCH_CHECK_VALUE(t.dim() == 2, "block_tables must be (num_seqs, max_blocks), got ", t.sizes());
+  OC_VALUE(t.dim() == 2, "block_tables must be (num_seqs, max_blocks), got ", t.sizes());
   return ints(t, like, "block_tables");
 }
 
@@ -153,13 +178,13 @@ std::tuple<OptTensor, OptTensor> rotary_append(const OptTensor& q_, const OptTen
                                                const OptTensor& tables_, const OptTensor& seq_ids_, bool interleaved,
                                                bool inverse, double k_scale, double v_scale, bool return_keys,
                                                int64_t num_sms, int64_t status, int64_t stream) {
-  TORCH_CHECK_VALUE(q_.has_value() || k_.has_value(), "give q, k or both");
+  OC_VALUE(q_.has_value() || k_.has_value(), "give q, k or both");
   const Tensor& like = q_.has_value() ? *q_ : *k_;
   need_cuda(like, like);
   const c10::DeviceGuard guard(like.device());
   oc_rotary_args a = {};
   a.dtype = float_code(like, "q");
-  TORCH_CHECK_VALUE(like.dim() == 3, "q and k must be (tokens, heads, head_dim), got ", like.sizes());
+  OC_VALUE(like.dim() == 3, "q and k must be (tokens, heads, head_dim), got ", like.sizes());
   const int64_t T = like.size(0), D = like.size(2);
   a.tokens = T;
   a.head_dim = as_int(D, "head_dim");
@@ -167,9 +192,9 @@ std::tuple<OptTensor, OptTensor> rotary_append(const OptTensor& q_, const OptTen
   OptTensor q_out, k_out;
   auto part = [&](const Tensor& t, const char* name) {
     need_input(t, like, name);
-    TORCH_CHECK_TYPE(t.scalar_type() == like.scalar_type(), name, " must be ", like.scalar_type(), ", got ",
+    OC_TYPE(t.scalar_type() == like.scalar_type(), name, " must be ", like.scalar_type(), ", got ",
                      t.scalar_type());
-    TORCH_CHECK_VALUE(t.dim() == 3 && t.size(0) == T && t.size(2) == D, name, " must be (", T, ", heads, ", D,
+    OC_VALUE(t.dim() == 3 && t.size(0) == T && t.size(2) == D, name, " must be (", T, ", heads, ", D,
                       "), got ", t.sizes());
     return rows(t);
   };
@@ -184,26 +209,26 @@ std::tuple<OptTensor, OptTensor> rotary_append(const OptTensor& q_, const OptTen
     a.qo_tok_stride = q_out->stride(0);
     a.qo_head_stride = q_out->stride(1);
   }
-  TORCH_CHECK_VALUE(positions_.dim() == 1 && positions_.size(0) == T, "positions must be (", T, ",), got ",
+  OC_VALUE(positions_.dim() == 1 && positions_.size(0) == T, "positions must be (", T, ",), got ",
                     positions_.sizes());
   need_cuda(positions_, like);
-  TORCH_CHECK_TYPE(positions_.scalar_type() == at::kInt || positions_.scalar_type() == at::kLong,
+  OC_TYPE(positions_.scalar_type() == at::kInt || positions_.scalar_type() == at::kLong,
                    "positions must be int32 or int64, got ", positions_.scalar_type());
   pos = positions_.contiguous();
   a.positions = pos.data_ptr();
   a.positions_64 = pos.scalar_type() == at::kLong;
-  TORCH_CHECK_VALUE(cos_.has_value() == sin_.has_value(), "give cos and sin together");
+  OC_VALUE(cos_.has_value() == sin_.has_value(), "give cos and sin together");
   if (cos_.has_value()) {
     cos = floats(*cos_, like, "cos");
     sin = floats(*sin_, like, "sin");
-    TORCH_CHECK_VALUE(cos.dim() == 2 && cos.sizes() == sin.sizes() && 2 * cos.size(1) <= D,
+    OC_VALUE(cos.dim() == 2 && cos.sizes() == sin.sizes() && 2 * cos.size(1) <= D,
                       "cos and sin must be (positions, rotary_dim / 2) with rotary_dim <= head_dim (", D, "), got ",
                       cos.sizes(), " and ", sin.sizes());
     a.cos_tab = cos.data_ptr<float>();
     a.sin_tab = sin.data_ptr<float>();
     a.table_rows = cos.size(0);
     a.rotary_dim = 2 * (int)cos.size(1);
-    TORCH_CHECK_VALUE(T == 0 || a.table_rows > 0, "cos and sin have no rows");
+    OC_VALUE(T == 0 || a.table_rows > 0, "cos and sin have no rows");
   }
   if (k_.has_value()) {
     k = part(*k_, "k");
@@ -218,18 +243,18 @@ std::tuple<OptTensor, OptTensor> rotary_append(const OptTensor& q_, const OptTen
       a.ko_head_stride = k_out->stride(1);
     }
   }
-  TORCH_CHECK_VALUE(k_cache.has_value() == v_cache.has_value() && k_cache.has_value() == tables_.has_value() &&
+  OC_VALUE(k_cache.has_value() == v_cache.has_value() && k_cache.has_value() == tables_.has_value() &&
                         k_cache.has_value() == v_.has_value(),
                     "give v, k_cache, v_cache and block_tables together");
   if (k_cache.has_value()) {
-    TORCH_CHECK_VALUE(k_.has_value(), "give k with the caches");
+    OC_VALUE(k_.has_value(), "give k with the caches");
     v = part(*v_, "v");
-    TORCH_CHECK_VALUE(v.size(1) == k.size(1), "v must have k's heads (", k.size(1), "), got ", v.size(1));
+    OC_VALUE(v.size(1) == k.size(1), "v must have k's heads (", k.size(1), "), got ", v.size(1));
     need_cache(*k_cache, *v_cache, like, k.size(1), D);
     a.cache_dtype = cache_code(*k_cache, *v_cache, like);
-    TORCH_CHECK_VALUE(a.cache_dtype == OC_F8E4M3 || (k_scale == 1.0 && v_scale == 1.0),
+    OC_VALUE(a.cache_dtype == OC_F8E4M3 || (k_scale == 1.0 && v_scale == 1.0),
                       "k_scale and v_scale belong to float8 caches");
-    TORCH_CHECK_VALUE(k_scale > 0 && v_scale > 0, "k_scale and v_scale must be positive");
+    OC_VALUE(k_scale > 0 && v_scale > 0, "k_scale and v_scale must be positive");
     tables = need_tables(*tables_, like);
     a.v = v.data_ptr();
     a.v_tok_stride = v.stride(0);
@@ -251,17 +276,17 @@ std::tuple<OptTensor, OptTensor> rotary_append(const OptTensor& q_, const OptTen
     a.k_scale = (float)k_scale;
     a.v_scale = (float)v_scale;
     if (seq_ids_.has_value()) {
-      TORCH_CHECK_VALUE(seq_ids_->dim() == 1 && seq_ids_->size(0) == T, "seq_ids must be (", T, ",), got ",
+      OC_VALUE(seq_ids_->dim() == 1 && seq_ids_->size(0) == T, "seq_ids must be (", T, ",), got ",
                         seq_ids_->sizes());
       seq_ids = ints(*seq_ids_, like, "seq_ids");
       a.seq_ids = seq_ids.data_ptr<int32_t>();
     } else {
-      TORCH_CHECK_VALUE(T == a.num_seqs, "without seq_ids there must be one token per sequence: ", T, " tokens, ",
+      OC_VALUE(T == a.num_seqs, "without seq_ids there must be one token per sequence: ", T, " tokens, ",
                         a.num_seqs, " sequences");
     }
     // an empty table or cache has no storage to point to, and no slot either
     if (a.k_cache == nullptr || a.block_tables == nullptr) {
-      TORCH_CHECK_VALUE(T == 0, "the caches or block_tables are empty");
+      OC_VALUE(T == 0, "the caches or block_tables are empty");
     }
   }
   a.flags = (interleaved ? OC_ROTARY_INTERLEAVED : 0) | (inverse ? OC_ROTARY_INVERSE : 0);
@@ -281,27 +306,27 @@ std::tuple<Tensor, OptTensor> paged_decode(const Tensor& q_, const Tensor& k_cac
   const c10::DeviceGuard guard(q_.device());
   oc_paged_decode_args a = {};
   a.dtype = float_code(q_, "q");
-  TORCH_CHECK_VALUE(q_.dim() == 3, "q must be (num_seqs, heads, head_dim), got ", q_.sizes());
+  OC_VALUE(q_.dim() == 3, "q must be (num_seqs, heads, head_dim), got ", q_.sizes());
   const int64_t S = q_.size(0), H = q_.size(1), D = q_.size(2);
   need_cache(k_cache, v_cache, q_, -1, D);
   a.cache_dtype = cache_code(k_cache, v_cache, q_);
-  TORCH_CHECK_VALUE(a.cache_dtype == OC_F8E4M3 || (k_scale == 1.0 && v_scale == 1.0),
+  OC_VALUE(a.cache_dtype == OC_F8E4M3 || (k_scale == 1.0 && v_scale == 1.0),
                     "k_scale and v_scale belong to float8 caches");
   const int64_t HK = k_cache.size(1);
-  TORCH_CHECK_VALUE(HK > 0 && H % HK == 0 && H > 0, "the query heads (", H, ") must be a multiple of the kv heads (",
+  OC_VALUE(HK > 0 && H % HK == 0 && H > 0, "the query heads (", H, ") must be a multiple of the kv heads (",
                     HK, ")");
-  TORCH_CHECK_VALUE(D > 0 && D <= 256, "head_dim (", D, ") must be between 1 and 256");
-  TORCH_CHECK_VALUE(softcap >= 0, "softcap must not be negative");
+  OC_VALUE(D > 0 && D <= 256, "head_dim (", D, ") must be between 1 and 256");
+  OC_VALUE(softcap >= 0, "softcap must not be negative");
   const Tensor q = rows(q_), tables = need_tables(tables_, q);
-  TORCH_CHECK_VALUE(tables.size(0) == S, "block_tables must have one row per sequence (", S, "), got ",
+  OC_VALUE(tables.size(0) == S, "block_tables must have one row per sequence (", S, "), got ",
                     tables.size(0));
-  TORCH_CHECK_VALUE(seq_lens_.dim() == 1 && seq_lens_.size(0) == S, "seq_lens must be (", S, ",), got ",
+  OC_VALUE(seq_lens_.dim() == 1 && seq_lens_.size(0) == S, "seq_lens must be (", S, ",), got ",
                     seq_lens_.sizes());
   const Tensor lens = ints(seq_lens_, q, "seq_lens");
   Tensor slopes;
   if (slopes_.has_value()) {
     slopes = floats(*slopes_, q, "alibi_slopes");
-    TORCH_CHECK_VALUE(slopes.dim() == 1 && slopes.size(0) == H, "alibi_slopes must be (", H, ",), got ",
+    OC_VALUE(slopes.dim() == 1 && slopes.size(0) == H, "alibi_slopes must be (", H, ",), got ",
                       slopes.sizes());
     a.slopes = slopes.data_ptr<float>();
   }
@@ -365,33 +390,33 @@ std::tuple<Tensor, OptTensor> prompt(const Tensor& q_, const Tensor& k_, const T
   const c10::DeviceGuard guard(q_.device());
   oc_prompt_args a = {};
   a.dtype = float_code(q_, "q");
-  TORCH_CHECK_TYPE(k_.scalar_type() == q_.scalar_type() && v_.scalar_type() == q_.scalar_type(),
+  OC_TYPE(k_.scalar_type() == q_.scalar_type() && v_.scalar_type() == q_.scalar_type(),
                    "k and v must be of q's dtype (", q_.scalar_type(), "), got ", k_.scalar_type(), " and ",
                    v_.scalar_type());
-  TORCH_CHECK_VALUE(q_.dim() == 3 && k_.dim() == 3 && k_.sizes() == v_.sizes() && k_.size(2) == q_.size(2),
+  OC_VALUE(q_.dim() == 3 && k_.dim() == 3 && k_.sizes() == v_.sizes() && k_.size(2) == q_.size(2),
                     "q must be (tokens, heads, head_dim), k and v (key tokens, kv heads, head_dim) alike, got ",
                     q_.sizes(), ", ", k_.sizes(), " and ", v_.sizes());
   const int64_t T = q_.size(0), H = q_.size(1), D = q_.size(2), TK = k_.size(0), HK = k_.size(1);
-  TORCH_CHECK_VALUE(HK > 0 && H > 0 && H % HK == 0, "the query heads (", H, ") must be a multiple of the kv heads (",
+  OC_VALUE(HK > 0 && H > 0 && H % HK == 0, "the query heads (", H, ") must be a multiple of the kv heads (",
                     HK, ")");
-  TORCH_CHECK_VALUE(D > 0 && D <= (q_.scalar_type() == at::kFloat ? 256 : 128) &&
+  OC_VALUE(D > 0 && D <= (q_.scalar_type() == at::kFloat ? 256 : 128) &&
                         (D % 8 == 0 || q_.scalar_type() == at::kFloat),
                     "head_dim (", D, ") must be a multiple of 8 up to 128, or up to 256 in float32");
-  TORCH_CHECK_VALUE(softcap >= 0, "softcap must not be negative");
+  OC_VALUE(softcap >= 0, "softcap must not be negative");
   const Tensor q = rows(q_), k = rows(k_), v = rows(v_);
-  TORCH_CHECK_VALUE(cu_q_.has_value() || !cu_k_.has_value(), "give cu_seqlens with cu_seqlens_k");
+  OC_VALUE(cu_q_.has_value() || !cu_k_.has_value(), "give cu_seqlens with cu_seqlens_k");
   Tensor cu_q, cu_k, prefix, slopes;
   if (cu_q_.has_value()) {
     cu_q = ints(*cu_q_, q, "cu_seqlens");
-    TORCH_CHECK_VALUE(cu_q.dim() == 1 && cu_q.size(0) >= 1, "cu_seqlens must be (documents + 1,), got ", cu_q.sizes());
-    TORCH_CHECK_VALUE(cu_k_.has_value() || TK == T, "without cu_seqlens_k there must be as many keys (", TK,
+    OC_VALUE(cu_q.dim() == 1 && cu_q.size(0) >= 1, "cu_seqlens must be (documents + 1,), got ", cu_q.sizes());
+    OC_VALUE(cu_k_.has_value() || TK == T, "without cu_seqlens_k there must be as many keys (", TK,
                       ") as queries (", T, ")");
     a.docs = as_int(cu_q.size(0) - 1, "documents");
     a.cu_q = cu_q.data_ptr<int32_t>();
     a.cu_k = a.cu_q;
     if (cu_k_.has_value()) {
       cu_k = ints(*cu_k_, q, "cu_seqlens_k");
-      TORCH_CHECK_VALUE(cu_k.dim() == 1 && cu_k.size(0) == cu_q.size(0), "cu_seqlens_k must be (", cu_q.size(0),
+      OC_VALUE(cu_k.dim() == 1 && cu_k.size(0) == cu_q.size(0), "cu_seqlens_k must be (", cu_q.size(0),
                         ",), got ", cu_k.sizes());
       a.cu_k = cu_k.data_ptr<int32_t>();
     }
@@ -400,13 +425,13 @@ std::tuple<Tensor, OptTensor> prompt(const Tensor& q_, const Tensor& k_, const T
   }
   if (prefix_.has_value()) {
     prefix = ints(*prefix_, q, "prefix_lens");
-    TORCH_CHECK_VALUE(prefix.dim() == 1 && prefix.size(0) == a.docs, "prefix_lens must be (", a.docs, ",), got ",
+    OC_VALUE(prefix.dim() == 1 && prefix.size(0) == a.docs, "prefix_lens must be (", a.docs, ",), got ",
                       prefix.sizes());
     a.prefix_lens = prefix.data_ptr<int32_t>();
   }
   if (slopes_.has_value()) {
     slopes = floats(*slopes_, q, "alibi_slopes");
-    TORCH_CHECK_VALUE(slopes.dim() == 1 && slopes.size(0) == H, "alibi_slopes must be (", H, ",), got ",
+    OC_VALUE(slopes.dim() == 1 && slopes.size(0) == H, "alibi_slopes must be (", H, ",), got ",
                       slopes.sizes());
     a.slopes = slopes.data_ptr<float>();
   }
@@ -454,26 +479,26 @@ struct CacheList {
   // a list or tuple of tensors, looked at without a conversion: a model has tens of caches, a call a few us
   CacheList(py::handle caches, const Tensor& like) {
     const bool list = PyList_Check(caches.ptr());
-    TORCH_CHECK_TYPE(list || PyTuple_Check(caches.ptr()), "caches must be a list or tuple of tensors");
+    OC_TYPE(list || PyTuple_Check(caches.ptr()), "caches must be a list or tuple of tensors");
     const Py_ssize_t n = list ? PyList_GET_SIZE(caches.ptr()) : PyTuple_GET_SIZE(caches.ptr());
     base.reserve(n);
     stride.reserve(n);
     const Tensor* first = nullptr;
     for (Py_ssize_t i = 0; i < n; ++i) {
       PyObject* o = list ? PyList_GET_ITEM(caches.ptr(), i) : PyTuple_GET_ITEM(caches.ptr(), i);
-      TORCH_CHECK_TYPE(THPVariable_Check(o), "caches must be a list or tuple of tensors");
+      OC_TYPE(THPVariable_Check(o), "caches must be a list or tuple of tensors");
       const Tensor& c = THPVariable_Unpack(o);
       need_cuda(c, like);
       if (!first || c.scalar_type() != first->scalar_type() || c.sizes() != first->sizes() ||
           c.strides() != first->strides()) {
-        TORCH_CHECK_VALUE(c.dim() >= 2, "a cache must be (num_blocks, ...), got ", c.sizes());
+        OC_VALUE(c.dim() >= 2, "a cache must be (num_blocks, ...), got ", c.sizes());
         const int64_t es = c.element_size(), pages = c.size(0);
         const int64_t bytes = pages ? c.numel() / pages * es : 0;
         bool dense = bytes > 0 && c.stride(0) * es >= bytes;  // a page of contiguous elements
         for (int64_t d = c.dim() - 1, run = 1; dense && d > 0; run *= c.size(d--))
           dense = c.size(d) == 1 || c.stride(d) == run;
-        TORCH_CHECK_VALUE(pages == 0 || dense, "a page of a cache must be contiguous, got strides ", c.strides());
-        TORCH_CHECK_VALUE(!first || (pages == num_pages && (pages == 0 || bytes == page_bytes)),
+        OC_VALUE(pages == 0 || dense, "a page of a cache must be contiguous, got strides ", c.strides());
+        OC_VALUE(!first || (pages == num_pages && (pages == 0 || bytes == page_bytes)),
                           "the caches must have pages of one size and number");
         num_pages = pages;
         if (pages) page_bytes = bytes;
@@ -489,14 +514,14 @@ struct CacheList {
 
 Tensor need_int32(const Tensor& t, const Tensor& like, const char* name, int64_t dim) {
   need_cuda(t, like);
-  TORCH_CHECK_TYPE(t.scalar_type() == at::kInt, name, " must be int32, got ", t.scalar_type());
-  TORCH_CHECK_VALUE(t.dim() == dim && (t.numel() == 0 || t.stride(-1) == 1), name, " must have ", dim,
+  OC_TYPE(t.scalar_type() == at::kInt, name, " must be int32, got ", t.scalar_type());
+  OC_VALUE(t.dim() == dim && (t.numel() == 0 || t.stride(-1) == 1), name, " must have ", dim,
                     " dimensions, the last contiguous");
   return t;
 }
 
 void need_len(const Tensor& t, int64_t n, const char* name) {
-  TORCH_CHECK_VALUE(t.size(0) == n, name, " must be (", n, ",), got ", t.sizes());
+  OC_VALUE(t.size(0) == n, name, " must be (", n, ",), got ", t.sizes());
 }
 
 void copy_pages(py::handle caches, const Tensor& src_, const Tensor& dst_, int64_t num_sms,
@@ -504,7 +529,7 @@ void copy_pages(py::handle caches, const Tensor& src_, const Tensor& dst_, int64
   need_cuda(src_, src_);
   const c10::DeviceGuard guard(src_.device());
   const Tensor src = ints(src_, src_, "src"), dst = ints(dst_, src_, "dst");
-  TORCH_CHECK_VALUE(src.dim() == 1 && src.sizes() == dst.sizes(), "src and dst must be (pairs,) alike, got ",
+  OC_VALUE(src.dim() == 1 && src.sizes() == dst.sizes(), "src and dst must be (pairs,) alike, got ",
                     src.sizes(), " and ", dst.sizes());
   const CacheList c(caches, src);
   if (src.numel() == 0 || c.count() == 0) return;
@@ -522,10 +547,10 @@ std::tuple<Tensor, Tensor, Tensor> fork_sequences(const Tensor& tables, const Te
   need_int32(refs, tables, "refcounts", 1);
   const int64_t S = tables.size(0);
   need_len(lens, S, "seq_lens");
-  TORCH_CHECK_VALUE(source_.dim() == 1, "source must be (", S, ",), got ", source_.sizes());
+  OC_VALUE(source_.dim() == 1, "source must be (", S, ",), got ", source_.sizes());
   need_len(source_, S, "source");
   const Tensor source = ints(source_, tables, "source");
-  TORCH_CHECK_VALUE(block_size > 0, "block_size (", block_size, ") must be positive");
+  OC_VALUE(block_size > 0, "block_size (", block_size, ") must be positive");
   Tensor t = at::empty({S, tables.size(1)}, tables.options()), l = at::empty({S}, lens.options()),
          r = at::empty({refs.size(0)}, refs.options());
   check(oc_fork_sequences(tables.data_ptr<int32_t>(), tables.stride(0), t.data_ptr<int32_t>(), t.stride(0),
@@ -545,12 +570,12 @@ void reserve_pages(py::handle caches, const Tensor& tables, const Tensor& lens, 
   need_int32(refs, tables, "refcounts", 1);
   const int64_t S = tables.size(0);
   need_len(lens, S, "seq_lens");
-  TORCH_CHECK_VALUE(wanted_.dim() == 1, "wanted must be (", S, ",), got ", wanted_.sizes());
+  OC_VALUE(wanted_.dim() == 1, "wanted must be (", S, ",), got ", wanted_.sizes());
   need_len(wanted_, S, "wanted");
   const Tensor wanted = ints(wanted_, tables, "wanted");
-  TORCH_CHECK_VALUE(block_size > 0, "block_size (", block_size, ") must be positive");
+  OC_VALUE(block_size > 0, "block_size (", block_size, ") must be positive");
   const CacheList c(caches, tables);
-  TORCH_CHECK_VALUE(c.count() == 0 || c.num_pages == refs.size(0), "the caches have ", c.num_pages,
+  OC_VALUE(c.count() == 0 || c.num_pages == refs.size(0), "the caches have ", c.num_pages,
                     " pages, refcounts ", refs.size(0));
   if (S == 0) return;
   const size_t bytes = oc_reserve_workspace_bytes(as_int(S, "num_seqs"), refs.size(0));
@@ -570,7 +595,7 @@ std::tuple<Tensor, Tensor> compact_pages(py::handle caches, const Tensor& tables
   need_int32(refs, tables, "refcounts", 1);
   const CacheList c(caches, tables);
   const int64_t P = refs.size(0);
-  TORCH_CHECK_VALUE(c.count() == 0 || c.num_pages == P, "the caches have ", c.num_pages, " pages, refcounts ", P);
+  OC_VALUE(c.count() == 0 || c.num_pages == P, "the caches have ", c.num_pages, " pages, refcounts ", P);
   Tensor t = at::empty({tables.size(0), tables.size(1)}, tables.options()), r = at::empty({P}, refs.options());
   if (P == 0) return {t.fill_(-1), r};
   const size_t bytes = oc_compact_workspace_bytes(P);
