@@ -195,7 +195,7 @@ struct Runs {
   }
 };
 
-// Workspace: header (the place before each sequence, and after all), then per CTA two states of 8 NT heads: acc, m, l.
+// Workspace: header (the place before each sequence, and after all), then per CTA two states of 8 NT heads.
 struct Space {
   int32_t* before;  // num_seqs + 1
   float* states;
@@ -203,7 +203,8 @@ struct Space {
   __host__ __device__ Space(void* p, int num_seqs)
       : before(static_cast<int32_t*>(p)), states(reinterpret_cast<float*>(static_cast<char*>(p) + header(num_seqs))) {}
 };
-__host__ __device__ constexpr int state_floats(int heads, int dp) { return heads * (dp + 2); }
+// acc, then of each head the maximum, the sum of the rounded weights, the sum of the weights
+__host__ __device__ constexpr int state_floats(int heads, int dp) { return heads * (dp + 4); }
 
 // A cache as the copy engine sees it: dimension 0 is a row's columns, the
 // others (slot, kv head, page) are ordered by their strides; role[i] says
@@ -225,7 +226,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<sizeof(C), DP, NT>::PER_SM)
   __shared__ __align__(8) uint64_t bars[kWarps][kBufs];
   __shared__ int part[kWarps];
   __shared__ int found[3];  // sequence, unit, tile
-  __shared__ float stat[kWarps][8][2];
+  __shared__ float stat[kWarps][8][3];
   char* const ring = raw + (-smem_u32(raw) & 1023u);
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
@@ -417,7 +418,11 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<sizeof(C), DP, NT>::PER_SM)
 
   // ---------------------------------------------------------------- the unit's state
   uint32_t qf[KS][NT][2];
-  float acc[KS][NT][4], m[NT][2], l[NT][2], sc[NT][2], slope[NT][2];
+  float acc[KS][NT][4], m[NT][2], sc[NT][2], slope[NT][2];
+  // sums of the weights, by the products' own unit (a row of ones times P): of the weights as they were rounded, so
+  // that a row with one large weight loses nothing; [0] and [1] are this lane's heads, summed over all keys of the warp
+  float l[NT][4];
+  float le[NT][2];  // and of the weights before rounding, over this lane's keys: what the logarithm is taken of
   const bool capped = a.softcap > 0.f, biased = a.slopes != nullptr;
   const float cap2 = a.softcap * kLog2e;
 
@@ -465,7 +470,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<sizeof(C), DP, NT>::PER_SM)
         sc[n][c] = a.scale * a.k_scale / qs * (capped ? 1.f / a.softcap : kLog2e);
         slope[n][c] = biased && hr < heads ? a.slopes[h0 + hr] * kLog2e : 0.f;
         m[n][c] = -INFINITY;
-        l[n][c] = 0.f;
+        l[n][c] = l[n][c + 2] = le[n][c] = 0.f;
 #pragma unroll
         for (int k = 0; k < KS; ++k) acc[k][n][c] = acc[k][n][c + 2] = 0.f;
       }
@@ -565,6 +570,8 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<sizeof(C), DP, NT>::PER_SM)
           const float back = m[n][c] == -INFINITY ? 0.f : exp2f(m[n][c] - x);
           m[n][c] = x;
           l[n][c] *= back;
+          l[n][c + 2] *= back;
+          le[n][c] *= back;
 #pragma unroll
           for (int k = 0; k < KS; ++k) {
             acc[k][n][c] *= back;
@@ -597,10 +604,13 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<sizeof(C), DP, NT>::PER_SM)
         for (int c = 0; c < 4; ++c) {
           const float mc = m[n][c & 1];
           e[c] = ex2(s[kt][n][c] - (mc == -INFINITY ? 0.f : mc));
-          l[n][c & 1] += e[c];
+          le[n][c & 1] += e[c];
         }
         p[n][0] = transpose8x8(pack16<BF16>(e[0], e[1]));
         p[n][1] = transpose8x8(pack16<BF16>(e[2], e[3]));
+        constexpr uint32_t one = BF16 ? 0x3f803f80u : 0x3c003c00u;
+        const uint32_t ones[4] = {one, one, one, one};
+        mma16816<BF16>(l[n], ones, p[n][0], p[n][1]);
       }
       if constexpr (F8) {
         // matrices: keys 0-7 and 8-15 of one 16-column chunk, then of the next
@@ -643,13 +653,14 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<sizeof(C), DP, NT>::PER_SM)
       __syncthreads();  // every warp has left its buffer (and the round before) behind
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        float sum = l[n][c];
+        float exact = le[n][c];
 #pragma unroll
-        for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        for (int o = 4; o < 32; o <<= 1) exact += __shfl_xor_sync(0xffffffffu, exact, o);
         const int hr = 2 * t + c;
         if (g == 0) {
           stat[warp][hr][0] = m[n][c];
-          stat[warp][hr][1] = sum;
+          stat[warp][hr][1] = l[n][c];
+          stat[warp][hr][2] = exact;
         }
 #pragma unroll
         for (int k = 0; k < KS; ++k) {  // columns are XORed by the head so that the four lanes of a row spread over banks
@@ -661,7 +672,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<sizeof(C), DP, NT>::PER_SM)
       __syncthreads();
       // a warp per head
       for (int hr = warp; hr < min(8, heads - n * 8); hr += kWarps) {
-        float top = -INFINITY, sum = 0.f, f[kWarps];
+        float top = -INFINITY, sum = 0.f, exact = 0.f, f[kWarps];
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) top = fmaxf(top, stat[w][hr][0]);
 #pragma unroll
@@ -669,6 +680,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<sizeof(C), DP, NT>::PER_SM)
           // a maximum of -inf with a sum that is not 0 is a NaN score: it stays
           f[w] = stat[w][hr][0] == -INFINITY ? (stat[w][hr][1] == 0.f ? 0.f : 1.f) : exp2f(stat[w][hr][0] - top);
           sum = fmaf(stat[w][hr][1], f[w], sum);
+          exact = fmaf(stat[w][hr][2], f[w], exact);
         }
         const int swz = ((hr >> 1) & 3) << 3, head = h0 + n * 8 + hr;
         const float inv = sum == 0.f ? 0.f : a.v_scale / sum;
@@ -693,10 +705,12 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<sizeof(C), DP, NT>::PER_SM)
           if (DIRECT || complete) {
             if (a.lse)
               a.lse[(int64_t)cs.seq * a.kv_heads * a.group + head] =
-                  sum == 0.f ? -INFINITY : ((top == -INFINITY ? 0.f : top) + log2f(sum)) * kLn2;
+                  sum == 0.f ? -INFINITY : ((top == -INFINITY ? 0.f : top) + log2f(exact)) * kLn2;
           } else {
-            state[HT * DP + 2 * (n * 8 + hr)] = top;
-            state[HT * DP + 2 * (n * 8 + hr) + 1] = sum;
+            float* totals = state + HT * DP + 4 * (n * 8 + hr);
+            totals[0] = top;
+            totals[1] = sum;
+            totals[2] = exact;
           }
         }
       }
@@ -753,7 +767,7 @@ template <typename T, int DP, int NT>
 __global__ void __launch_bounds__(512) join_kernel(const __grid_constant__ oc_paged_decode_args a, int wave, int late_ctas) {
   constexpr int HT = 8 * NT, MOST = 16;
   const int W = blockDim.x >> 5;
-  __shared__ float sm[MOST][2];
+  __shared__ float sm[MOST][3];
   __shared__ float so[MOST][DP];
   pdl_launch_dependents();
   pdl_wait();
@@ -772,18 +786,19 @@ __global__ void __launch_bounds__(512) join_kernel(const __grid_constant__ oc_pa
     return ws.states + (int64_t)(2 * c + slot) * state_floats(HT, DP);
   };
   // each warp joins every W-th part by itself, then the warps' states are joined
-  float top = -INFINITY, sum = 0.f, x[DP / 32];
+  float top = -INFINITY, sum = 0.f, exact = 0.f, x[DP / 32];
 #pragma unroll
   for (int i = 0; i < DP / 32; ++i) x[i] = 0.f;
   constexpr int U = 5;  // parts whose loads go out together
   for (int c = c0 + warp; c <= c1; c += U * W) {
-    float mc[U], lc[U], v[U][DP / 32];
+    float mc[U], lc[U], le[U], v[U][DP / 32];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const bool on = c + u * W <= c1;
       const float* s = state(on ? c + u * W : c);
-      mc[u] = s[HT * DP + 2 * hr];
-      lc[u] = s[HT * DP + 2 * hr + 1];
+      mc[u] = s[HT * DP + 4 * hr];
+      lc[u] = s[HT * DP + 4 * hr + 1];
+      le[u] = s[HT * DP + 4 * hr + 2];
 #pragma unroll
       for (int i = 0; i < DP / 32; ++i) v[u][i] = s[hr * DP + lane + 32 * i];
       if (!on) {
@@ -799,6 +814,7 @@ __global__ void __launch_bounds__(512) join_kernel(const __grid_constant__ oc_pa
       const float back = top == -INFINITY ? 1.f : exp2f(top - m), f = mc[u] == -INFINITY ? 1.f : exp2f(mc[u] - m);
       top = m;
       sum = fmaf(lc[u], f, sum * back);
+      exact = fmaf(le[u], f, exact * back);
 #pragma unroll
       for (int i = 0; i < DP / 32; ++i) x[i] = fmaf(v[u][i], f, x[i] * back);
     }
@@ -808,15 +824,19 @@ __global__ void __launch_bounds__(512) join_kernel(const __grid_constant__ oc_pa
   if (lane == 0) {
     sm[warp][0] = top;
     sm[warp][1] = sum;
+    sm[warp][2] = exact;
   }
   __syncthreads();
   top = -INFINITY;
   for (int w = 0; w < W; ++w) top = fmaxf(top, sm[w][0]);
-  float all = 0.f, f[MOST];
+  float all = 0.f, all_exact = 0.f, f[MOST];
 #pragma unroll
   for (int w = 0; w < MOST; ++w) {
     f[w] = w >= W ? 0.f : sm[w][0] == -INFINITY ? (sm[w][1] == 0.f ? 0.f : 1.f) : exp2f(sm[w][0] - top);
-    if (w < W) all = fmaf(sm[w][1], f[w], all);
+    if (w < W) {
+      all = fmaf(sm[w][1], f[w], all);
+      all_exact = fmaf(sm[w][2], f[w], all_exact);
+    }
   }
   const float inv = all == 0.f ? 0.f : a.v_scale / all;
   T* out = static_cast<T*>(a.out) + (int64_t)seq * a.out_seq_stride + (int64_t)h * a.out_head_stride;
@@ -829,7 +849,7 @@ __global__ void __launch_bounds__(512) join_kernel(const __grid_constant__ oc_pa
   }
   if (a.lse && threadIdx.x == 0)
     a.lse[(int64_t)seq * a.kv_heads * a.group + h] =
-        all == 0.f ? -INFINITY : ((top == -INFINITY ? 0.f : top) + log2f(all)) * kLn2;
+        all == 0.f ? -INFINITY : ((top == -INFINITY ? 0.f : top) + log2f(all_exact)) * kLn2;
 }
 
 // ------------------------------------------------------------------ any type, any alignment

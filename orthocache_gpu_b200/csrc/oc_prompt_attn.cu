@@ -113,6 +113,11 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&v);
   }
 }
+template <bool BF16>
+__device__ __forceinline__ float2 unpack16(uint32_t two) {
+  if constexpr (BF16) return float2{__uint_as_float(two << 16), __uint_as_float(two & 0xffff0000u)};
+  return __half22float2(*reinterpret_cast<const __half2*>(&two));
+}
 
 // k tanh(r x) of 128 scores.  |r x| <= 3/4 for the whole warp, the rule with
 // caps of some tens: x times an even polynomial, fitted to the smallest largest
@@ -151,8 +156,9 @@ __device__ __forceinline__ void cap_scores(float* s, float r, float k) {
 }
 
 // GENERAL: scores are capped, biased or scaled by a factor that is not
-// positive; else the scale is folded into the exponential.
-template <typename T, int DP, bool GENERAL>
+// positive; else the scale is folded into the exponential.  LSE: the logarithm
+// of the sum is asked for.
+template <typename T, int DP, bool GENERAL, bool LSE>
 __global__ void __launch_bounds__(kThreads, 1)
     prompt_kernel(const __grid_constant__ oc_prompt_args a, const __grid_constant__ Maps maps) {
   using L = Tile<DP>;
@@ -413,6 +419,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float c = GENERAL ? 1.f : a.scale * kLog2e;
         const float inv_cap = a.softcap > 0.f ? a.scale / a.softcap : 0.f;
         float m = -INFINITY, l = 0.f;
+        float le = 0.f;  // LSE: the sum of the weights before rounding
         float odd = 0.f;  // becomes NaN if a score or a result is not finite
         int done = 0;
         for (int j = next(-1); j < key_tiles; j = next(j)) {
@@ -472,6 +479,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const float back = grow ? (m == -INFINITY ? 0.f : ex2((m - m_new) * c)) : 1.f;
             m = m_new;
             l *= back;
+            if (LSE) le *= back;
             if (done > 0) {
               if (!wait_all(o_full(t), (done - 1) & 1)) break;
               tc_fence_after();
@@ -489,7 +497,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           const float mc = m == -INFINITY ? 0.f : m * c;
           const float2 c2 = both(c), mc2 = both(offset - mc);
-          float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
+          float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}}, exact = {0.f, 0.f};
           // 32 keys at a time: P goes out while the next are computed
           auto weigh = [&](int x) {
             uint32_t q[16];
@@ -498,8 +506,11 @@ __global__ void __launch_bounds__(kThreads, 1)
               float2 e = fma2(float2{s[x * 32 + 2 * i], s[x * 32 + 2 * i + 1]}, c2, mc2);
               e.x = ex2(e.x);
               e.y = ex2(e.y);
-              sum[i & 1] = add2(sum[i & 1], e);
               q[i] = pack16<BF16>(e.x, e.y);
+              // the sum is that of the rounded weights, the ones that the values get: a row with one large weight
+              // loses nothing
+              if (LSE) exact = add2(exact, e);
+              sum[i & 1] = add2(sum[i & 1], unpack16<BF16>(q[i]));
             }
             tmem_st16(s_at + x * 16, q);
           };
@@ -516,6 +527,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           hand_over(p_full(t));
           sum[0] = add2(sum[0], sum[1]);
           l += sum[0].x + sum[0].y;
+          if (LSE) le += exact.x + exact.y;
           ++done;
         }
         // ---------------------------------------------------------- output
@@ -548,9 +560,9 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (mine && d < a.head_dim) *reinterpret_cast<Vec<T, 8>*>(out + d) = v;
             }
           }
-          if (mine && a.lse)
+          if (LSE && mine)
             a.lse[(row0 + r) * a.lse_tok_stride + h] =
-                l == 0.f ? -INFINITY : ((m == -INFINITY ? 0.f : m * c) + log2f(l)) * kLn2;
+                l == 0.f ? -INFINITY : ((m == -INFINITY ? 0.f : m * c) + log2f(le)) * kLn2;
           // rows that are not finite, again from the definition (their tile of Q is no longer needed)
           unsigned again = __ballot_sync(0xffffffffu, mine && !(odd == 0.f));
           float* qs = reinterpret_cast<float*>(raw + (base - smem_u32(raw)) + t * L::BYTES + (warp & 3) * 1024);
@@ -572,7 +584,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 [&](int x) { return !(x < doc.prefix || (x >= sw.lo && x < sw.hi)); },
                 [&](int x) { return k + x * a.k_tok_stride; }, [&](int x) { return v + x * a.v_tok_stride; },
                 [&](int x) { return fabsf((float)(pw - x)); }, [&](int d, float x) { o[d] = from_f32<T>(x); });
-            if (a.lse && lane == 0) a.lse[row * a.lse_tok_stride + h] = lse;
+            if (LSE && lane == 0) a.lse[row * a.lse_tok_stride + h] = lse;
           }
         }
       }
@@ -668,9 +680,9 @@ bool encode(CUtensorMap* map, int& swap, const void* base, int dtype, int head_d
              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int DP, bool GENERAL>
+template <typename T, int DP, bool GENERAL, bool LSE>
 int launch_tiled(const oc_prompt_args& a, const Maps& maps, unsigned tiles, void* stream) {
-  auto kernel = prompt_kernel<T, DP, GENERAL>;
+  auto kernel = prompt_kernel<T, DP, GENERAL, LSE>;
   static std::atomic<uint64_t> ready;
   if (!allow_smem(reinterpret_cast<const void*>(kernel), ready, Tile<DP>::SMEM)) return OC_ERR_CUDA;
   return launch_pdl(kernel, dim3((unsigned)(a.kv_heads * a.group), tiles), dim3(kThreads), Tile<DP>::SMEM, stream, a,
@@ -694,11 +706,12 @@ int launch(const oc_prompt_args& a, void* stream) {
   const int64_t tiles = a.tokens / (2 * kBM) + (a.cu_q ? a.docs + 2 : 1);
   if (tiles > 65535) return OC_ERR_TOO_LARGE;
   const bool general = a.softcap > 0.f || a.slopes || !(a.scale > 0.f);
-  if (a.head_dim <= 64)
-    return general ? launch_tiled<T, 64, true>(a, maps, (unsigned)tiles, stream)
-                   : launch_tiled<T, 64, false>(a, maps, (unsigned)tiles, stream);
-  return general ? launch_tiled<T, 128, true>(a, maps, (unsigned)tiles, stream)
-                 : launch_tiled<T, 128, false>(a, maps, (unsigned)tiles, stream);
+  auto by_lse = [&](auto dp, auto gen) {
+    return a.lse ? launch_tiled<T, dp(), gen(), true>(a, maps, (unsigned)tiles, stream)
+                 : launch_tiled<T, dp(), gen(), false>(a, maps, (unsigned)tiles, stream);
+  };
+  auto by_scores = [&](auto dp) { return general ? by_lse(dp, std::true_type()) : by_lse(dp, std::false_type()); };
+  return a.head_dim <= 64 ? by_scores(std::integral_constant<int, 64>()) : by_scores(std::integral_constant<int, 128>());
 }
 
 }  // namespace
