@@ -119,9 +119,9 @@ __device__ __forceinline__ float2 unpack16(uint32_t two) {
   return __half22float2(*reinterpret_cast<const __half2*>(&two));
 }
 
-// k tanh(r x) of 128 scores.  |r x| <= 3/4 for the whole warp, the rule with
+// k tanh(r x) of 128 scores.  |r x| <= 5/8 for the whole warp, the rule with
 // caps of some tens: x times an even polynomial, fitted to the smallest largest
-// absolute error (1e-8), on the multiply units; else 1 - 2 / (1 + 2^(2 x log2 e)), two
+// absolute error (3e-8), on the multiply units; else 1 - 2 / (1 + 2^(2 x log2 e)), two
 // operations of the exponential unit a score (absolute error some 1e-7).
 __device__ __forceinline__ void cap_scores(float* s, float r, float k) {
   float top = 0.f;
@@ -130,16 +130,15 @@ __device__ __forceinline__ void cap_scores(float* s, float r, float k) {
     const float2 q = mul2(float2{s[i], s[i + 1]}, float2{s[i], s[i + 1]});
     top = max3(top, q.x, q.y);
   }
-  if (__all_sync(0xffffffffu, top * r * r <= 0.5625f)) {
+  if (__all_sync(0xffffffffu, top * r * r <= 0.390625f)) {
     const float2 r2 = both(r), kr = both(k * r);
 #pragma unroll
     for (int i = 0; i < 128; i += 2) {
       const float2 v = {s[i], s[i + 1]}, x = mul2(v, r2), q = mul2(x, x);
-      float2 p = fma2(q, both(-0.0044934507459402084f), both(0.019237229600548744f));
-      p = fma2(q, p, both(-0.053149256855249405f));
-      p = fma2(q, p, both(0.13320580124855042f));
-      p = fma2(q, p, both(-0.33332470059394836f));
-      p = fma2(q, p, both(0.9999998211860657f));
+      float2 p = fma2(q, both(0.014530060812830925f), both(-0.051362860947847366f));
+      p = fma2(q, p, both(0.13291031122207642f));
+      p = fma2(q, p, both(-0.33330482244491577f));
+      p = fma2(q, p, both(0.999999463558197f));
       p = mul2(p, mul2(v, kr));
       s[i] = p.x;
       s[i + 1] = p.y;
