@@ -139,11 +139,8 @@ def require_binding():
 
 
 def call_context(t: torch.Tensor):
-    """(SM count, status word address, stream) of a call on ``t``'s device; zeros for a CPU tensor, which the
-    binding refuses."""
+    """(SM count, status word address, stream) of a call on ``t``'s device; the binding asks once per stream."""
     dev = t.device
-    if dev.type != "cuda":
-        return 0, 0, 0
     st = stream_ptr(dev)
     return num_sms(dev), workspace(dev, st).status_ptr, st
 

@@ -7,10 +7,14 @@
 // output with torch, and calls the library's C ABI
 // (include/orthocache_b200.h) directly; it adds no GPU code.  The serving
 // operators check their arguments here too: ValueError for shapes and sizes,
-// TypeError for dtypes, RuntimeError for devices.
+// TypeError for dtypes, RuntimeError for devices; a step of a small model is a
+// few microseconds on the GPU, so they take their arguments by position and
+// unpack them without conversions.
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/extension.h>
 
+#include <cmath>
 #include <cstdint>
 #include <limits>
 #include <string>
@@ -609,17 +613,176 @@ std::tuple<Tensor, Tensor> compact_pages(py::handle caches, const Tensor& tables
   return {t, r};
 }
 
+// ---------------------------------------------------------------- entry points of the serving operators
+struct Context {
+  int64_t num_sms = 0, status = 0, stream = 0;
+};
+
+// What a call on t's device needs: its current stream (asked for every time), and the SM count and the stream's
+// status word (from _lib.call_context, remembered per device and stream, as they last as long as the process).
+Context context_of(const Tensor& t) {
+  if (!t.is_cuda()) return {};  // the operator refuses it
+  static PyObject* current = nullptr;  // torch._C._cuda_getCurrentRawStream
+  static std::vector<std::pair<std::pair<int64_t, int64_t>, Context>> known;
+  if (!current) current = py::object(py::module_::import("torch._C").attr("_cuda_getCurrentRawStream")).release().ptr();
+  const int64_t device = t.get_device();
+  const py::object handle =
+      py::reinterpret_steal<py::object>(PyObject_CallFunction(current, "L", static_cast<long long>(device)));
+  if (!handle) throw python_error();
+  const int64_t stream = PyLong_AsLongLong(handle.ptr());
+  const std::pair<int64_t, int64_t> key(device, stream);
+  for (const auto& k : known)
+    if (k.first == key) return k.second;
+  const py::tuple c = py::module_::import("orthocache_gpu_b200._lib").attr("call_context")(
+      py::reinterpret_steal<py::object>(THPVariable_Wrap(t)));
+  known.push_back({key, Context{c[0].cast<int64_t>(), c[1].cast<int64_t>(), c[2].cast<int64_t>()}});
+  return known.back().second;
+}
+
+const Tensor& tensor(PyObject* o, const char* name) {
+  OC_TYPE(THPVariable_Check(o), name, " must be a tensor");
+  return THPVariable_Unpack(o);
+}
+OptTensor maybe(PyObject* o, const char* name) {
+  if (o == Py_None) return c10::nullopt;
+  return tensor(o, name);
+}
+double number(PyObject* o) {
+  const double x = PyFloat_AsDouble(o);
+  if (x == -1.0 && PyErr_Occurred()) throw python_error();
+  return x;
+}
+int64_t whole(PyObject* o) {
+  const long long x = PyLong_AsLongLong(o);
+  if (x == -1 && PyErr_Occurred()) throw python_error();
+  return x;
+}
+bool truth(PyObject* o) {
+  const int x = PyObject_IsTrue(o);
+  if (x < 0) throw python_error();
+  return x;
+}
+PyObject* give(const OptTensor& t) {
+  if (t.has_value()) return THPVariable_Wrap(*t);
+  Py_RETURN_NONE;
+}
+PyObject* give(const OptTensor& a, const OptTensor& b) {
+  PyObject *x = give(a), *y = give(b);
+  PyObject* both = PyTuple_Pack(2, x, y);
+  Py_DECREF(x);
+  Py_DECREF(y);
+  return both;
+}
+
+// q, k, v, positions, cos, sin, k_cache, v_cache, tables, seq_ids, interleaved, inverse, k_scale, v_scale, return_keys
+PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  OC_TYPE(n == 15, "rotary takes 15 arguments");
+  const OptTensor q = maybe(a[0], "q"), k = maybe(a[1], "k");
+  OC_VALUE(q.has_value() || k.has_value(), "give q, k or both");
+  const Context c = context_of(q.has_value() ? *q : *k);
+  const bool keys = truth(a[14]);
+  const auto r = rotary_append(q, k, maybe(a[2], "v"), tensor(a[3], "positions"), maybe(a[4], "cos"), maybe(a[5], "sin"),
+                               maybe(a[6], "k_cache"), maybe(a[7], "v_cache"), maybe(a[8], "block_tables"),
+                               maybe(a[9], "seq_ids"), truth(a[10]), truth(a[11]), number(a[12]), number(a[13]), keys,
+                               c.num_sms, c.status, c.stream);
+  return keys ? give(std::get<0>(r), std::get<1>(r)) : give(std::get<0>(r));
+  END_HANDLE_TH_ERRORS
+}
+
+// q, k_cache, v_cache, tables, seq_lens, scale or None, softcap, slopes, window, k_scale, v_scale, return_lse
+PyObject* py_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  OC_TYPE(n == 12, "decode takes 12 arguments");
+  const Tensor& q = tensor(a[0], "q");
+  const Context c = context_of(q);
+  const double scale = a[5] == Py_None ? 1.0 / std::sqrt((double)(q.dim() ? q.size(-1) : 1)) : number(a[5]);
+  const bool lse = truth(a[11]);
+  const auto r = paged_decode(q, tensor(a[1], "k_cache"), tensor(a[2], "v_cache"), tensor(a[3], "block_tables"),
+                              tensor(a[4], "seq_lens"), scale, number(a[6]), maybe(a[7], "alibi_slopes"), whole(a[8]),
+                              number(a[9]), number(a[10]), lse, c.num_sms, c.status, c.stream);
+  return lse ? give(std::get<0>(r), std::get<1>(r)) : give(std::get<0>(r));
+  END_HANDLE_TH_ERRORS
+}
+
+// q, k, v, cu_seqlens, cu_seqlens_k, causal, prefix_lens, window, scale or None, softcap, slopes, return_lse
+PyObject* py_prompt(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  OC_TYPE(n == 12, "prompt takes 12 arguments");
+  const Tensor& q = tensor(a[0], "q");
+  const Context c = context_of(q);
+  const double scale = a[8] == Py_None ? 1.0 / std::sqrt((double)(q.dim() ? q.size(-1) : 1)) : number(a[8]);
+  const bool lse = truth(a[11]);
+  const auto r = prompt(q, tensor(a[1], "k"), tensor(a[2], "v"), maybe(a[3], "cu_seqlens"), maybe(a[4], "cu_seqlens_k"),
+                        truth(a[5]), maybe(a[6], "prefix_lens"), whole(a[7]), scale, number(a[9]),
+                        maybe(a[10], "alibi_slopes"), lse, c.num_sms, c.status, c.stream);
+  return lse ? give(std::get<0>(r), std::get<1>(r)) : give(std::get<0>(r));
+  END_HANDLE_TH_ERRORS
+}
+
+// caches, src, dst
+PyObject* py_copy_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  OC_TYPE(n == 3, "copy_pages takes 3 arguments");
+  const Tensor& src = tensor(a[1], "src");
+  const Context c = context_of(src);
+  copy_pages(a[0], src, tensor(a[2], "dst"), c.num_sms, c.status, c.stream);
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
+// tables, lens, refs, source, block_size
+PyObject* py_fork(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  OC_TYPE(n == 5, "fork_sequences takes 5 arguments");
+  const Tensor& table = tensor(a[0], "block_tables");
+  const Context c = context_of(table);
+  const auto r = fork_sequences(table, tensor(a[1], "seq_lens"), tensor(a[2], "refcounts"), tensor(a[3], "source"),
+                                whole(a[4]), c.status, c.stream);
+  PyObject *x = THPVariable_Wrap(std::get<0>(r)), *y = THPVariable_Wrap(std::get<1>(r)),
+           *z = THPVariable_Wrap(std::get<2>(r));
+  PyObject* all = PyTuple_Pack(3, x, y, z);
+  Py_DECREF(x);
+  Py_DECREF(y);
+  Py_DECREF(z);
+  return all;
+  END_HANDLE_TH_ERRORS
+}
+
+// caches, tables, lens, refs, wanted, block_size
+PyObject* py_reserve(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  OC_TYPE(n == 6, "reserve_pages takes 6 arguments");
+  const Tensor& table = tensor(a[1], "block_tables");
+  const Context c = context_of(table);
+  reserve_pages(a[0], table, tensor(a[2], "seq_lens"), tensor(a[3], "refcounts"), tensor(a[4], "wanted"), whole(a[5]),
+                c.num_sms, c.status, c.stream);
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
+// caches, tables, refs
+PyObject* py_compact(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  OC_TYPE(n == 3, "compact_pages takes 3 arguments");
+  const Tensor& table = tensor(a[1], "block_tables");
+  const Context c = context_of(table);
+  const auto r = compact_pages(a[0], table, tensor(a[2], "refcounts"), c.num_sms, c.status, c.stream);
+  return give(std::get<0>(r), std::get<1>(r));
+  END_HANDLE_TH_ERRORS
+}
+
+#define OC_METHOD(name, fn) {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fn)), METH_FASTCALL, nullptr}
+PyMethodDef serving_methods[] = {OC_METHOD("rotary", py_rotary), OC_METHOD("decode", py_decode),
+                                 OC_METHOD("prompt", py_prompt), OC_METHOD("copy_pages", py_copy_pages),
+                                 OC_METHOD("fork_sequences", py_fork), OC_METHOD("reserve_pages", py_reserve),
+                                 OC_METHOD("compact_pages", py_compact), {nullptr, nullptr, 0, nullptr}};
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "compiled binding of the V2 / V3 decode calls and the paged-serving operators of liborthocache_b200";
   m.def("v2", &v2);
   m.def("v3", &v3);
-  m.def("rotary_append", &rotary_append);
-  m.def("paged_decode", &paged_decode);
-  m.def("prompt", &prompt);
-  m.def("copy_pages", &copy_pages);
-  m.def("fork_sequences", &fork_sequences);
-  m.def("reserve_pages", &reserve_pages);
-  m.def("compact_pages", &compact_pages);
+  if (PyModule_AddFunctions(m.ptr(), serving_methods) != 0) throw py::error_already_set();
 }

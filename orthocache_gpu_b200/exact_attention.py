@@ -32,10 +32,8 @@ def paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     Splits the work over the cache's length where there are few sequences; nothing synchronises with the
     host.  A length or a page outside its tables sets the stream's status word (:func:`check_status`).
     """
-    out, lse = _lib.require_binding().paged_decode(
-        q, k_cache, v_cache, block_tables, seq_lens, q.shape[-1] ** -0.5 if scale is None else scale, softcap,
-        alibi_slopes, window, k_scale, v_scale, return_lse, *_lib.call_context(q))
-    return (out, lse) if return_lse else out
+    return _lib.require_binding().decode(q, k_cache, v_cache, block_tables, seq_lens, scale, softcap, alibi_slopes,
+                                         window, k_scale, v_scale, return_lse)
 
 
 def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None, *,
@@ -52,7 +50,5 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     float16 and bfloat16 with head_dim a multiple of 8 up to 128; float32 up to 256.  Returns out like q,
     or (out, lse) with lse (tokens, heads) float32.
     """
-    out, lse = _lib.require_binding().prompt(
-        q, k, v, cu_seqlens, cu_seqlens_k, causal, prefix_lens, window,
-        q.shape[-1] ** -0.5 if scale is None else scale, softcap, alibi_slopes, return_lse, *_lib.call_context(q))
-    return (out, lse) if return_lse else out
+    return _lib.require_binding().prompt(q, k, v, cu_seqlens, cu_seqlens_k, causal, prefix_lens, window, scale, softcap,
+                                         alibi_slopes, return_lse)

@@ -23,7 +23,7 @@ def copy_pages(caches: Sequence[torch.Tensor], src: torch.Tensor, dst: torch.Ten
 
     A negative id skips the pair; no dst may be the src or dst of another pair.
     """
-    _lib.require_binding().copy_pages(caches, src, dst, *_lib.call_context(src))
+    _lib.require_binding().copy_pages(caches, src, dst)
 
 
 def fork_sequences(block_tables: torch.Tensor, seq_lens: torch.Tensor, refcounts: torch.Tensor, source: torch.Tensor,
@@ -34,9 +34,7 @@ def fork_sequences(block_tables: torch.Tensor, seq_lens: torch.Tensor, refcounts
     (the unfilled last one too: :func:`reserve_pages` copies it before a write); a negative source frees
     the row.  Reordering of beams, forks for sampling, and the end of a sequence are all this call.
     """
-    _, status, stream = _lib.call_context(block_tables)
-    return _lib.require_binding().fork_sequences(block_tables, seq_lens, refcounts, source, block_size, status,
-                                                 stream)
+    return _lib.require_binding().fork_sequences(block_tables, seq_lens, refcounts, source, block_size)
 
 
 def reserve_pages(caches: Sequence[torch.Tensor], block_tables: torch.Tensor, seq_lens: torch.Tensor,
@@ -49,8 +47,7 @@ def reserve_pages(caches: Sequence[torch.Tensor], block_tables: torch.Tensor, se
     and the stream's status word is set, so check it (:func:`check_status`) before the rows are written to.
     ``seq_lens`` does not change.
     """
-    _lib.require_binding().reserve_pages(caches, block_tables, seq_lens, refcounts, wanted, block_size,
-                                         *_lib.call_context(block_tables))
+    _lib.require_binding().reserve_pages(caches, block_tables, seq_lens, refcounts, wanted, block_size)
 
 
 def compact_pages(caches: Sequence[torch.Tensor], block_tables: torch.Tensor,
@@ -60,8 +57,7 @@ def compact_pages(caches: Sequence[torch.Tensor], block_tables: torch.Tensor,
     Cache contents move in place: the k-th used page at or above n goes to the k-th free one below it, so
     pages already below n stay.
     """
-    return _lib.require_binding().compact_pages(caches, block_tables, refcounts,
-                                                *_lib.call_context(block_tables))
+    return _lib.require_binding().compact_pages(caches, block_tables, refcounts)
 
 
 class PagedKVCache:

@@ -80,8 +80,8 @@ def rotary_embedding(x: torch.Tensor, positions: torch.Tensor, cos: torch.Tensor
     ``interleaved``; the rest are copied.  ``inverse`` turns back: the transposed map, which is also the
     gradient with respect to x of the forward one.
     """
-    return _lib.require_binding().rotary_append(x, None, None, positions, cos, sin, None, None, None, None,
-                                                interleaved, inverse, 1.0, 1.0, False, *_lib.call_context(x))[0]
+    return _lib.require_binding().rotary(x, None, None, positions, cos, sin, None, None, None, None, interleaved,
+                                         inverse, 1.0, 1.0, False)
 
 
 def rotary_append_paged(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,
@@ -100,7 +100,5 @@ def rotary_append_paged(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Ten
     A position outside the tables or the block table, or a page outside the cache, appends nothing and
     sets the stream's status word (:func:`check_status`).
     """
-    out, keys = _lib.require_binding().rotary_append(q, k, v, positions, cos, sin, k_cache, v_cache, block_tables,
-                                                     seq_ids, interleaved, False, k_scale, v_scale, return_keys,
-                                                     *_lib.call_context(k))
-    return (out, keys) if return_keys else out
+    return _lib.require_binding().rotary(q, k, v, positions, cos, sin, k_cache, v_cache, block_tables, seq_ids,
+                                         interleaved, False, k_scale, v_scale, return_keys)

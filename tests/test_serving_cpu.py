@@ -118,7 +118,9 @@ def test_messages_of_the_binding_carry_numbers_and_shapes():
     with pytest.raises(RuntimeError, match=r"fused_orthocache_attention_v2: invalid argument .*\(code 1\)"):
         b.v2(x[0], x, x, 1.0, 1, 148, torch.float32, None, 0, 0, 0, 0, 0)
     with pytest.raises(ValueError, match="give q, k or both"):
-        b.rotary_append(None, None, None, x, None, None, None, None, None, None, False, False, 1.0, 1.0, False, 0, 0, 0)
+        b.rotary(None, None, None, x, None, None, None, None, None, None, False, False, 1.0, 1.0, False)
+    with pytest.raises(TypeError, match="q must be a tensor"):
+        b.decode(3, *[x] * 4, None, 0.0, None, 0, 1.0, 1.0, False)
 
 
 def test_paged_cache_refuses_a_block_size_that_is_no_power_of_two():
