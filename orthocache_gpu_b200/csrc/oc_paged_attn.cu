@@ -880,7 +880,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) decode_row_kernel(const __grid
   };
   const int each = ((span.n - span.lo + kRowWarps - 1) / kRowWarps + 31) & ~31;  // keys of a warp
   const int first = min(span.n, span.lo + warp * each), last = min(span.n, first + each);
-  const float lse = attend_row<C>(
+  const float lse = attend_row<C, kRowMaxDim, false>(
       qs, a.head_dim, RowScore{a.scale * a.k_scale, a.softcap, a.slopes ? a.slopes[h] : 0.f}, a.v_scale, first, last,
       [](int) { return false; },
       [&](int j) { return row(a.k_cache, a.kc_block_stride, a.kc_head_stride, a.kc_tok_stride, j); },

@@ -578,7 +578,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const T* k = static_cast<const T*>(a.k) + doc.k0 * a.k_tok_stride + (int64_t)hk * a.k_head_stride;
             const T* v = static_cast<const T*>(a.v) + doc.k0 * a.v_tok_stride + (int64_t)hk * a.v_head_stride;
             T* o = static_cast<T*>(a.out) + row * a.out_tok_stride + (int64_t)h * a.out_head_stride;
-            const float lse = attend_row<T>(
+            const float lse = attend_row<T, 128, false>(
                 qs, a.head_dim, RowScore{a.scale, a.softcap, -slope}, 1.f, 0, doc.n,
                 [&](int x) { return !(x < doc.prefix || (x >= sw.lo && x < sw.hi)); },
                 [&](int x) { return k + x * a.k_tok_stride; }, [&](int x) { return v + x * a.v_tok_stride; },
@@ -597,8 +597,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 // ------------------------------------------------------------------ any type, any alignment
 // One warp per (query row, head).
-template <typename T>
-__global__ void __launch_bounds__(32) prompt_row_kernel(const oc_prompt_args a) {
+template <typename T, int DMAX, bool WIDE>
+__global__ void __launch_bounds__(32) prompt_row_kernel(const __grid_constant__ oc_prompt_args a) {
   __shared__ float qs[kRowMaxDim];
   pdl_launch_dependents();
   pdl_wait();
@@ -625,7 +625,7 @@ __global__ void __launch_bounds__(32) prompt_row_kernel(const oc_prompt_args a) 
   const T* k = static_cast<const T*>(a.k) + doc.k0 * a.k_tok_stride + hk * a.k_head_stride;
   const T* v = static_cast<const T*>(a.v) + doc.k0 * a.v_tok_stride + hk * a.v_head_stride;
   T* out = static_cast<T*>(a.out) + t * a.out_tok_stride + h * a.out_head_stride;
-  const float lse = attend_row<T>(
+  const float lse = attend_row<T, DMAX, WIDE>(
       qs, a.head_dim, RowScore{a.scale, a.softcap, a.slopes ? -a.slopes[h] : 0.f}, 1.f, 0, doc.n,
       [&](int j) { return !(j < doc.prefix || (j >= see.lo && j < see.hi)); },
       [&](int j) { return k + j * a.k_tok_stride; }, [&](int j) { return v + j * a.v_tok_stride; },
@@ -635,7 +635,14 @@ __global__ void __launch_bounds__(32) prompt_row_kernel(const oc_prompt_args a) 
 
 template <typename T>
 int launch_rows(const oc_prompt_args& a, void* stream) {
-  return launch_pdl(prompt_row_kernel<T>, dim3((unsigned)a.tokens, (unsigned)(a.kv_heads * a.group)), 32, 0, stream, a);
+  auto wide = [&](const void* p, int64_t tok, int64_t head) {
+    return aligned_to(p, 16) && tok * sizeof(T) % 16 == 0 && head * sizeof(T) % 16 == 0;
+  };
+  const bool w = a.head_dim * sizeof(T) % 16 == 0 && wide(a.k, a.k_tok_stride, a.k_head_stride);
+  auto kernel = a.head_dim > 128 ? prompt_row_kernel<T, 256, false>
+                : w              ? prompt_row_kernel<T, 128, true>
+                                 : prompt_row_kernel<T, 128, false>;
+  return launch_pdl(kernel, dim3((unsigned)a.tokens, (unsigned)(a.kv_heads * a.group)), 32, 0, stream, a);
 }
 
 // ------------------------------------------------------------------ host side
@@ -704,6 +711,11 @@ int launch(const oc_prompt_args& a, void* stream) {
   // pairs of query tiles: the documents' lengths are on the device, so an upper bound; the rest leave at once
   const int64_t tiles = a.tokens / (2 * kBM) + (a.cu_q ? a.docs + 2 : 1);
   if (tiles > 65535) return OC_ERR_TOO_LARGE;
+  // A few tokens: a warp per row is through sooner than a tile is set up, and many short documents would each take a
+  // CTA for a part of its rows (31 tokens in 12 documents, 32 heads: 24 us by tiles, 5.5 by rows; 152 in 8: 15.5 and 41;
+  // one prompt of 77: 6.3 by tiles).
+  const int64_t heads = (int64_t)a.kv_heads * a.group;
+  if (a.key_tokens <= 32 || (a.key_tokens <= 64 && tiles * heads > a.num_sms)) return launch_rows<T>(a, stream);
   const bool general = a.softcap > 0.f || a.slopes || !(a.scale > 0.f);
   auto by_lse = [&](auto dp, auto gen) {
     return a.lse ? launch_tiled<T, dp(), gen(), true>(a, maps, (unsigned)tiles, stream)

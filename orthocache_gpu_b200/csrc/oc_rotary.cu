@@ -218,7 +218,8 @@ int launch(const oc_rotary_args& a, void* stream) {
 constexpr int kStages = 3, kStageBytes = 4096, kStreamWarps = 16;
 constexpr uint32_t kPolls = 1u << 22;  // bound of a wait for a copy
 
-template <typename T, typename C, int N, bool INTER>
+// JOINED: q, k and v of a token lie side by side and make one piece.
+template <typename T, typename C, int N, bool INTER, bool JOINED>
 __global__ void __launch_bounds__(kStreamWarps * 32, 1)
     rotary_stream_kernel(const __grid_constant__ oc_rotary_args a, int columns) {
   constexpr int NT = INTER ? N / 2 : N;  // table entries of a vector
@@ -235,18 +236,19 @@ __global__ void __launch_bounds__(kStreamWarps * 32, 1)
   pdl_launch_dependents();
   pdl_wait();
 
-  // a token's pieces: runs of `most` heads of q, of k, of v
+  // a token's pieces: runs of at most `most` heads of q, of k, of v, or all of them
   const int row = a.head_dim * (int)sizeof(T), most = kStageBytes / row;
-  const int nq = (a.q_heads + most - 1) / most, nk = (a.kv_heads + most - 1) / most;
-  const int pieces = nq + nk * (a.v ? 2 : 1);
+  const int hq = a.q_heads, hk = a.kv_heads, heads = hq + hk * (a.v ? 2 : 1);
+  const int nq = (hq + most - 1) / most, nk = (hk + most - 1) / most;
+  const int pieces = JOINED ? 1 : nq + nk * (a.v ? 2 : 1);
   struct Piece {
-    int part, h0, heads;  // 0 q, 1 k, 2 v
+    int part, h0, heads;  // 0 q, 1 k, 2 v; the piece's first head in the part, and how many
   };
   auto piece_of = [&](int i) {
     Piece p;
-    p.part = i < nq ? 0 : i < nq + nk ? 1 : 2;
+    p.part = JOINED || i < nq ? 0 : i < nq + nk ? 1 : 2;
     p.h0 = (p.part == 0 ? i : p.part == 1 ? i - nq : i - nq - nk) * most;
-    p.heads = min(most, (p.part == 0 ? a.q_heads : a.kv_heads) - p.h0);
+    p.heads = min(most, (JOINED ? heads : p.part == 0 ? hq : hk) - p.h0);
     return p;
   };
   const int64_t warps = (int64_t)gridDim.x * kStreamWarps, me = (int64_t)blockIdx.x * kStreamWarps + warp;
@@ -354,30 +356,38 @@ __global__ void __launch_bounds__(kStreamWarps * 32, 1)
       if (late) break;
       parity ^= 1u << stage;
       const char* in = mine + stage * kStageBytes;
+      // where a head goes: out (q, or the copy of k), and the cache; of the piece's part, or looked up head by head
       T* out = nullptr;
-      int64_t out_head = 0, cache_head = 0;
       C* cache = nullptr;
+      int64_t out_head = 0, cache_head = 0;
       float inv = 1.f;
-      if (p.part == 0) {
-        out = static_cast<T*>(a.q_out) + t * a.qo_tok_stride + lo;
-        out_head = a.qo_head_stride;
-      } else if (p.part == 1) {
-        if (a.k_out) out = static_cast<T*>(a.k_out) + t * a.ko_tok_stride + lo;
-        out_head = a.ko_head_stride;
-        if (now.page >= 0)
-          cache = static_cast<C*>(a.k_cache) + now.page * a.kc_block_stride + now.slot * a.kc_tok_stride + lo;
-        cache_head = a.kc_head_stride;
-        inv = k_inv;
-      } else {
-        if (now.page >= 0)
-          cache = static_cast<C*>(a.v_cache) + now.page * a.vc_block_stride + now.slot * a.vc_tok_stride + lo;
-        cache_head = a.vc_head_stride;
-        inv = v_inv;
-      }
-      const bool rotate = turn && p.part != 2;
+      auto place = [&](int part) {
+        if (part == 0) {
+          out = static_cast<T*>(a.q_out) + t * a.qo_tok_stride + lo;
+          out_head = a.qo_head_stride;
+          cache = nullptr;
+        } else if (part == 1) {
+          out = a.k_out ? static_cast<T*>(a.k_out) + t * a.ko_tok_stride + lo : nullptr;
+          out_head = a.ko_head_stride;
+          cache = now.page >= 0 ? static_cast<C*>(a.k_cache) + now.page * a.kc_block_stride + now.slot * a.kc_tok_stride + lo
+                                : nullptr;
+          cache_head = a.kc_head_stride;
+          inv = k_inv;
+        } else {
+          out = nullptr;
+          cache = now.page >= 0 ? static_cast<C*>(a.v_cache) + now.page * a.vc_block_stride + now.slot * a.vc_tok_stride + lo
+                                : nullptr;
+          cache_head = a.vc_head_stride;
+          inv = v_inv;
+        }
+      };
+      if (!JOINED) place(p.part);
       if (active) {
 #pragma unroll 2
         for (int h = hl; h < p.heads; h += side) {
+          const int part = !JOINED ? p.part : h < hq ? 0 : h < hq + hk ? 1 : 2;
+          const int head = !JOINED ? p.h0 + h : part == 0 ? h : part == 1 ? h - hq : h - hq - hk;
+          if (JOINED) place(part);
           const T* src = reinterpret_cast<const T*>(in + h * row) + lo;
           const Vec<T, N> xv = *reinterpret_cast<const Vec<T, N>*>(src);
           Vec<T, N> yv = {};
@@ -388,7 +398,7 @@ __global__ void __launch_bounds__(kStreamWarps * 32, 1)
             x[j] = to_f32(xv.e[j]);
             y[j] = to_f32(yv.e[j]);
           }
-          if (rotate) {
+          if (turn && part != 2) {
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
               float& u = INTER ? x[2 * j] : x[j];
@@ -399,12 +409,12 @@ __global__ void __launch_bounds__(kStreamWarps * 32, 1)
             }
           }
           if (out) {
-            T* dst = out + (p.h0 + h) * out_head;
+            T* dst = out + head * out_head;
             store_vec<T, N, true>(dst, N, x);
             if (paired) store_vec<T, N, true>(dst + half, N, y);
           }
           if (cache) {
-            C* dst = cache + (p.h0 + h) * cache_head;
+            C* dst = cache + head * cache_head;
             store_cache<C, N, true>(dst, N, x, inv);
             if (paired) store_cache<C, N, true>(dst + half, N, y, inv);
           }
@@ -444,9 +454,14 @@ int launch_aligned(const oc_rotary_args& a, void* stream) {
   int columns;
   if (!streams<T, N, INTER>(a, columns)) return launch<T, C, N, true, INTER>(a, stream);
   constexpr int smem = kStreamWarps * kStages * kStageBytes;
-  auto kernel = rotary_stream_kernel<T, C, N, INTER>;
-  static std::atomic<uint64_t> ready;
-  if (!allow_smem(reinterpret_cast<const void*>(kernel), ready, smem)) return OC_ERR_CUDA;
+  // parts of one projection's output, small enough for one piece a token (8 + 2 heads of 128: 62 us apart, 52 joined)
+  const bool joined = a.q && a.k && a.v && a.q_tok_stride == a.k_tok_stride && a.q_tok_stride == a.v_tok_stride &&
+                      static_cast<const T*>(a.q) + a.q_heads * a.head_dim == a.k &&
+                      static_cast<const T*>(a.k) + a.kv_heads * a.head_dim == a.v &&
+                      (int64_t)(a.q_heads + 2 * a.kv_heads) * a.head_dim * sizeof(T) <= kStageBytes;
+  auto kernel = joined ? rotary_stream_kernel<T, C, N, INTER, true> : rotary_stream_kernel<T, C, N, INTER, false>;
+  static std::atomic<uint64_t> ready[2];
+  if (!allow_smem(reinterpret_cast<const void*>(kernel), ready[joined], smem)) return OC_ERR_CUDA;
   const int64_t ctas = (a.tokens + kStreamWarps - 1) / kStreamWarps;
   return launch_pdl(kernel, dim3((unsigned)(ctas < a.num_sms ? ctas : a.num_sms)), dim3(kStreamWarps * 32), smem, stream,
                     a, columns);
