@@ -375,7 +375,7 @@ int oc_fused_attention_v2_noalloc(const void* q, int q_dtype, int64_t q_head_str
  * OC_ROTARY_INTERLEAVED, by the angle whose cosine and sine are cos_tab /
  * sin_tab (table_rows, rotary_dim / 2) float32; OC_ROTARY_INVERSE turns back.
  * rotary_dim 0: no rotation.  q, k (with v), k_out and the caches are each
- * optional.  Caches are of dtype, or OC_F8E4M3 holding round(k / k_scale),
+ * optional.  Caches are of dtype, or OC_F8E4M3 holding round(k (1 / k_scale)),
  * saturated.  A position outside the tables or the block table, and a page
  * outside [0, num_blocks), sets OC_STATUS_POSITION / OC_STATUS_BAD_PAGE and
  * skips the token's append. */

@@ -21,6 +21,14 @@
 // cover the latency of one another's products.  Values in slots that are not
 // visible are zeroed in shared memory before use and their scores masked, so
 // their contents have no effect.
+//
+// Measured on one B200, in a graph: 16 ragged sequences of up to 8191 tokens,
+// 32 heads of 64 in float16, 98 us for 593 MB (6.0 TB/s, 0.92 of a copy); 64
+// sequences of up to 8192, 8 heads of 128 in 8 bits, 98 us for 537 MB (5.5
+// TB/s; conversions to 16 bits keep the issue slots 54% busy); one sequence of
+// 32768 tokens, 8 heads of 128 in bfloat16, 32 us for 134 MB: 21 us of data at
+// 6.4 TB/s, the rest is the chain length, page, first copy, and the join.  300
+// tokens of one sequence: 6.2 us, that chain alone.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 

@@ -8,6 +8,12 @@
 //
 // Every element is read once and written once (k twice where k_out is asked
 // for): memory bound for prompts, launch latency for steps.
+//
+// Measured on one B200: one token of 32 + 4 heads of 64, 2.5 us in a graph and
+// 6.2 us a call, which is the host's time; 64 tokens of 32 + 8 heads of 128,
+// 3.2 us in a graph.  8191 tokens of 32 + 8 heads of 128 in bfloat16 with an
+// 8-bit cache, 38 us (4.9 TB/s of 189 MB): instructions are issued in 61% of
+// the cycles, and the conversions to 8 bits take as many as the rotation.
 #include "oc_ops.cuh"
 #include "oc_ptx.cuh"
 
@@ -350,86 +356,86 @@ __global__ void __launch_bounds__(kStreamWarps * 32, 1)
   uint32_t parity = 0;
   bool late = false;
   for (int64_t left = end - begin; left > 0; --left) {
-      if (now.page == -1 && lane == 0) raise_status(a.status, OC_STATUS_BAD_PAGE);
-      const Piece p = piece_of(i);
-      late = !__all_sync(0xffffffffu, mbar_wait_bounded(my_bar + 8 * stage, parity >> stage & 1, kPolls));
-      if (late) break;
-      parity ^= 1u << stage;
-      const char* in = mine + stage * kStageBytes;
-      // where a head goes: out (q, or the copy of k), and the cache; of the piece's part, or looked up head by head
-      T* out = nullptr;
-      C* cache = nullptr;
-      int64_t out_head = 0, cache_head = 0;
-      float inv = 1.f;
-      auto place = [&](int part) {
-        if (part == 0) {
-          out = static_cast<T*>(a.q_out) + t * a.qo_tok_stride + lo;
-          out_head = a.qo_head_stride;
-          cache = nullptr;
-        } else if (part == 1) {
-          out = a.k_out ? static_cast<T*>(a.k_out) + t * a.ko_tok_stride + lo : nullptr;
-          out_head = a.ko_head_stride;
-          cache = now.page >= 0 ? static_cast<C*>(a.k_cache) + now.page * a.kc_block_stride + now.slot * a.kc_tok_stride + lo
-                                : nullptr;
-          cache_head = a.kc_head_stride;
-          inv = k_inv;
-        } else {
-          out = nullptr;
-          cache = now.page >= 0 ? static_cast<C*>(a.v_cache) + now.page * a.vc_block_stride + now.slot * a.vc_tok_stride + lo
-                                : nullptr;
-          cache_head = a.vc_head_stride;
-          inv = v_inv;
-        }
-      };
-      if (!JOINED) place(p.part);
-      if (active) {
+    if (now.page == -1 && lane == 0) raise_status(a.status, OC_STATUS_BAD_PAGE);
+    const Piece p = piece_of(i);
+    late = !__all_sync(0xffffffffu, mbar_wait_bounded(my_bar + 8 * stage, parity >> stage & 1, kPolls));
+    if (late) break;
+    parity ^= 1u << stage;
+    const char* in = mine + stage * kStageBytes;
+    // where a head goes: out (q, or the copy of k), and the cache; of the piece's part, or looked up head by head
+    T* out = nullptr;
+    C* cache = nullptr;
+    int64_t out_head = 0, cache_head = 0;
+    float inv = 1.f;
+    auto place = [&](int part) {
+      if (part == 0) {
+        out = static_cast<T*>(a.q_out) + t * a.qo_tok_stride + lo;
+        out_head = a.qo_head_stride;
+        cache = nullptr;
+      } else if (part == 1) {
+        out = a.k_out ? static_cast<T*>(a.k_out) + t * a.ko_tok_stride + lo : nullptr;
+        out_head = a.ko_head_stride;
+        cache = now.page >= 0 ? static_cast<C*>(a.k_cache) + now.page * a.kc_block_stride + now.slot * a.kc_tok_stride + lo
+                              : nullptr;
+        cache_head = a.kc_head_stride;
+        inv = k_inv;
+      } else {
+        out = nullptr;
+        cache = now.page >= 0 ? static_cast<C*>(a.v_cache) + now.page * a.vc_block_stride + now.slot * a.vc_tok_stride + lo
+                              : nullptr;
+        cache_head = a.vc_head_stride;
+        inv = v_inv;
+      }
+    };
+    if (!JOINED) place(p.part);
+    if (active) {
 #pragma unroll 2
-        for (int h = hl; h < p.heads; h += side) {
-          const int part = !JOINED ? p.part : h < hq ? 0 : h < hq + hk ? 1 : 2;
-          const int head = !JOINED ? p.h0 + h : part == 0 ? h : part == 1 ? h - hq : h - hq - hk;
-          if (JOINED) place(part);
-          const T* src = reinterpret_cast<const T*>(in + h * row) + lo;
-          const Vec<T, N> xv = *reinterpret_cast<const Vec<T, N>*>(src);
-          Vec<T, N> yv = {};
-          if (paired) yv = *reinterpret_cast<const Vec<T, N>*>(src + half);
-          float x[N], y[N];
+      for (int h = hl; h < p.heads; h += side) {
+        const int part = !JOINED ? p.part : h < hq ? 0 : h < hq + hk ? 1 : 2;
+        const int head = !JOINED ? p.h0 + h : part == 0 ? h : part == 1 ? h - hq : h - hq - hk;
+        if (JOINED) place(part);
+        const T* src = reinterpret_cast<const T*>(in + h * row) + lo;
+        const Vec<T, N> xv = *reinterpret_cast<const Vec<T, N>*>(src);
+        Vec<T, N> yv = {};
+        if (paired) yv = *reinterpret_cast<const Vec<T, N>*>(src + half);
+        float x[N], y[N];
 #pragma unroll
-          for (int j = 0; j < N; ++j) {
-            x[j] = to_f32(xv.e[j]);
-            y[j] = to_f32(yv.e[j]);
-          }
-          if (turn && part != 2) {
+        for (int j = 0; j < N; ++j) {
+          x[j] = to_f32(xv.e[j]);
+          y[j] = to_f32(yv.e[j]);
+        }
+        if (turn && part != 2) {
 #pragma unroll
-            for (int j = 0; j < NT; ++j) {
-              float& u = INTER ? x[2 * j] : x[j];
-              float& w = INTER ? x[2 * j + 1] : y[j];
-              const float u0 = u, w0 = w;
-              u = u0 * now.c[j] - w0 * now.s[j];
-              w = w0 * now.c[j] + u0 * now.s[j];
-            }
-          }
-          if (out) {
-            T* dst = out + head * out_head;
-            store_vec<T, N, true>(dst, N, x);
-            if (paired) store_vec<T, N, true>(dst + half, N, y);
-          }
-          if (cache) {
-            C* dst = cache + head * cache_head;
-            store_cache<C, N, true>(dst, N, x, inv);
-            if (paired) store_cache<C, N, true>(dst + half, N, y, inv);
+          for (int j = 0; j < NT; ++j) {
+            float& u = INTER ? x[2 * j] : x[j];
+            float& w = INTER ? x[2 * j + 1] : y[j];
+            const float u0 = u, w0 = w;
+            u = u0 * now.c[j] - w0 * now.s[j];
+            w = w0 * now.c[j] + u0 * now.s[j];
           }
         }
+        if (out) {
+          T* dst = out + head * out_head;
+          store_vec<T, N, true>(dst, N, x);
+          if (paired) store_vec<T, N, true>(dst + half, N, y);
+        }
+        if (cache) {
+          C* dst = cache + head * cache_head;
+          store_cache<C, N, true>(dst, N, x, inv);
+          if (paired) store_cache<C, N, true>(dst + half, N, y, inv);
+        }
       }
-      __syncwarp();  // every lane has read the stage before it is filled again
-      issue();
-      stage = stage + 1 == kStages ? 0 : stage + 1;
-      if (++i == pieces) {
-        i = 0;
-        ++t;
-        now = next;
-        next = look(ahead);
-        ahead = place_of(t + 2);
-      }
+    }
+    __syncwarp();  // every lane has read the stage before it is filled again
+    issue();
+    stage = stage + 1 == kStages ? 0 : stage + 1;
+    if (++i == pieces) {
+      i = 0;
+      ++t;
+      now = next;
+      next = look(ahead);
+      ahead = place_of(t + 2);
+    }
   }
   if (late) {  // report it, and let this warp's other copies land before the CTA's memory is reused
     if (lane == 0) raise_status(a.status, OC_STATUS_TIMEOUT);

@@ -94,7 +94,7 @@ def rotary_append_paged(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Ten
     q (tokens, q_heads, head_dim), k and v (tokens, kv_heads, head_dim), strided views allowed; token t
     sits at ``positions[t]`` of sequence ``seq_ids[t]`` (default: token t belongs to sequence t; a
     negative id appends nothing).  ``cos`` / ``sin`` as in :func:`rotary_embedding`; None appends without
-    rotating (positions given by a bias instead).  float8_e4m3fn caches hold round(k / k_scale), saturated.
+    rotating (positions given by a bias instead).  float8_e4m3fn caches hold round(k (1 / k_scale)), saturated.
     Returns the rotated q, or (q, k) with ``return_keys``; q None gives None.
 
     A position outside the tables or the block table, or a page outside the cache, appends nothing and
