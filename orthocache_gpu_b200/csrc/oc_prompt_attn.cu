@@ -27,8 +27,8 @@
 // us in a graph (1240 TFLOP/s; one call after another under the power cap,
 // 537), tensor cores and exponential unit each 59% busy: what is left is the
 // hand-over between the two and the first and last tiles of a CTA.  4099
-// tokens in 7 documents, capped scores, a window of 1024, 16 heads of 128: 50
-// us: the cap's polynomial is 8 packed operations for two scores, and the 2.2
+// tokens in 7 documents, capped scores, a window of 1024, 16 heads of 128: 45
+// us: the cap's polynomial is 6 packed operations for two scores, and the 2.2
 // CTAs an SM end unevenly.
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -121,33 +121,49 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&v);
   }
 }
+// a + the two 16-bit numbers of a word: an addition of mixed types each, without conversions (a causal prompt of 8192
+// tokens, 32 heads of 128: 448 -> 441 us; capped, a window of 1024: 79 -> 75).
 template <bool BF16>
-__device__ __forceinline__ float2 unpack16(uint32_t two) {
-  if constexpr (BF16) return float2{__uint_as_float(two << 16), __uint_as_float(two & 0xffff0000u)};
-  return __half22float2(*reinterpret_cast<const __half2*>(&two));
+__device__ __forceinline__ float2 add16(float2 a, uint32_t two) {
+  float2 r;
+  if constexpr (BF16)
+    asm("{.reg .b16 l, h; mov.b32 {l, h}, %2; add.rn.f32.bf16 %0, l, %3; add.rn.f32.bf16 %1, h, %4;}"
+        : "=f"(r.x), "=f"(r.y)
+        : "r"(two), "f"(a.x), "f"(a.y));
+  else
+    asm("{.reg .b16 l, h; mov.b32 {l, h}, %2; add.rn.f32.f16 %0, l, %3; add.rn.f32.f16 %1, h, %4;}"
+        : "=f"(r.x), "=f"(r.y)
+        : "r"(two), "f"(a.x), "f"(a.y));
+  return r;
 }
 
 // k tanh(r x) of 128 scores.  |r x| <= 5/8 for the whole warp, the rule with
 // caps of some tens: x times an even polynomial, fitted to the smallest largest
-// absolute error (3e-8), on the multiply units; else 1 - 2 / (1 + 2^(2 x log2 e)), two
-// operations of the exponential unit a score (absolute error some 1e-7).
+// absolute error (3e-8), on the multiply units, with k and the powers of r in
+// the coefficients (6 packed operations for two scores; the coefficients are
+// made anew for each tile, since 10 more registers held across tiles spill); else
+// 1 - 2 / (1 + 2^(2 x log2 e)), two operations of the exponential unit a score
+// (absolute error some 1e-7).
 __device__ __forceinline__ void cap_scores(float* s, float r, float k) {
-  float top = 0.f;
+  float tops[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int i = 0; i < 128; i += 2) {
-    const float2 q = mul2(float2{s[i], s[i + 1]}, float2{s[i], s[i + 1]});
-    top = max3(top, q.x, q.y);
-  }
-  if (__all_sync(0xffffffffu, top * r * r <= 0.390625f)) {
-    const float2 r2 = both(r), kr = both(k * r);
+  for (int i = 0; i < 128; i += 2) tops[i >> 1 & 3] = max3_abs(tops[i >> 1 & 3], s[i], s[i + 1]);
+  const float top = max3(max3(tops[0], tops[1], tops[2]), tops[3], tops[3]);
+  if (__all_sync(0xffffffffu, fabsf(top * r) <= 0.625f)) {
+    float f;
+    asm volatile("mul.f32 %0, %1, %2;" : "=f"(f) : "f"(k), "f"(r));  // volatile: not moved out of the loop over tiles
+    const float r2 = r * r;
+    const float2 c0 = both(0.999999463558197f * f), c1 = both(-0.33330482244491577f * (f *= r2)),
+                 c2 = both(0.13291031122207642f * (f *= r2)), c3 = both(-0.051362860947847366f * (f *= r2)),
+                 c4 = both(0.014530060812830925f * (f *= r2));
 #pragma unroll
     for (int i = 0; i < 128; i += 2) {
-      const float2 v = {s[i], s[i + 1]}, x = mul2(v, r2), q = mul2(x, x);
-      float2 p = fma2(q, both(0.014530060812830925f), both(-0.051362860947847366f));
-      p = fma2(q, p, both(0.13291031122207642f));
-      p = fma2(q, p, both(-0.33330482244491577f));
-      p = fma2(q, p, both(0.999999463558197f));
-      p = mul2(p, mul2(v, kr));
+      const float2 v = {s[i], s[i + 1]}, q = mul2(v, v);
+      float2 p = fma2(q, c4, c3);
+      p = fma2(q, p, c2);
+      p = fma2(q, p, c1);
+      p = fma2(q, p, c0);
+      p = mul2(p, v);
       s[i] = p.x;
       s[i + 1] = p.y;
     }
@@ -467,12 +483,19 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
             }
           }
-          // the mask, where it cuts this tile for some row of the warp
+          // the mask, where it cuts this tile for some row of the warp: the upper end, then what lies between the
+          // prefix and the lower end
           const bool whole = k0 + kBN <= doc.prefix || (k0 >= see.lo && k0 + kBN <= see.hi);
           if (!__all_sync(0xffffffffu, whole)) {
+            const int pre = doc.prefix - k0, hi = max(see.hi - k0, pre), lo = see.lo - k0;
+            if (__any_sync(0xffffffffu, hi < kBN)) {
 #pragma unroll
-            for (int i = 0; i < 128; ++i)
-              if (!(k0 + i < doc.prefix || (k0 + i >= see.lo && k0 + i < see.hi))) s[i] = -INFINITY;
+              for (int i = 0; i < 128; ++i) s[i] = i < hi ? s[i] : -INFINITY;
+            }
+            if (__any_sync(0xffffffffu, lo > max(pre, 0))) {
+#pragma unroll
+              for (int i = 0; i < 128; ++i) s[i] = i >= lo || i < pre ? s[i] : -INFINITY;
+            }
           }
           float top[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
@@ -517,7 +540,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               // the sum is that of the rounded weights, the ones that the values get: a row with one large weight
               // loses nothing
               if (LSE) exact = add2(exact, e);
-              sum[i & 1] = add2(sum[i & 1], unpack16<BF16>(q[i]));
+              sum[i & 1] = add16<BF16>(sum[i & 1], q[i]);
             }
             tmem_st16(s_at + x * 16, q);
           };

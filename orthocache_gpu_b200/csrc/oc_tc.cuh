@@ -86,6 +86,13 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
+// Of absolute values.
+__device__ __forceinline__ float max3_abs(float a, float b, float c) {
+  float d;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 // ------------------------------------------------------------------ descriptors
 // Shared-memory operand with the 128-byte swizzle.  group: bytes between
 // groups of 8 rows (of 8 k for an operand whose contiguous dimension is not
