@@ -7,12 +7,13 @@
 // the tensor cores at D = 128 (512 at D = 64) and 1024 cycles of the
 // exponential unit (16 a cycle), so the two are kept busy at the same time:
 // a CTA works on two tiles of 128 queries in turn, and while one tile's scores
-// go through the softmax the tensor cores multiply for the other.
+// go through the softmax the tensor cores multiply for the other.  (Short
+// documents and windows at up to 64 columns: two CTAs an SM, a tile each.)
 //
 // Roles: 4 + 4 softmax warps (a thread per query row), one warp that issues
 // the matrix instructions, one that issues the copies.  Q, K and V arrive by
 // TMA in 128-byte-swizzled panels of 64 columns; S = Q K^T and O += P V
-// accumulate in tensor memory (S0 S1 O0 O1, 512 columns); P overwrites S in 16
+// accumulate in tensor memory (S0 S1 O0 O1, at most 512 columns); P overwrites S in 16
 // bits and is the second product's operand from there, V is read as it lies
 // (contiguous in D).  O is rescaled only when a row's maximum has grown by
 // 2^8: almost never after the first tiles.  Key tiles that the mask hides from
@@ -87,18 +88,23 @@ __device__ __forceinline__ Sight sight_of(const oc_prompt_args& a, const Doc& d,
 }
 
 // ------------------------------------------------------------------ the tiled kernel
-constexpr int kBM = 128;       // queries of a tile; two tiles a CTA
+constexpr int kBM = 128;       // queries of a tile; one or two tiles a CTA
 constexpr int kBN = 128;       // keys of a tile
-constexpr int kThreads = 384;  // softmax 0, softmax 1, matrix warp, copy warp, two idle warps
 constexpr uint32_t kPolls = 1u << 22;  // bound of a wait
 
-template <int DP>
+template <int DP, int TILES_>
 struct Tile {
   static constexpr int PANEL = kBN * 128;      // bytes of 128 rows of 64 columns
   static constexpr int PANELS = DP / 64;
   static constexpr int BYTES = PANEL * PANELS;  // of a Q, K or V tile
-  static constexpr int STAGES = DP == 128 ? 5 : 8;
-  static constexpr int SMEM = (2 + STAGES) * BYTES + 1024;
+  static constexpr int TILES = TILES_;                  // of queries, a CTA
+  static constexpr int PER_SM = 3 - TILES;              // resident CTAs
+  static constexpr int STAGES = DP == 64 && TILES == 2 ? 8 : 5;  // 4 at least: copies are awaited a tile ahead
+  static constexpr int SMEM = (TILES + STAGES) * BYTES + 1024;
+  static constexpr int MATRIX = 4 * TILES, COPY = MATRIX + 1;  // warps, after the softmax warps of every tile; two more idle
+  static constexpr int THREADS = 32 * (MATRIX + 4);
+  static constexpr int COLUMNS = 512 / PER_SM;          // of tensor memory: the tiles' scores, then their outputs
+  static constexpr int OUT = 128 * TILES;
 };
 
 struct Maps {
@@ -181,16 +187,16 @@ __device__ __forceinline__ void cap_scores(float* s, float r, float k) {
 // GENERAL: scores are capped, biased or scaled by a factor that is not
 // positive; else the scale is folded into the exponential.  LSE: the logarithm
 // of the sum is asked for.
-template <typename T, int DP, bool GENERAL, bool LSE>
-__global__ void __launch_bounds__(kThreads, 1)
+template <typename T, int DP, int TILES, bool GENERAL, bool LSE>
+__global__ void __launch_bounds__(Tile<DP, TILES>::THREADS, Tile<DP, TILES>::PER_SM)
     prompt_kernel(const __grid_constant__ oc_prompt_args a, const __grid_constant__ Maps maps) {
-  using L = Tile<DP>;
+  using L = Tile<DP, TILES>;
   constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
   extern __shared__ char raw[];
   __shared__ __align__(8) uint64_t bars[2 * L::STAGES + 10];
   __shared__ uint32_t tmem_at;
   __shared__ Doc s_doc;
-  __shared__ int s_tile;  // which pair of query tiles of the document; -1: none
+  __shared__ int s_tile;  // which TILES query tiles of the document; -1: none
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
@@ -203,7 +209,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto o_full = [&](int t) { return bar0 + 8 * (2 * L::STAGES + 6 + t); };
   auto p_most = [&](int t) { return bar0 + 8 * (2 * L::STAGES + 8 + t); };  // P of the tile's first 96 keys
 
-  if (warp == 8 && lane == 0) {
+  if (warp == L::MATRIX && lane == 0) {
     for (int s = 0; s < L::STAGES; ++s) {
       mbar_init(kv_full(s), 1);
       mbar_init(kv_empty(s), 1);
@@ -217,10 +223,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     mbar_init_fence();
   }
-  if (warp == 9) tmem_alloc(smem_u32(&tmem_at), 512);
+  if (warp == L::COPY) tmem_alloc(smem_u32(&tmem_at), L::COLUMNS);
   pdl_launch_dependents();
   pdl_wait();
-  // the pair of query tiles of this CTA, the document's last pair first (causal: the longest)
+  // the query tiles of this CTA, the document's last first (causal: the longest)
   if (warp == 0) {
     int before = 0, doc = -2, tile = -1;
     for (int d0 = a.cu_q ? -1 : 0; d0 <= a.docs && tile < 0; d0 += 32) {
@@ -228,7 +234,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       int n = 0;
       if (d <= a.docs && (a.cu_q || d == 0)) {
         const Doc x = get_doc(a, d);
-        n = (int)((x.q1 - x.q0 + 2 * kBM - 1) / (2 * kBM));
+        n = (int)((x.q1 - x.q0 + TILES * kBM - 1) / (TILES * kBM));
       }
       int up = n;
 #pragma unroll
@@ -265,14 +271,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     doc.shift = __shfl_sync(0xffffffffu, s_doc.shift, 0);
     doc.prefix = __shfl_sync(0xffffffffu, s_doc.prefix, 0);
     const int h = blockIdx.x, hk = h / a.group;
-    const int64_t row0 = doc.q0 + (int64_t)pair * 2 * kBM;  // first query row of tile 0
-    const int rows = (int)min((int64_t)2 * kBM, doc.q1 - row0);
+    const int64_t row0 = doc.q0 + (int64_t)pair * TILES * kBM;  // first query row of tile 0
+    const int rows = (int)min((int64_t)TILES * kBM, doc.q1 - row0);
     const int key_tiles = (doc.n + kBN - 1) / kBN;
     // key tiles that some query of tile t sees: [lo, hi) of t, and those below `shared` (the prefix)
     const int shared = (doc.prefix + kBN - 1) / kBN;
     int from[2] = {key_tiles, key_tiles}, to[2] = {0, 0};
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+    for (int t = 0; t < TILES; ++t) {
       const int n = min(kBM, rows - t * kBM), p = (int)(row0 - doc.q0) + t * kBM + doc.shift;
       const Sight first = sight_of(a, doc, p), last = sight_of(a, doc, p + n - 1);
       if (n > 0 && last.hi > first.lo) {
@@ -282,6 +288,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     const int from_any = min(from[0], from[1]), to_any = max(to[0], to[1]);
     auto need = [&](int t, int j) {
+      if (t >= TILES) return false;
       return (j < shared && rows > t * kBM) || (j >= (t ? from[1] : from[0]) && j < (t ? to[1] : to[0]));
     };
     auto next = [&](int j) {  // the next key tile that one of the two needs
@@ -301,10 +308,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       return ok;
     };
 
-    // registers: 8 warps x 32 x 208 + 4 x 32 x 88 = 384 x 168, what the CTA was launched with
-    if (warp >= 8) {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-      if (warp == 9) {
+    // registers: 8 warps x 32 x 208 + 4 x 32 x 88 = 384 x 168, or 4 x 32 x 208 + 4 x 32 x 48 = 256 x 128, what the CTA
+    // was launched with
+    if (warp >= L::MATRIX) {
+      if constexpr (TILES == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+      else asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+      if (warp == L::COPY) {
         // ------------------------------------------------------------ copies
         if (lane == 0) {
           auto tile_in = [&](const CUtensorMap* map, int swap, int head, int64_t row, uint32_t dst, uint32_t bar) {
@@ -317,13 +326,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           auto stage_in = [&](const CUtensorMap* map, int swap, int j) {
             const int s = idx % L::STAGES;
             if (!wait(kv_empty(s), ((idx / L::STAGES) & 1) ^ 1)) return;
-            tile_in(map, swap, hk, doc.k0 + (int64_t)j * kBN, base + (2 + s) * L::BYTES, kv_full(s));
+            tile_in(map, swap, hk, doc.k0 + (int64_t)j * kBN, base + (TILES + s) * L::BYTES, kv_full(s));
             ++idx;
           };
           if (start < key_tiles) {
             tile_in(&maps.q, maps.q_swap, h, row0, base, q_full(0));
             stage_in(&maps.k, maps.k_swap, start);
-            if (rows > kBM) tile_in(&maps.q, maps.q_swap, h, row0 + kBM, base + L::BYTES, q_full(1));
+            if (TILES == 2 && rows > kBM) tile_in(&maps.q, maps.q_swap, h, row0 + kBM, base + L::BYTES, q_full(1));
             for (int j = start; j < key_tiles && ok;) {
               stage_in(&maps.v, maps.v_swap, j);
               j = next(j);
@@ -333,20 +342,20 @@ __global__ void __launch_bounds__(kThreads, 1)
           // every copy has landed before the CTA's memory is given back
           if (start < key_tiles) {
             mbar_wait_bounded(q_full(0), 0, kPolls);
-            if (rows > kBM) mbar_wait_bounded(q_full(1), 0, kPolls);
+            if (TILES == 2 && rows > kBM) mbar_wait_bounded(q_full(1), 0, kPolls);
           }
           for (int i = idx > L::STAGES ? idx - L::STAGES : 0; i < idx; ++i)
             mbar_wait_bounded(kv_full(i % L::STAGES), (i / L::STAGES) & 1, kPolls);
         }
         __syncwarp();
-      } else if (warp == 8) {
+      } else if (warp == L::MATRIX) {
         // ------------------------------------------------------------ matrix instructions
         if (start < key_tiles) {
           constexpr uint32_t qk = instr_desc(kBM, kBN, BF16, false), pv = instr_desc(kBM, DP, BF16, true);
           constexpr uint32_t hi = smem_desc_hi(1024);
           const bool one = elect_one();
-          const uint32_t q_lo = smem_desc_lo(base, 16), k_lo = smem_desc_lo(base + 2 * L::BYTES, 16),
-                         v_lo = smem_desc_lo(base + 2 * L::BYTES, L::PANEL);
+          const uint32_t q_lo = smem_desc_lo(base, 16), k_lo = smem_desc_lo(base + TILES * L::BYTES, 16),
+                         v_lo = smem_desc_lo(base + TILES * L::BYTES, L::PANEL);
           int done[2] = {0, 0};  // tiles whose P V has been issued
           auto scores = [&](int t, int stage) {
             if (one) {
@@ -367,7 +376,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (one) {
 #pragma unroll
               for (int k = 0; k < 6; ++k)
-                tc_mma_ts(tmem + 256 + t * 128, tmem + t * 128 + k * 8, va + ((k * 2048) >> 4), hi, pv,
+                tc_mma_ts(tmem + L::OUT + t * 128, tmem + t * 128 + k * 8, va + ((k * 2048) >> 4), hi, pv,
                           done[t] > 0 || k > 0);
             }
             if (!wait_all(p_full(t), done[t] & 1)) return;
@@ -375,7 +384,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (one) {
 #pragma unroll
               for (int k = 6; k < 8; ++k)
-                tc_mma_ts(tmem + 256 + t * 128, tmem + t * 128 + k * 8, va + ((k * 2048) >> 4), hi, pv, true);
+                tc_mma_ts(tmem + L::OUT + t * 128, tmem + t * 128 + k * 8, va + ((k * 2048) >> 4), hi, pv, true);
               tc_commit(o_full(t));
             }
             ++done[t];
@@ -385,7 +394,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           };
           wait_all(kv_full(0), 0);
 #pragma unroll
-          for (int t = 0; t < 2; ++t)
+          for (int t = 0; t < TILES; ++t)
             if (ok && rows > t * kBM && wait_all(q_full(t), 0) && need(t, start)) scores(t, 0);
           free_stage(0);
           // A wait, even for a barrier that has completed, takes some 200 cycles next to operands that stream from
@@ -431,7 +440,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // ------------------------------------------------------------ softmax: a thread per query row
       const int t = warp >> 2, r = t * kBM + (warp & 3) * 32 + lane;  // row of the pair
       const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-      const uint32_t s_at = tmem + lanes + t * 128, o_at = tmem + lanes + 256 + t * 128;
+      const uint32_t s_at = tmem + lanes + t * 128, o_at = tmem + lanes + L::OUT + t * 128;
       const bool active = rows > t * kBM;
       if (active) {
         const bool mine = r < rows;
@@ -623,7 +632,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 9) tmem_free(tmem, 512);
+  if (warp == L::COPY) tmem_free(tmem, L::COLUMNS);
 }
 
 // ------------------------------------------------------------------ any type, any alignment
@@ -717,13 +726,13 @@ bool encode(CUtensorMap* map, int& swap, const void* base, int dtype, int head_d
              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int DP, bool GENERAL, bool LSE>
+template <typename T, int DP, int TILES, bool GENERAL, bool LSE>
 int launch_tiled(const oc_prompt_args& a, const Maps& maps, unsigned tiles, void* stream) {
-  auto kernel = prompt_kernel<T, DP, GENERAL, LSE>;
+  using L = Tile<DP, TILES>;
+  auto kernel = prompt_kernel<T, DP, TILES, GENERAL, LSE>;
   static std::atomic<uint64_t> ready;
-  if (!allow_smem(reinterpret_cast<const void*>(kernel), ready, Tile<DP>::SMEM)) return OC_ERR_CUDA;
-  return launch_pdl(kernel, dim3((unsigned)(a.kv_heads * a.group), tiles), dim3(kThreads), Tile<DP>::SMEM, stream, a,
-                    maps);
+  if (!allow_smem(reinterpret_cast<const void*>(kernel), ready, L::SMEM)) return OC_ERR_CUDA;
+  return launch_pdl(kernel, dim3((unsigned)(a.kv_heads * a.group), tiles), dim3(L::THREADS), L::SMEM, stream, a, maps);
 }
 
 template <typename T>
@@ -739,8 +748,14 @@ int launch(const oc_prompt_args& a, void* stream) {
       !encode(&maps.v, maps.v_swap, a.v, a.dtype, a.head_dim, a.key_tokens, a.kv_heads, a.v_tok_stride,
               a.v_head_stride))
     return launch_rows<T>(a, stream);
-  // pairs of query tiles: the documents' lengths are on the device, so an upper bound; the rest leave at once
-  const int64_t tiles = a.tokens / (2 * kBM) + (a.cu_q ? a.docs + 2 : 1);
+  // Two query tiles a CTA share every copy of K and V; one a CTA, two CTAs an SM, begin and end apart and waste less at
+  // the edges of documents and windows.  Up to 64 columns the second have room, and a document of some 4096 tokens, or
+  // a window, is where they meet (32 heads of 64: a window of 512 in 8192 tokens 100 us by two, 88 by one; 16 heads,
+  // 2048 tokens capped 49 and 45; 3001 tokens 61.4 and 60.3; 32 heads, 8192 tokens 380 and 390).
+  const int64_t reach = a.cu_q && a.docs > 0 ? a.key_tokens / a.docs : a.key_tokens;
+  const int per_cta = a.head_dim <= 64 && (reach <= 4096 || (a.window > 0 && a.window <= 4096)) ? 1 : 2;
+  // groups of query tiles: the documents' lengths are on the device, so an upper bound; the rest leave at once
+  const int64_t tiles = a.tokens / (per_cta * kBM) + (a.cu_q ? a.docs + 2 : 1);
   if (tiles > 65535) return OC_ERR_TOO_LARGE;
   // A few tokens: a warp per row is through sooner than a tile is set up, and many short documents would each take a
   // CTA for a part of its rows (31 tokens in 12 documents, 32 heads: 24 us by tiles, 5.5 by rows; 152 in 8: 15.5 and 41;
@@ -748,12 +763,17 @@ int launch(const oc_prompt_args& a, void* stream) {
   const int64_t heads = (int64_t)a.kv_heads * a.group;
   if (a.key_tokens <= 32 || (a.key_tokens <= 64 && tiles * heads > a.num_sms)) return launch_rows<T>(a, stream);
   const bool general = a.softcap > 0.f || a.slopes || !(a.scale > 0.f);
-  auto by_lse = [&](auto dp, auto gen) {
-    return a.lse ? launch_tiled<T, dp(), gen(), true>(a, maps, (unsigned)tiles, stream)
-                 : launch_tiled<T, dp(), gen(), false>(a, maps, (unsigned)tiles, stream);
+  auto by_lse = [&](auto dp, auto n, auto gen) {
+    return a.lse ? launch_tiled<T, dp(), n(), gen(), true>(a, maps, (unsigned)tiles, stream)
+                 : launch_tiled<T, dp(), n(), gen(), false>(a, maps, (unsigned)tiles, stream);
   };
-  auto by_scores = [&](auto dp) { return general ? by_lse(dp, std::true_type()) : by_lse(dp, std::false_type()); };
-  return a.head_dim <= 64 ? by_scores(std::integral_constant<int, 64>()) : by_scores(std::integral_constant<int, 128>());
+  auto by_scores = [&](auto dp, auto n) {
+    return general ? by_lse(dp, n, std::true_type()) : by_lse(dp, n, std::false_type());
+  };
+  using std::integral_constant;
+  if (a.head_dim > 64) return by_scores(integral_constant<int, 128>(), integral_constant<int, 2>());
+  return per_cta == 2 ? by_scores(integral_constant<int, 64>(), integral_constant<int, 2>())
+                      : by_scores(integral_constant<int, 64>(), integral_constant<int, 1>());
 }
 
 }  // namespace

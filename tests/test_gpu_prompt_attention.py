@@ -90,6 +90,14 @@ def test_one_document_by_default_and_long_sums():
     run([0, 4500], 1, 1, 64, torch.float16, window=1000)
 
 
+@pytest.mark.parametrize("dtype, D", [(torch.bfloat16, 64), (torch.float16, 56)])
+@pytest.mark.parametrize("cu, kw", [([0, 4353], {}), ([2, 4300], dict(softcap=30.0, alibi=True)), ([0, 8200, 8230], {}),
+                                    ([0, 4133], dict(prefix=[200], window=4100)), ([0, 4224], dict(causal=False))])
+def test_long_documents_of_narrow_heads(dtype, D, cu, kw):
+    """Documents of more than 4096 tokens on average take two query tiles a CTA where shorter ones take one."""
+    run(cu, 1, 2, D, dtype, spare=1, **kw)
+
+
 @pytest.mark.parametrize("dtype, D", [(torch.bfloat16, 64), (torch.float16, 128), (torch.float32, 24)])
 def test_hidden_nan_and_infinities_have_no_effect(dtype, D):
     cu = [0, 150, 400]
