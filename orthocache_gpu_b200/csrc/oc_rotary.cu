@@ -10,7 +10,7 @@
 // for): memory bound for prompts, launch latency for steps.
 //
 // Measured on one B200: one token of 32 + 4 heads of 64, 2.5 us in a graph and
-// 6.2 us a call, which is the host's time; 64 tokens of 32 + 8 heads of 128,
+// 5.9 us a call, which is the host's time; 64 tokens of 32 + 8 heads of 128,
 // 3.2 us in a graph.  8191 tokens of 32 + 8 heads of 128 in bfloat16 with an
 // 8-bit cache, 38 us (4.9 TB/s of 189 MB): instructions are issued in 61% of
 // the cycles, and the conversions to 8 bits take as many as the rotation.
