@@ -26,7 +26,7 @@
 //
 // Measured on one B200: 8192 tokens, causal, 32 heads of 128 in bfloat16, 441
 // us in a graph (1250 TFLOP/s; one call after another under the power cap,
-// 516), tensor cores and exponential unit each 59% busy: what is left is the
+// 516), tensor cores and exponential unit each 62% busy: what is left is the
 // hand-over between the two and the first and last tiles of a CTA.  4099
 // tokens in 7 documents, capped scores, a window of 1024, 16 heads of 128: 45
 // us: the cap's polynomial is 6 packed operations for two scores, and the 2.2
