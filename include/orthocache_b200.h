@@ -475,9 +475,11 @@ int oc_fork_sequences(const int32_t* table_in, int64_t table_in_stride, int32_t*
 
 /* Gives every sequence room for wanted[i] tokens, in place: a partly filled
  * last page that others hold too is copied (the last of its holders keeps it
- * if all of them grow), and pages are added.  The k-th page needed, by row and
- * column, is the k-th lowest free one.  All or nothing: if pages or table
- * columns do not suffice, nothing changes and OC_STATUS_PAGES is set.
+ * if all of them grow), pages behind the row's tokens that others hold (of a
+ * row that was shortened) are replaced without a copy, and pages are added.
+ * The k-th page needed, by row and column, is the k-th lowest free one.  All
+ * or nothing: if pages or table columns do not suffice, nothing changes and
+ * OC_STATUS_PAGES is set.
  * workspace: oc_reserve_workspace_bytes(num_seqs, num_pages) bytes. */
 size_t oc_reserve_workspace_bytes(int num_seqs, int64_t num_pages);
 int oc_reserve_pages(void* const* caches, const int64_t* page_strides, int num_caches, int64_t page_bytes,

@@ -319,12 +319,18 @@ struct ReserveSpace {
 
 // One CTA.  What a row needs is worked out with rows spread over the threads
 // and kept in shared memory; they are then taken in runs, one run per thread,
-// so that the prefix sum over threads is the prefix sum over rows.
+// so that the prefix sum over threads is the prefix sum over rows.  A row
+// writes to the pages from the one that its next token goes to.  Of those,
+// shared ones are replaced: the first one copied if it holds tokens of the
+// row, the ones behind it (a sequence that was shortened while others held its
+// pages) without a copy.
 __global__ void __launch_bounds__(kThreads) reserve_kernel(int32_t* table, int64_t stride, const int32_t* lens,
                                                            int32_t* refs, const int32_t* wanted, int num_seqs,
                                                            int max_blocks, int64_t num_pages, int block_size,
                                                            void* workspace, uint32_t* status) {
-  extern __shared__ int2 rows[];  // x: the page that the row shares and would write to, or -1; y: pages that it holds
+  // x: the page that the row shares and would write to first, or -1; y: pages that it holds, ~y if it shares some
+  // behind that one
+  extern __shared__ int2 rows[];
   __shared__ int32_t short_list[kShortList];
   __shared__ int bad;
   pdl_launch_dependents();
@@ -334,28 +340,34 @@ __global__ void __launch_bounds__(kThreads) reserve_kernel(int32_t* table, int64
   const int4 first_counts = four_at(refs, (int64_t)threadIdx.x * 4, num_pages, 1);
   if (threadIdx.x == 0) bad = 0;
   __syncthreads();
+  auto shared = [&](int page) { return page >= 0 && page < num_pages && refs[page] > 1; };
   // 1: the page that a growing sequence would write to and others hold too; the pages that it has
   for (int r = threadIdx.x; r < num_seqs; r += blockDim.x) {
-    const int len = lens[r], part = len / block_size;
+    const int len = lens[r], first = len / block_size;
     const int goal = pages_for(max(wanted[r], 0), block_size);
     int page = -1, held = pages_for(max(len, 0), block_size);
+    bool later = false;
     if (len < 0 || goal > max_blocks) {
       bad = 1;
-    } else {
-      const bool inside = wanted[r] > len && len % block_size != 0 && part < max_blocks;
-      const int p = inside ? table[r * stride + part] : -1;
-      while (held < goal && table[r * stride + held] >= 0) ++held;
-      if (p >= 0 && p < num_pages && refs[p] > 1) page = p;
+    } else if (wanted[r] > len) {  // so first < goal
+      const int p = table[r * stride + first];
+      for (; held < goal; ++held) {
+        const int next = table[r * stride + held];
+        if (next < 0) break;
+        if (held > first) later |= shared(next);
+      }
+      if (shared(p)) page = p;
     }
-    rows[r] = int2{page, held};
+    rows[r] = int2{page, later ? ~held : held};
   }
   __syncthreads();
   // 2: what each row needs
   const int per = (num_seqs + blockDim.x - 1) / blockDim.x, r0 = threadIdx.x * per, r1 = min(num_seqs, r0 + per);
   Two need = {0, 0};  // pages, and copies among them
-  unsigned copies = 0;  // one bit per row of the run
+  unsigned replaced = 0;  // one bit per row of the run: its first page
+  int some_later = 0;
   for (int r = r0; r < r1; ++r) {
-    const int p = rows[r].x;
+    const int p = rows[r].x, held = rows[r].y < 0 ? ~rows[r].y : rows[r].y;
     if (p >= 0) {
       int writers = 0, last = -1;
       for (int o = 0; o < num_seqs; ++o)
@@ -365,13 +377,17 @@ __global__ void __launch_bounds__(kThreads) reserve_kernel(int32_t* table, int64
         }
       // if every holder writes, the last of them keeps the page
       if (!(writers == refs[p] && last == r)) {
-        copies |= 1u << (r - r0);
+        replaced |= 1u << (r - r0);
         ++need.a;
-        ++need.b;
+        need.b += lens[r] % block_size != 0;
       }
     }
+    if (rows[r].y < 0) {
+      some_later = 1;
+      for (int c = lens[r] / block_size + 1; c < held; ++c) need.a += shared(table[r * stride + c]);
+    }
     const int goal = pages_for(max(wanted[r], 0), block_size);
-    need.a += !bad && goal > rows[r].y ? goal - rows[r].y : 0;
+    need.a += !bad && goal > held ? goal - held : 0;
   }
   Two total;
   const Two before = block_scan(need, total);
@@ -393,7 +409,7 @@ __global__ void __launch_bounds__(kThreads) reserve_kernel(int32_t* table, int64
       }
     found += sum.a;
   }
-  __syncthreads();  // the list is complete
+  some_later = __syncthreads_or(some_later);  // the list is complete
   if (bad || found < total.a) {
     if (threadIdx.x == 0) {
       raise_status(status, OC_STATUS_PAGES);
@@ -402,17 +418,36 @@ __global__ void __launch_bounds__(kThreads) reserve_kernel(int32_t* table, int64
     return;
   }
   // 4: hand them out (pages that are handed out were free: no count below is read above)
+  if (some_later) {  // which ones are shared is settled before the first count changes: entry -2 - page
+    for (int r = r0; r < r1; ++r)
+      for (int c = lens[r] / block_size + 1; c < ~rows[r].y; ++c) {
+        const int p = table[r * stride + c];
+        if (shared(p)) table[r * stride + c] = -2 - p;
+      }
+    __syncthreads();
+  }
   for (int r = r0; r < r1; ++r) {
-    if (copies >> (r - r0) & 1) {
+    const int first = lens[r] / block_size, held = rows[r].y < 0 ? ~rows[r].y : rows[r].y;
+    if (replaced >> (r - r0) & 1) {
       const int p = rows[r].x, q = list[rank++];
-      table[r * stride + lens[r] / block_size] = q;
+      table[r * stride + first] = q;
       refs[q] = 1;
       atomicSub(refs + p, 1);
-      ws.src[copied] = p;
-      ws.dst[copied++] = q;
+      if (lens[r] % block_size != 0) {
+        ws.src[copied] = p;
+        ws.dst[copied++] = q;
+      }
+    }
+    for (int c = first + 1; c < ~rows[r].y; ++c) {
+      const int p = -2 - table[r * stride + c];
+      if (p < 0) continue;
+      const int q = list[rank++];
+      table[r * stride + c] = q;
+      refs[q] = 1;
+      atomicSub(refs + p, 1);
     }
     const int goal = pages_for(max(wanted[r], 0), block_size);
-    for (int c = rows[r].y; c < goal; ++c) {
+    for (int c = held; c < goal; ++c) {
       const int q = list[rank++];
       table[r * stride + c] = q;
       refs[q] = 1;

@@ -42,9 +42,11 @@ def reserve_pages(caches: Sequence[torch.Tensor], block_tables: torch.Tensor, se
     """Make room, in place, for sequence i to grow to wanted[i] tokens.
 
     Where a row grows and its unfilled last page has other holders, the page is copied in every cache;
-    if all its holders grow, the last of them keeps it.  The k-th page needed (by row, then column) is the
-    k-th lowest free one.  All or nothing: if free pages or table columns do not suffice, nothing changes
-    and the stream's status word is set, so check it (:func:`check_status`) before the rows are written to.
+    if all its holders grow, the last of them keeps it.  A row may have been shortened since the last call:
+    the pages that it still holds behind its tokens are used again, and those of them that others hold are
+    replaced, without a copy.  The k-th page needed (by row, then column) is the k-th lowest free one.  All
+    or nothing: if free pages or table columns do not suffice, nothing changes and the stream's status word is
+    set, so check it (:func:`check_status`) before the rows are written to.
     ``seq_lens`` does not change.
     """
     _lib.require_binding().reserve_pages(caches, block_tables, seq_lens, refcounts, wanted, block_size)
