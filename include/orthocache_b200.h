@@ -407,9 +407,10 @@ int oc_rotary_append_paged(const oc_rotary_args* args, void* stream);
  *   x = scale * k_scale * q.k_j;  x = softcap * tanh(x / softcap) if softcap > 0;
  *   s_j = x + slopes[h] * (j - (seq_lens[i] - 1));
  * with window > 0 only the last window keys are seen.  A sequence of length 0
- * gives 0 and lse -inf.  Keys and values of other slots of a page are never
- * used, whatever they hold.  lse (num_seqs, heads) float32, natural
- * logarithm, is optional.  Caches are of dtype, or both OC_F8E4M3.
+ * gives 0 and lse -inf; one whose scores are all -inf gives NaN (0 / 0) and
+ * lse -inf.  Keys and values of other slots of a page are never used, whatever
+ * they hold.  lse (num_seqs, heads) float32, natural logarithm, is optional.
+ * Caches are of dtype, or both OC_F8E4M3.
  * workspace: oc_paged_decode_workspace_bytes() of the same arguments. */
 typedef struct {
   const void *q, *k_cache, *v_cache;
@@ -435,7 +436,8 @@ int oc_paged_decode_attention(const oc_paged_decode_args* args, void* stream);
  * at p sees key j of its document if j < prefix_lens[d] (when given), or if
  * (j <= p or not causal) and (window == 0 or j > p - window).  Scores as in
  * oc_paged_decode_attention, with the bias - slopes[h] * |p - j|.  A query
- * that sees nothing, and a row outside every document, gives 0 and lse -inf.
+ * that sees nothing, and a row outside every document, gives 0 and lse -inf;
+ * one whose visible scores are all -inf gives NaN and lse -inf.
  * lse (tokens, heads) float32 is optional.  OC_F16, OC_BF16: head_dim a
  * multiple of 8 up to 128; OC_F32: head_dim up to 256. */
 typedef struct {

@@ -22,8 +22,10 @@ struct RowScore {
 // mask within that range; key(j) / value(j): the row's address (null: not
 // readable, counts as zeros); bias_of(j): what slope multiplies.  out(d, x)
 // takes the normalised columns.  DMAX: head_dim at most; WIDE: rows of whole,
-// aligned 16-byte vectors.  Returns the natural-log sum (-inf if empty).
-template <typename T, int DMAX, bool WIDE, typename Hidden, typename Key, typename Value, typename Bias, typename Out>
+// aligned 16-byte vectors.  Returns the natural-log sum (-inf if empty).  A row
+// without a visible key is 0, one whose visible scores are all -inf is NaN
+// (0 / 0); with PART, for one stretch of a row's keys, both are the sum itself.
+template <typename T, int DMAX, bool WIDE, bool PART, typename Hidden, typename Key, typename Value, typename Bias, typename Out>
 __device__ float attend_row(const float* q_row, int head_dim, RowScore sc, float v_scale, int first, int last,
                             Hidden hidden, Key key, Value value, Bias bias_of, Out out) {
   constexpr int C = DMAX / 32;         // columns of a lane
@@ -33,10 +35,15 @@ __device__ float attend_row(const float* q_row, int head_dim, RowScore sc, float
 #pragma unroll
   for (int i = 0; i < C; ++i) acc[i] = 0.f;
   float m = -INFINITY, l = 0.f;
+  bool some = false;  // a visible key
   for (int j0 = first; j0 < last; j0 += 32) {
     const int j = j0 + lane;
+    const bool visible = j < last && !hidden(j);
+    const unsigned seen = __ballot_sync(0xffffffffu, visible);
+    if (!seen) continue;
+    some = true;
     float s = -INFINITY;
-    if (j < last && !hidden(j)) {
+    if (visible) {
       const T* k = key(j);
       float x = 0.f;
       if (k) {
@@ -57,12 +64,9 @@ __device__ float attend_row(const float* q_row, int head_dim, RowScore sc, float
       s = x + (sc.slope != 0.f ? sc.slope * bias_of(j) : 0.f);
     }
     float top = s;
-    bool nan = s != s;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     const float m_new = fmaxf(m, top);
-    nan = __any_sync(0xffffffffu, nan);
-    if (m_new == -INFINITY && !nan) continue;  // nothing visible yet (or scores of -inf, which weigh nothing)
     // fmaxf passes NaN over: a NaN score makes p, and through it the row, NaN
     const float shift = m_new == -INFINITY ? 0.f : m_new;
     const float p = s == -INFINITY ? 0.f : exp2f((s - shift) * kLog2e);
@@ -74,7 +78,6 @@ __device__ float attend_row(const float* q_row, int head_dim, RowScore sc, float
     m = m_new;
 #pragma unroll
     for (int i = 0; i < C; ++i) acc[i] *= back;
-    const unsigned seen = __ballot_sync(0xffffffffu, s != -INFINITY);
     for (int k0 = 0; k0 < 32; k0 += U) {
       if (!(seen >> k0 & ((1u << U) - 1))) continue;
       float v[U][C];
@@ -93,7 +96,7 @@ __device__ float attend_row(const float* q_row, int head_dim, RowScore sc, float
       }
     }
   }
-  const float inv = l == 0.f ? 0.f : v_scale / l;
+  const float inv = l == 0.f ? (some && !PART ? NAN : 0.f) : v_scale / l;
 #pragma unroll
   for (int i = 0; i < C; ++i)
     if (lane + 32 * i < head_dim) out(lane + 32 * i, acc[i] * inv);

@@ -691,7 +691,8 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<sizeof(C), DP, NT>::PER_SM)
           exact = fmaf(stat[w][hr][2], f[w], exact);
         }
         const int swz = ((hr >> 1) & 3) << 3, head = h0 + n * 8 + hr;
-        const float inv = sum == 0.f ? 0.f : a.v_scale / sum;
+        // no weight at all: 0 where nothing is visible, NaN (0 / 0) where every visible score is -inf
+        const float inv = sum == 0.f ? (cs.span.n > cs.span.lo ? NAN : 0.f) : a.v_scale / sum;
         float* state = nullptr;
         if constexpr (!DIRECT)
           state = Space(a.workspace, a.num_seqs).states + (int64_t)(2 * blockIdx.x + slot) * state_floats(HT, DP);
@@ -809,17 +810,14 @@ __global__ void __launch_bounds__(512) join_kernel(const __grid_constant__ oc_pa
       le[u] = s[HT * DP + 4 * hr + 2];
 #pragma unroll
       for (int i = 0; i < DP / 32; ++i) v[u][i] = s[hr * DP + lane + 32 * i];
-      if (!on) {
-        mc[u] = -INFINITY;
-        lc[u] = 0.f;
-      }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      // a maximum of -inf with a sum that is not 0 is a NaN score: it stays
-      if (mc[u] == -INFINITY && lc[u] == 0.f) continue;
+      if (c + u * W > c1) continue;
+      // a maximum of -inf with a sum that is not 0 is a NaN score: it stays; and 0 times an infinite value is NaN
       const float m = fmaxf(top, mc[u]);
-      const float back = top == -INFINITY ? 1.f : exp2f(top - m), f = mc[u] == -INFINITY ? 1.f : exp2f(mc[u] - m);
+      const float back = top == -INFINITY ? 1.f : exp2f(top - m);
+      const float f = mc[u] == -INFINITY ? (lc[u] == 0.f ? 0.f : 1.f) : exp2f(mc[u] - m);
       top = m;
       sum = fmaf(lc[u], f, sum * back);
       exact = fmaf(le[u], f, exact * back);
@@ -846,7 +844,7 @@ __global__ void __launch_bounds__(512) join_kernel(const __grid_constant__ oc_pa
       all_exact = fmaf(sm[w][2], f[w], all_exact);
     }
   }
-  const float inv = all == 0.f ? 0.f : a.v_scale / all;
+  const float inv = all == 0.f ? NAN : a.v_scale / all;  // a unit that is split sees some keys
   T* out = static_cast<T*>(a.out) + (int64_t)seq * a.out_seq_stride + (int64_t)h * a.out_head_stride;
   for (int d = threadIdx.x; d < a.head_dim; d += blockDim.x) {
     float y = 0.f;
@@ -888,7 +886,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) decode_row_kernel(const __grid
   };
   const int each = ((span.n - span.lo + kRowWarps - 1) / kRowWarps + 31) & ~31;  // keys of a warp
   const int first = min(span.n, span.lo + warp * each), last = min(span.n, first + each);
-  const float lse = attend_row<C, kRowMaxDim, false>(
+  const float lse = attend_row<C, kRowMaxDim, false, true>(
       qs, a.head_dim, RowScore{a.scale * a.k_scale, a.softcap, a.slopes ? a.slopes[h] : 0.f}, a.v_scale, first, last,
       [](int) { return false; },
       [&](int j) { return row(a.k_cache, a.kc_block_stride, a.kc_head_stride, a.kc_tok_stride, j); },
@@ -904,13 +902,12 @@ __global__ void __launch_bounds__(kRowWarps * 32) decode_row_kernel(const __grid
     f[w] = sums[w] == -INFINITY ? 0.f : exp2f((sums[w] - (top == -INFINITY ? 0.f : top)) * kLog2e);  // NaN stays
     all += f[w];
   }
-  const float inv = all == 0.f ? 0.f : 1.f / all;
+  const float inv = all == 0.f ? (span.n > span.lo ? NAN : 0.f) : 1.f / all;
   T* out = static_cast<T*>(a.out) + seq * a.out_seq_stride + h * a.out_head_stride;
   for (int d = threadIdx.x; d < a.head_dim; d += blockDim.x) {
     float x = 0.f;
 #pragma unroll
-    for (int w = 0; w < kRowWarps; ++w)
-      if (sums[w] != -INFINITY) x = fmaf(part[w][d], f[w], x);
+    for (int w = 0; w < kRowWarps; ++w) x = fmaf(part[w][d], f[w], x);
     out[d] = from_f32<T>(x * inv);
   }
   if (a.lse && threadIdx.x == 0)

@@ -573,6 +573,8 @@ __global__ void __launch_bounds__(Tile<DP, TILES>::THREADS, Tile<DP, TILES>::PER
         if (ok && done > 0) wait_all(o_full(t), (done - 1) & 1);
         tc_fence_after();
         if (ok) {
+          // no weight at all: 0 where nothing is visible; where every visible score is -inf the definition decides
+          if (l == 0.f && (see.hi > see.lo || doc.prefix > 0)) odd = NAN;
           const float inv = l == 0.f ? 0.f : 1.f / l;
           T* out = static_cast<T*>(a.out) + (row0 + r) * a.out_tok_stride + (int64_t)h * a.out_head_stride;
 #pragma unroll
@@ -618,7 +620,7 @@ __global__ void __launch_bounds__(Tile<DP, TILES>::THREADS, Tile<DP, TILES>::PER
             const T* k = static_cast<const T*>(a.k) + doc.k0 * a.k_tok_stride + (int64_t)hk * a.k_head_stride;
             const T* v = static_cast<const T*>(a.v) + doc.k0 * a.v_tok_stride + (int64_t)hk * a.v_head_stride;
             T* o = static_cast<T*>(a.out) + row * a.out_tok_stride + (int64_t)h * a.out_head_stride;
-            const float lse = attend_row<T, 128, false>(
+            const float lse = attend_row<T, 128, false, false>(
                 qs, a.head_dim, RowScore{a.scale, a.softcap, -slope}, 1.f, 0, doc.n,
                 [&](int x) { return !(x < doc.prefix || (x >= sw.lo && x < sw.hi)); },
                 [&](int x) { return k + x * a.k_tok_stride; }, [&](int x) { return v + x * a.v_tok_stride; },
@@ -665,7 +667,7 @@ __global__ void __launch_bounds__(32) prompt_row_kernel(const __grid_constant__ 
   const T* k = static_cast<const T*>(a.k) + doc.k0 * a.k_tok_stride + hk * a.k_head_stride;
   const T* v = static_cast<const T*>(a.v) + doc.k0 * a.v_tok_stride + hk * a.v_head_stride;
   T* out = static_cast<T*>(a.out) + t * a.out_tok_stride + h * a.out_head_stride;
-  const float lse = attend_row<T, DMAX, WIDE>(
+  const float lse = attend_row<T, DMAX, WIDE, false>(
       qs, a.head_dim, RowScore{a.scale, a.softcap, a.slopes ? -a.slopes[h] : 0.f}, 1.f, 0, doc.n,
       [&](int j) { return !(j < doc.prefix || (j >= see.lo && j < see.hi)); },
       [&](int j) { return k + j * a.k_tok_stride; }, [&](int j) { return v + j * a.v_tok_stride; },

@@ -4,7 +4,8 @@ Next to the eviction kernels, which drop tiles, these attend to every visible
 key: x = scale * q.k; x = softcap * tanh(x / softcap) where asked for; a bias
 of -slope * distance per head; a mask; softmax; the sum over values.  A key
 that the mask hides has no effect, whatever its slot holds (infinities and
-NaN included), and a query that sees nothing gives 0 and a log-sum of -inf.
+NaN included), and a query that sees nothing gives 0 and a log-sum of -inf;
+one whose visible scores are all -inf gives NaN, as 0 / 0 does.
 """
 
 from __future__ import annotations
