@@ -409,8 +409,10 @@ int oc_rotary_append_paged(const oc_rotary_args* args, void* stream);
  * with window > 0 only the last window keys are seen.  A sequence of length 0
  * gives 0 and lse -inf; one whose scores are all -inf gives NaN (0 / 0) and
  * lse -inf.  Keys and values of other slots of a page are never used, whatever
- * they hold.  lse (num_seqs, heads) float32, natural logarithm, is optional.
- * Caches are of dtype, or both OC_F8E4M3.
+ * they hold; those of a page outside [0, num_blocks) count as zeros
+ * (OC_STATUS_BAD_PAGE), and a length outside its table is clamped
+ * (OC_STATUS_POSITION).  lse (num_seqs, heads) float32, natural logarithm, is
+ * optional.  Caches are of dtype, or both OC_F8E4M3.
  * workspace: oc_paged_decode_workspace_bytes() of the same arguments. */
 typedef struct {
   const void *q, *k_cache, *v_cache;

@@ -32,7 +32,6 @@
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
-#include <climits>
 #include <mutex>
 #include <utility>
 
@@ -341,53 +340,47 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<sizeof(C), DP, NT>::PER_SM)
   const int block_shift = __ffs(a.block_size) - 1;
   const int run_rows = a.block_size < S::KW ? a.block_size : S::KW, runs = S::KW / run_rows;
   Walk<S> ld = cs;
-  constexpr int kNoRun = INT_MIN;
+  static_assert(S::KW <= 32 || (S::KW == 64 && S::ROW == 64), "a lane per run: pages of one 64-byte row are not tiled");
   struct Source {
-    bool on;             // there is such a tile
-    int page, slot, hk;  // of run `lane` (+ 32 where pages are single slots); kNoRun: nothing to copy
-    int page2;
+    bool on, run;        // there is such a tile; it has a run `lane` with visible keys
+    int page, slot, hk;  // of that run
   };
   // the pages of the next tile, as the table has them: nothing waits for them here
   auto look = [&]() {
-    Source p = {ld.at < end, kNoRun, 0, 0, kNoRun};
+    Source p = {ld.at < end, false, 0, 0, 0};
     if (!p.on) return p;
     const int key0 = (ld.span.lo & -S::KW) + ld.tile * S::CT + warp * S::KW;
     p.hk = ld.sub / gtiles;
     const int32_t* table = a.block_tables + (int64_t)ld.seq * a.block_table_stride;
-    auto page_of = [&](int r) {
-      const int j = key0 + r * run_rows;
-      return r >= runs || j >= ld.span.n || j + run_rows <= ld.span.lo ? kNoRun : table[j >> block_shift];
-    };
+    const int j = key0 + lane * run_rows;
     p.slot = key0 & (a.block_size - 1);  // 0 where a tile has several runs
-    p.page = page_of(lane);
-    if (S::KW > 32 && runs > 32) p.page2 = page_of(lane + 32);
+    p.run = lane < runs && j < ld.span.n && j + run_rows > ld.span.lo;
+    if (p.run) p.page = table[j >> block_shift];
     ld.next(a, subs);
     return p;
   };
-  auto usable = [&](int page) {
-    if (page >= 0 && page < a.num_blocks) return true;
-    if (page != kNoRun) raise_status(a.status, OC_STATUS_BAD_PAGE);
-    return false;
-  };
   const uint64_t policy = policy_evict_first();
-  auto copy_run = [&](const CUtensorMap* map, const int* role, const Source& p, int page, int r, uint32_t buf,
-                      uint32_t bar) {
+  auto copy_run = [&](const CUtensorMap* map, const int* role, const Source& p, int page, uint32_t buf, uint32_t bar) {
     auto coord = [&](int i) { return role[i] == 0 ? p.slot : role[i] == 1 ? p.hk : page; };
     const int c1 = coord(0), c2 = coord(1), c3 = coord(2);
     for (int x = 0; x < S::PANELS; ++x)  // columns from head_dim on arrive as zeros
-      tma_load_4d(buf + x * (S::KW * S::PANEL) + r * run_rows * S::PANEL, map, x * (S::PANEL / (int)sizeof(C)), c1, c2,
+      tma_load_4d(buf + x * (S::KW * S::PANEL) + lane * run_rows * S::PANEL, map, x * (S::PANEL / (int)sizeof(C)), c1, c2,
                   c3, bar, policy);
   };
   // fills buffer b with K (or V) of a tile
   auto issue = [&](const CUtensorMap* map, const int* role, const Source& p, int b) {
     const uint32_t buf = my_ring + b * S::BUF, bar = my_bar + 8 * b;
-    const bool first = usable(p.page), second = S::KW > 32 && usable(p.page2);
-    int n = __popc(__ballot_sync(0xffffffffu, first));
-    if (S::KW > 32) n += __popc(__ballot_sync(0xffffffffu, second));
+    const int n = __popc(__ballot_sync(0xffffffffu, p.run));
     if (lane == 0) mbar_arrive_expect_tx(bar, n * S::PANELS * run_rows * S::PANEL);
     __syncwarp();
-    if (first) copy_run(map, role, p, p.page, lane, buf, bar);
-    if (second) copy_run(map, role, p, p.page2, lane + 32, buf, bar);
+    if (p.run) {
+      int page = p.page;
+      if (page < 0 || page >= a.num_blocks) {  // a coordinate outside the cache: the copy engine delivers zeros
+        raise_status(a.status, OC_STATUS_BAD_PAGE);
+        page = -1;
+      }
+      copy_run(map, role, p, page, buf, bar);
+    }
   };
   // The unit's queries: head g, the columns of this lane's operand (8-bit keys come out of their conversion in
   // another order: 4t, 4t + 1 | 4t + 2, 4t + 3).  Loads without branches, of a head and column that exist, so that
