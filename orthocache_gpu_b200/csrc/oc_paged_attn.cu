@@ -940,7 +940,7 @@ void plan_nt(const oc_paged_decode_args& a, Plan& p) {
   using S = Shape<ES, DP, NT>;
   const int64_t gt = (a.group + 8 * NT - 1) / (8 * NT), units = a.num_seqs * (int64_t)a.kv_heads * gt;
   int64_t most = (int64_t)a.max_blocks * a.block_size;
-  if (a.window > 0 && a.window + S::KW < most) most = a.window + S::KW;
+  if (a.window > 0 && (int64_t)a.window + S::KW < most) most = (int64_t)a.window + S::KW;
   const int64_t tiles = (most + S::CT - 1) / S::CT, wave = (int64_t)a.num_sms * S::PER_SM;
   const int64_t useful = (units * (tiles + kUnitCost) + kMinShare - 1) / kMinShare;
   p.nt = NT;
