@@ -83,8 +83,8 @@ struct Sight {
   int lo, hi;
 };
 __device__ __forceinline__ Sight sight_of(const oc_prompt_args& a, const Doc& d, int p) {
-  const int lo = a.window > 0 ? p - a.window + 1 : 0;
-  return Sight{lo < 0 ? 0 : lo, a.causal ? min(p + 1, d.n) : d.n};
+  const int64_t lo = a.window > 0 ? (int64_t)p - a.window + 1 : 0;  // p may be negative: fewer keys than queries
+  return Sight{lo < 0 ? 0 : (int)lo, a.causal ? min(p + 1, d.n) : d.n};
 }
 
 // ------------------------------------------------------------------ the tiled kernel
