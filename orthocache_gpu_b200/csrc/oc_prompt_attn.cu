@@ -74,7 +74,7 @@ __device__ __forceinline__ Doc get_doc(const oc_prompt_args& a, int d) {
     }
   }
   r.shift = r.n - (int)(r.q1 - r.q0);
-  r.prefix = a.prefix_lens && d >= 0 && d < a.docs ? min(a.prefix_lens[d], r.n) : 0;
+  r.prefix = a.prefix_lens && d >= 0 && d < a.docs ? min(max(a.prefix_lens[d], 0), r.n) : 0;
   return r;
 }
 

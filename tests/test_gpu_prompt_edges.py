@@ -31,3 +31,14 @@ def test_a_window_that_hides_nothing(dtype, D, cu, cu_k, causal, window):
     if not causal:
         assert want[1].isfinite().all()
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("dtype, D", [(torch.bfloat16, 64), (torch.float16, 128), (torch.float32, 40)])
+@pytest.mark.parametrize("prefix", [-1, -500, -2 ** 31])
+@pytest.mark.parametrize("window", [0, 40])
+def test_a_negative_prefix_is_none(dtype, D, prefix, window):
+    q, k, v = _data(500, 500, D, dtype)
+    want = oc.prompt_attention(q, k, v, _ints(0, 200, 500), window=window, prefix_lens=_ints(0, 0), return_lse=True)
+    got = oc.prompt_attention(q, k, v, _ints(0, 200, 500), window=window, prefix_lens=_ints(prefix, prefix), return_lse=True)
+    oc.check_status()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
