@@ -68,6 +68,14 @@ enum {
   OC_STATUS_PAGES = 16    /* oc_reserve_pages: too few free pages or table columns */
 };
 
+/* *word: a status word of the current device that the library keeps: zero at
+ * first, valid as long as the process, the same for every stream and graph. */
+int oc_device_status(uint32_t** word);
+
+/* Clears `bits` of a status word on the stream, atomically: bits that another
+ * launch sets meanwhile stay. */
+int oc_clear_status(uint32_t* word, uint32_t bits, void* stream);
+
 /* gate selector of oc_fused_attention_paged */
 enum { OC_GATE_ZETA = 0, OC_GATE_CAUCHY_SCHWARZ = 2 };
 

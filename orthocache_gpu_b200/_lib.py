@@ -65,6 +65,8 @@ SIGNATURES = {
     "oc_gemv_qkv_rope": (_i, [_vp, _vp, _vp, C.c_float, _vp, _vp, _i64, _i64, _i, _i, _i, _vp, _vp, _vp, _vp, _vp,
                               _vp, _i64, _i, _vp]),
     "oc_tail_merge": (_i, [_vp, _i, _i, _i, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _vp, C.c_float, _vp, _i, _vp]),
+    "oc_device_status": (_i, [_vp]),
+    "oc_clear_status": (_i, [_vp, C.c_uint32, _vp]),
     "oc_rotary_append_paged": (_i, [_vp, _vp]),
     "oc_paged_decode_workspace_bytes": (_sz, [_vp]),
     "oc_paged_decode_attention": (_i, [_vp, _vp]),
@@ -136,13 +138,6 @@ def require_binding():
         raise RuntimeError("orthocache_gpu_b200: the compiled binding (_lib/oc_torch.so) is not built, or "
                            "ORTHOCACHE_B200_LIB selects another library; run `python -m orthocache_gpu_b200._build`")
     return b
-
-
-def call_context(t: torch.Tensor):
-    """(SM count, status word address, stream) of a call on ``t``'s device; the binding asks once per stream."""
-    dev = t.device
-    st = stream_ptr(dev)
-    return num_sms(dev), workspace(dev, st).status_ptr, st
 
 
 def dtype_code(t: torch.Tensor) -> int:
@@ -251,14 +246,25 @@ def workspace(device: torch.device, stream: int | None = None) -> _Workspace:
     key = (device.index, stream)
     w = _ws.get(key)
     if w is None:
-        w = _ws[key] = _Workspace(device)
+        w = _ws.setdefault(key, _Workspace(device))  # one object, whichever thread comes first
+    return w
+
+
+_words: dict = {}
+
+
+def _device_word(device: torch.device):
+    """A view of the status word that the serving operators report to on ``device`` (None without the binding)."""
+    w = _words.get(device.index)
+    if w is None and binding() is not None:
+        w = _words[device.index] = binding().status_word(device.index)
     return w
 
 
 def _raise_status(status: int) -> None:
     bits = [m for b, m in STATUS_BITS.items() if status & b]
-    raise RuntimeError("orthocache_gpu_b200 kernel reported (a launch on this stream since the status was "
-                       "last checked): " + "; ".join(bits))
+    raise RuntimeError("orthocache_gpu_b200 kernel reported (a launch since the status was last checked): "
+                       + "; ".join(bits))
 
 
 def read_stats(ws: _Workspace) -> int:
@@ -271,20 +277,33 @@ def read_stats(ws: _Workspace) -> int:
 
 
 def check_status(device=None) -> None:
-    """Raise if a launch on ``device``'s current stream reported an error since the last check.
+    """Raise if a launch on ``device`` reported an error since the last check.
 
     Calls made with ``stats=False`` do not synchronise and so cannot raise
     themselves; their errors stay in the stream's sticky status word until
     this function (or the next ``stats=True`` call on the stream) reads it.
-    Synchronises with the stream.  Clears the word after reading it.
+    The serving operators (rotary append, exact attention, pages) report to
+    one sticky word of the device instead, from every stream and every replay
+    of a captured graph.  Synchronises with the current stream: what other
+    streams still have to run is not waited for.  Clears what it has read.
     """
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     if dev.index is None:
         dev = torch.device("cuda", torch.cuda.current_device())
-    ws = workspace(dev)
-    status = int(ws.ctrl[1].item())
+    status = 0
+    word = _device_word(dev)
+    if word is not None:
+        status = int(word.item())
+        if status:
+            with torch.cuda.device(dev):
+                check(load().oc_clear_status(word.data_ptr(), status, stream_ptr(dev)), "check_status")
+    ws = _ws.get((dev.index, stream_ptr(dev)))
+    if ws is not None:
+        own = int(ws.ctrl[1].item())
+        if own:
+            ws.ctrl[1].zero_()
+        status |= own
     if status:
-        ws.ctrl[1].zero_()
         _raise_status(status)
 
 

@@ -618,25 +618,35 @@ struct Context {
   int64_t num_sms = 0, status = 0, stream = 0;
 };
 
-// What a call on t's device needs: its current stream (asked for every time), and the SM count and the stream's
-// status word (from _lib.call_context, remembered per device and stream, as they last as long as the process).
+// The library's status word on a device.  One word for all streams: a captured call reports to the same place as an
+// eager one, whichever stream replays it, and nothing that a stream owns has to outlive it.
+uint32_t* status_of(int64_t device) {
+  const c10::DeviceGuard guard(c10::Device(c10::kCUDA, static_cast<c10::DeviceIndex>(device)));
+  uint32_t* w = nullptr;
+  check(oc_device_status(&w), "oc_device_status");
+  return w;
+}
+
+// What a call on t's device needs: its current stream (asked for every time), and the SM count and the status word
+// (remembered per device, as they last as long as the process).
 Context context_of(const Tensor& t) {
   if (!t.is_cuda()) return {};  // the operator refuses it
   static PyObject* current = nullptr;  // torch._C._cuda_getCurrentRawStream
-  static std::vector<std::pair<std::pair<int64_t, int64_t>, Context>> known;
+  static std::vector<std::pair<int64_t, Context>> known;
   if (!current) current = py::object(py::module_::import("torch._C").attr("_cuda_getCurrentRawStream")).release().ptr();
   const int64_t device = t.get_device();
   const py::object handle =
       py::reinterpret_steal<py::object>(PyObject_CallFunction(current, "L", static_cast<long long>(device)));
   if (!handle) throw python_error();
   const int64_t stream = PyLong_AsLongLong(handle.ptr());
-  const std::pair<int64_t, int64_t> key(device, stream);
   for (const auto& k : known)
-    if (k.first == key) return k.second;
-  const py::tuple c = py::module_::import("orthocache_gpu_b200._lib").attr("call_context")(
-      py::reinterpret_steal<py::object>(THPVariable_Wrap(t)));
-  known.push_back({key, Context{c[0].cast<int64_t>(), c[1].cast<int64_t>(), c[2].cast<int64_t>()}});
-  return known.back().second;
+    if (k.first == device) return Context{k.second.num_sms, k.second.status, stream};
+  const int64_t sms = py::module_::import("orthocache_gpu_b200._lib")
+                          .attr("num_sms")(py::reinterpret_steal<py::object>(THPVariable_Wrap(t)).attr("device"))
+                          .cast<int64_t>();
+  const Context c{sms, reinterpret_cast<int64_t>(status_of(device)), stream};
+  known.push_back({device, c});
+  return c;
 }
 
 const Tensor& tensor(PyObject* o, const char* name) {
@@ -784,5 +794,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "compiled binding of the V2 / V3 decode calls and the paged-serving operators of liborthocache_b200";
   m.def("v2", &v2);
   m.def("v3", &v3);
+  m.def("status_word", [](int64_t device) {  // a view of the device's status word
+    return at::from_blob(status_of(device), {1},
+                         at::TensorOptions().dtype(at::kInt).device(at::Device(at::kCUDA, static_cast<at::DeviceIndex>(device))));
+  });
   if (PyModule_AddFunctions(m.ptr(), serving_methods) != 0) throw py::error_already_set();
 }

@@ -31,7 +31,7 @@ def paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     lse (num_seqs, heads) float32, the natural logarithm of the softmax sum.
 
     Splits the work over the cache's length where there are few sequences; nothing synchronises with the
-    host.  A length or a page outside its tables sets the stream's status word (:func:`check_status`); the
+    host.  A length or a page outside its tables sets the device's status word (:func:`check_status`); the
     length is clamped, and the page's keys and values count as zeros.
     """
     return _lib.require_binding().decode(q, k_cache, v_cache, block_tables, seq_lens, scale, softcap, alibi_slopes,

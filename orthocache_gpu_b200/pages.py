@@ -45,7 +45,7 @@ def reserve_pages(caches: Sequence[torch.Tensor], block_tables: torch.Tensor, se
     if all its holders grow, the last of them keeps it.  A row may have been shortened since the last call:
     the pages that it still holds behind its tokens are used again, and those of them that others hold are
     replaced, without a copy.  The k-th page needed (by row, then column) is the k-th lowest free one.  All
-    or nothing: if free pages or table columns do not suffice, nothing changes and the stream's status word is
+    or nothing: if free pages or table columns do not suffice, nothing changes and the device's status word is
     set, so check it (:func:`check_status`) before the rows are written to.
     ``seq_lens`` does not change.
     """

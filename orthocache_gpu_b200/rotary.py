@@ -98,7 +98,7 @@ def rotary_append_paged(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Ten
     Returns the rotated q, or (q, k) with ``return_keys``; q None gives None.
 
     A position outside the tables or the block table, or a page outside the cache, appends nothing and
-    sets the stream's status word (:func:`check_status`).
+    sets the device's status word (:func:`check_status`).
     """
     return _lib.require_binding().rotary(q, k, v, positions, cos, sin, k_cache, v_cache, block_tables, seq_ids,
                                          interleaved, False, k_scale, v_scale, return_keys)
