@@ -86,7 +86,8 @@ class PagedLlama:
         """One token for every row: tokens (rows,), live (rows,) int32, 0 for idle rows; returns their logits."""
         m, c = self.m, self.cache
         c.reserve(live, check=check)
-        positions = c.seq_lens.clone()
+        # idle rows sit anywhere that exists: one that is full has no next position
+        positions = torch.where(live > 0, c.seq_lens, 0)
         c.seq_lens += live
         seq_ids = torch.where(live > 0, torch.arange(live.numel(), device=m.dev, dtype=torch.int32), -1)
         x = m.embed[tokens]
