@@ -309,8 +309,8 @@ __global__ void __launch_bounds__(kThreads) fork_kernel(const int32_t* table_in,
 }
 
 // ------------------------------------------------------------------ reserve
-// Workspace: [0] copies, then src[num_seqs], dst[num_seqs], and the free pages
-// handed out, free[num_pages].
+// Workspace: [0] copies, [1] whether the pages were reserved, then
+// src[num_seqs], dst[num_seqs], and the free pages handed out, free[num_pages].
 struct ReserveSpace {
   int32_t *count, *src, *dst, *free;
   __host__ __device__ ReserveSpace(void* p, int num_seqs)
@@ -413,7 +413,7 @@ __global__ void __launch_bounds__(kThreads) reserve_kernel(int32_t* table, int64
   if (bad || found < total.a) {
     if (threadIdx.x == 0) {
       raise_status(status, OC_STATUS_PAGES);
-      *ws.count = 0;
+      ws.count[0] = ws.count[1] = 0;
     }
     return;
   }
@@ -453,7 +453,10 @@ __global__ void __launch_bounds__(kThreads) reserve_kernel(int32_t* table, int64
       refs[q] = 1;
     }
   }
-  if (threadIdx.x == 0) *ws.count = total.b;
+  if (threadIdx.x == 0) {
+    ws.count[0] = total.b;
+    ws.count[1] = 1;
+  }
 }
 
 // ------------------------------------------------------------------ compact

@@ -566,8 +566,10 @@ std::tuple<Tensor, Tensor, Tensor> fork_sequences(const Tensor& tables, const Te
   return {t, l, r};
 }
 
-void reserve_pages(py::handle caches, const Tensor& tables, const Tensor& lens, const Tensor& refs,
-                   const Tensor& wanted_, int64_t block_size, int64_t num_sms, int64_t status, int64_t stream) {
+// Returns a tensor of one int32 on the device, 1 if the pages were reserved, else 0, where it is asked for.
+OptTensor reserve_pages(py::handle caches, const Tensor& tables, const Tensor& lens, const Tensor& refs,
+                        const Tensor& wanted_, int64_t block_size, bool return_done, int64_t num_sms, int64_t status,
+                        int64_t stream) {
   need_int32(tables, tables, "block_tables", 2);
   const c10::DeviceGuard guard(tables.device());
   need_int32(lens, tables, "seq_lens", 1);
@@ -581,15 +583,16 @@ void reserve_pages(py::handle caches, const Tensor& tables, const Tensor& lens, 
   const CacheList c(caches, tables);
   OC_VALUE(c.count() == 0 || c.num_pages == refs.size(0), "the caches have ", c.num_pages,
                     " pages, refcounts ", refs.size(0));
-  if (S == 0) return;
+  if (S == 0) return return_done ? OptTensor(at::ones({}, tables.options())) : c10::nullopt;
   const size_t bytes = oc_reserve_workspace_bytes(as_int(S, "num_seqs"), refs.size(0));
-  Tensor space = at::empty({(int64_t)bytes}, tables.options().dtype(at::kByte));
+  const Tensor space = at::empty({(int64_t)bytes / 4}, tables.options());
   check(oc_reserve_pages(c.base.data(), c.stride.data(), c.count(), c.page_bytes, tables.data_ptr<int32_t>(),
                          tables.stride(0), lens.data_ptr<int32_t>(), refs.data_ptr<int32_t>(),
                          wanted.data_ptr<int32_t>(), (int)S, as_int(tables.size(1), "max_blocks"), refs.size(0),
                          as_int(block_size, "block_size"), space.data_ptr(), bytes, word(status), (int)num_sms,
                          handle(stream)),
         "reserve_pages");
+  return return_done ? OptTensor(space.select(0, 1)) : c10::nullopt;
 }
 
 std::tuple<Tensor, Tensor> compact_pages(py::handle caches, const Tensor& tables, const Tensor& refs,
@@ -759,15 +762,14 @@ PyObject* py_fork(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// caches, tables, lens, refs, wanted, block_size
+// caches, tables, lens, refs, wanted, block_size, return_done
 PyObject* py_reserve(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  OC_TYPE(n == 6, "reserve_pages takes 6 arguments");
+  OC_TYPE(n == 7, "reserve_pages takes 7 arguments");
   const Tensor& table = tensor(a[1], "block_tables");
   const Context c = context_of(table);
-  reserve_pages(a[0], table, tensor(a[2], "seq_lens"), tensor(a[3], "refcounts"), tensor(a[4], "wanted"), whole(a[5]),
-                c.num_sms, c.status, c.stream);
-  Py_RETURN_NONE;
+  return give(reserve_pages(a[0], table, tensor(a[2], "seq_lens"), tensor(a[3], "refcounts"), tensor(a[4], "wanted"),
+                            whole(a[5]), truth(a[6]), c.num_sms, c.status, c.stream));
   END_HANDLE_TH_ERRORS
 }
 

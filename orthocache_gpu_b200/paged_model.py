@@ -83,9 +83,16 @@ class PagedLlama:
 
     @torch.no_grad()
     def step(self, tokens: torch.Tensor, live: torch.Tensor, check: bool = True) -> torch.Tensor:
-        """One token for every row: tokens (rows,), live (rows,) int32, 0 for idle rows; returns their logits."""
+        """One token for every row: tokens (rows,), live (rows,) int32, 0 for idle rows; returns their logits.
+
+        Raises if there are too few pages.  Without ``check`` the host does not wait, and a step that finds too
+        few pages leaves every sequence as it was: the device's status word tells (:func:`check_status`), and
+        the logits are of no use.
+        """
         m, c = self.m, self.cache
-        c.reserve(live, check=check)
+        done = c.reserve(live, check=check)
+        if done is not None:
+            live = live * done
         # idle rows sit anywhere that exists: one that is full has no next position
         positions = torch.where(live > 0, c.seq_lens, 0)
         c.seq_lens += live

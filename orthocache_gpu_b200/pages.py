@@ -38,7 +38,8 @@ def fork_sequences(block_tables: torch.Tensor, seq_lens: torch.Tensor, refcounts
 
 
 def reserve_pages(caches: Sequence[torch.Tensor], block_tables: torch.Tensor, seq_lens: torch.Tensor,
-                  refcounts: torch.Tensor, wanted: torch.Tensor, block_size: int) -> None:
+                  refcounts: torch.Tensor, wanted: torch.Tensor, block_size: int, *,
+                  return_done: bool = False) -> Optional[torch.Tensor]:
     """Make room, in place, for sequence i to grow to wanted[i] tokens.
 
     Where a row grows and its unfilled last page has other holders, the page is copied in every cache;
@@ -46,10 +47,13 @@ def reserve_pages(caches: Sequence[torch.Tensor], block_tables: torch.Tensor, se
     the pages that it still holds behind its tokens are used again, and those of them that others hold are
     replaced, without a copy.  The k-th page needed (by row, then column) is the k-th lowest free one.  All
     or nothing: if free pages or table columns do not suffice, nothing changes and the device's status word is
-    set, so check it (:func:`check_status`) before the rows are written to.
+    set.  Rows must not be written to then, as their pages may still be shared: check the word
+    (:func:`check_status`) first, or, where the host must not wait, take what ``return_done`` returns, a tensor
+    of one int32 on the device (1: reserved, 0: not), and let nothing grow where it is 0.
     ``seq_lens`` does not change.
     """
-    _lib.require_binding().reserve_pages(caches, block_tables, seq_lens, refcounts, wanted, block_size)
+    return _lib.require_binding().reserve_pages(caches, block_tables, seq_lens, refcounts, wanted, block_size,
+                                                return_done)
 
 
 def compact_pages(caches: Sequence[torch.Tensor], block_tables: torch.Tensor,
@@ -96,12 +100,17 @@ class PagedKVCache:
         source[list(rows)] = -1
         self.fork(source.to(self.seq_lens.device))
 
-    def reserve(self, tokens: torch.Tensor, check: bool = True) -> None:
-        """Make room for tokens[i] more tokens in row i; with ``check``, raise if there are too few pages."""
-        reserve_pages(self.caches, self.block_tables, self.seq_lens, self.refcounts, self.seq_lens + tokens,
-                      self.block_size)
+    def reserve(self, tokens: torch.Tensor, check: bool = True) -> Optional[torch.Tensor]:
+        """Make room for tokens[i] more tokens in row i; with ``check``, raise if there are too few pages.
+
+        Without ``check`` the host does not wait, and a tensor of one int32 comes back: 1, or 0 if there are too
+        few pages, in which case no row may be written to.
+        """
+        done = reserve_pages(self.caches, self.block_tables, self.seq_lens, self.refcounts, self.seq_lens + tokens,
+                             self.block_size, return_done=not check)
         if check:
             _lib.check_status(self.seq_lens.device)
+        return done
 
     def compact(self) -> None:
         """Move the pages in use to the lowest ids."""

@@ -3,6 +3,8 @@
 import pytest
 import torch
 
+import orthocache_gpu_b200 as oc
+
 pytestmark = pytest.mark.gpu
 
 VOCAB = 300
@@ -36,5 +38,55 @@ def test_a_full_idle_row_does_not_stop_the_others(kw):
     with pytest.raises(RuntimeError, match="too few free pages"):
         p.step(tokens, _ints(1, 0, 1))  # the full row cannot go on
     assert p.cache.seq_lens.tolist() == [48, 0, 8]
-    import orthocache_gpu_b200 as oc
     oc.check_status()
+
+
+def test_a_step_without_pages_changes_no_sequence_when_the_host_does_not_wait():
+    """Two samples share the unfilled page of their prompt, and no page is free."""
+    p = _paged(num_pages=1, max_seqs=2)
+    c = p.cache
+    p.prefill(_prompts(5), [0])
+    c.fork(_ints(0, 0))
+    before = [x.clone() for x in (c.block_tables, c.refcounts, c.seq_lens, *c.caches)]
+    p.step(torch.tensor([3, 4], device="cuda"), _ints(1, 1), check=False)
+    for x, y in zip((c.block_tables, c.refcounts, c.seq_lens, *c.caches), before):
+        assert torch.equal(x, y)
+    with pytest.raises(RuntimeError, match="too few free pages"):
+        oc.check_status()
+    c.fork(_ints(0, -1))  # one holder: it goes on
+    logits = p.step(torch.tensor([3, 4], device="cuda"), _ints(1, 0), check=False)
+    oc.check_status()
+    assert c.seq_lens.tolist() == [6, 0] and logits[0].isfinite().all()
+
+
+def test_steps_of_a_captured_graph_go_on_until_the_pages_are_full():
+    p = _paged(num_pages=4, max_seqs=2)
+    eager = _paged(num_pages=4, max_seqs=2)
+    for x in (p, eager):
+        x.prefill(_prompts(30, 14), [0, 1])  # three pages; the second row needs the fourth at 16 tokens, the first at 32
+    tokens, live = torch.tensor([3, 4], device="cuda"), _ints(1, 1)
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(graph, stream=side):
+        got = p.step(tokens, live, check=False)
+    for _ in range(2):
+        graph.replay()
+        assert torch.equal(got, eager.step(tokens, live))
+    oc.check_status()
+    graph.replay()  # both rows need a page, one is left
+    with pytest.raises(RuntimeError, match="too few free pages"):
+        oc.check_status()
+    assert p.cache.seq_lens.tolist() == [32, 16] and p.cache.free_pages() == 1
+
+
+def test_reserve_tells_on_the_device_whether_it_was_done():
+    c = oc.PagedKVCache(1, 4, 1, 8, max_seqs=2, max_tokens=64, block_size=4)
+    assert c.reserve(_ints(4, 4)) is None
+    done = c.reserve(_ints(8, 8), check=False)
+    assert done.is_cuda and done.dtype == torch.int32 and done.shape == () and int(done) == 1
+    oc.check_status()
+    assert int(c.reserve(_ints(9, 8), check=False)) == 0
+    with pytest.raises(RuntimeError, match="too few free pages"):
+        oc.check_status()
+    none = torch.zeros(0, dtype=torch.int32, device="cuda")
+    assert int(oc.reserve_pages([], none[:, None], none, c.refcounts, none, 4, return_done=True)) == 1
