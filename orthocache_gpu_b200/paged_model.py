@@ -61,10 +61,15 @@ class PagedLlama:
     def prefill(self, prompts: Sequence[torch.Tensor], rows: Sequence[int]) -> torch.Tensor:
         """Prompt i becomes sequence rows[i] (an idle row); returns the logits after each prompt."""
         m, s, c = self.m, self.m.s, self.cache
-        if len(prompts) != len(rows) or any(p.numel() == 0 for p in prompts):
-            raise ValueError("give one row for each prompt, and no empty prompt")
+        rows = [int(r) for r in rows]
+        if not rows or len(prompts) != len(rows) or any(p.numel() == 0 for p in prompts):
+            raise ValueError("give one row for each prompt, at least one, and no empty prompt")
+        if len(set(rows)) != len(rows) or min(rows) < 0 or max(rows) >= c.seq_lens.numel():
+            raise ValueError(f"rows ({rows}) must be distinct rows of the cache, of which there are {c.seq_lens.numel()}")
         lens = [p.numel() for p in prompts]
-        row = torch.tensor(list(rows), device=m.dev)
+        row = torch.tensor(rows, device=m.dev)
+        if bool(c.seq_lens[row].any()):  # its pages may be shared, and would be written to from their first slot on
+            raise ValueError(f"rows ({rows}) must be idle; free the sequences that they hold first")
         n = torch.tensor(lens, device=m.dev, dtype=torch.int32)
         tokens = torch.zeros_like(c.seq_lens).index_copy_(0, row, n)
         c.reserve(tokens)

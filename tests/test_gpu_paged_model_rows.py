@@ -90,3 +90,29 @@ def test_reserve_tells_on_the_device_whether_it_was_done():
         oc.check_status()
     none = torch.zeros(0, dtype=torch.int32, device="cuda")
     assert int(oc.reserve_pages([], none[:, None], none, c.refcounts, none, 4, return_done=True)) == 1
+
+
+def test_prompts_are_refused_on_rows_that_are_in_use():
+    p = _paged()
+    c = p.cache
+    p.prefill(_prompts(20), [0])
+    c.fork(_ints(0, -1, 0))
+    before = [x.clone() for x in (c.block_tables, c.refcounts, c.seq_lens, *c.caches)]
+    for rows in ([0], [2], [1, 2], [1, 1]):
+        with pytest.raises(ValueError, match="distinct" if rows == [1, 1] else "idle"):
+            p.prefill(_prompts(*[9] * len(rows)), rows)
+    for x, y in zip((c.block_tables, c.refcounts, c.seq_lens, *c.caches), before):
+        assert torch.equal(x, y)
+    c.free([2])
+    p.prefill(_prompts(9, 7), [2, 1])
+    assert c.seq_lens.tolist() == [20, 7, 9]
+
+
+@pytest.mark.parametrize("rows", [[3], [-1], [0, 3], [2 ** 31]])
+def test_prompts_are_refused_on_rows_outside_the_cache(rows):
+    p = _paged()
+    with pytest.raises(ValueError, match="rows of the cache"):
+        p.prefill(_prompts(*[9] * len(rows)), rows)
+    with pytest.raises(ValueError, match="at least one"):
+        p.prefill([], [])
+    assert p.cache.free_pages() == 24
