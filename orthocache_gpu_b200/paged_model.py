@@ -121,6 +121,8 @@ class PagedLlama:
         rows, n = c.seq_lens.numel(), len(prompts) * samples
         if n > rows:
             raise ValueError(f"{n} sequences, but the cache has {rows} rows")
+        if bool(c.seq_lens[:n].any()):
+            raise ValueError(f"the first {n} rows of the cache must be idle; free the sequences that they hold first")
 
         def pick(logits):
             if temperature == 0:
@@ -129,20 +131,22 @@ class PagedLlama:
             return (logits.float() / temperature - torch.log(-torch.log(u))).argmax(-1)
 
         first = [i * samples for i in range(len(prompts))]
-        logits = self.prefill(prompts, first)
-        source = torch.full((rows,), -1, dtype=torch.int32)
-        source[:n] = torch.arange(n, dtype=torch.int32) // samples * samples
-        c.fork(source.to(m.dev))
-        live = torch.zeros(rows, dtype=torch.int32, device=m.dev)
-        live[:n] = 1
-        tokens = torch.zeros(rows, dtype=torch.long, device=m.dev)
-        tokens[:n] = pick(logits.repeat_interleave(samples, 0))
-        taken = [tokens[:n].clone()]
-        for _ in range(steps - 1):
-            tokens = pick(self.step(tokens, live))
-            taken.append(tokens[:n].clone())
-        c.free(range(n))
-        c.compact()
+        try:
+            logits = self.prefill(prompts, first)
+            source = torch.full((rows,), -1, dtype=torch.int32)
+            source[:n] = torch.arange(n, dtype=torch.int32) // samples * samples
+            c.fork(source.to(m.dev))
+            live = torch.zeros(rows, dtype=torch.int32, device=m.dev)
+            live[:n] = 1
+            tokens = torch.zeros(rows, dtype=torch.long, device=m.dev)
+            tokens[:n] = pick(logits.repeat_interleave(samples, 0))
+            taken = [tokens[:n].clone()]
+            for _ in range(steps - 1):
+                tokens = pick(self.step(tokens, live))
+                taken.append(tokens[:n].clone())
+        finally:  # a step may find too few pages: what the samples hold goes back all the same
+            c.free(range(n))
+            c.compact()
         out = torch.stack(taken, 1).tolist()
         return [out[i * samples:(i + 1) * samples] for i in range(len(prompts))]
 

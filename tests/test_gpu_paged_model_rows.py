@@ -116,3 +116,17 @@ def test_prompts_are_refused_on_rows_outside_the_cache(rows):
     with pytest.raises(ValueError, match="at least one"):
         p.prefill([], [])
     assert p.cache.free_pages() == 24
+
+
+def test_samples_that_run_out_of_pages_give_theirs_back():
+    p = _paged(num_pages=5)
+    with pytest.raises(RuntimeError, match="too few free pages"):
+        p.sample(_prompts(30), 3, 12, temperature=0)  # 2 pages shared, 2 copies of the second, then 1 is left for 3
+    assert p.cache.free_pages() == 5 and not p.cache.seq_lens.any()
+    oc.check_status()
+    (got,) = p.sample(_prompts(30), 3, 2, temperature=0)
+    assert [len(t) for t in got] == [2, 2, 2]
+    p.prefill(_prompts(4), [1])
+    with pytest.raises(ValueError, match="idle"):
+        p.sample(_prompts(5), 2, 2)
+    assert p.cache.seq_lens.tolist() == [0, 4, 0]  # and the sequence that was there stays
