@@ -115,7 +115,8 @@ class PagedLlama:
                generator: Optional[torch.Generator] = None) -> List[List[List[int]]]:
         """``samples`` continuations of ``steps`` tokens for each prompt (temperature 0: greedy).
 
-        The prompts' pages are computed and held once; the cache is empty again, and compacted, afterwards.
+        The prompts' pages are computed and held once.  The samples take the first rows of the cache, which must
+        be idle and are so again, and the cache compacted, afterwards; other rows keep their sequences.
         """
         m, c = self.m, self.cache
         rows, n = c.seq_lens.numel(), len(prompts) * samples
@@ -133,7 +134,7 @@ class PagedLlama:
         first = [i * samples for i in range(len(prompts))]
         try:
             logits = self.prefill(prompts, first)
-            source = torch.full((rows,), -1, dtype=torch.int32)
+            source = torch.arange(rows, dtype=torch.int32)
             source[:n] = torch.arange(n, dtype=torch.int32) // samples * samples
             c.fork(source.to(m.dev))
             live = torch.zeros(rows, dtype=torch.int32, device=m.dev)

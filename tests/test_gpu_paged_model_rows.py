@@ -130,3 +130,13 @@ def test_samples_that_run_out_of_pages_give_theirs_back():
     with pytest.raises(ValueError, match="idle"):
         p.sample(_prompts(5), 2, 2)
     assert p.cache.seq_lens.tolist() == [0, 4, 0]  # and the sequence that was there stays
+
+
+def test_samples_leave_the_sequences_of_other_rows_alone():
+    p, alone = _paged(max_seqs=4), _paged(max_seqs=4)
+    step = torch.zeros(4, dtype=torch.long, device="cuda"), _ints(0, 0, 0, 1)
+    for x in (p, alone):
+        x.prefill(_prompts(20), [3])
+    p.sample(_prompts(30), 3, 4, temperature=0)
+    assert p.cache.seq_lens.tolist() == [0, 0, 0, 20] and p.cache.free_pages() == 22
+    assert torch.equal(p.step(*step)[3], alone.step(*step)[3])
