@@ -120,10 +120,15 @@ class PagedLlama:
         """
         m, c = self.m, self.cache
         rows, n = c.seq_lens.numel(), len(prompts) * samples
+        if samples < 1 or steps < 0:
+            raise ValueError(f"samples ({samples}) must be positive and steps ({steps}) not negative")
         if n > rows:
             raise ValueError(f"{n} sequences, but the cache has {rows} rows")
         if bool(c.seq_lens[:n].any()):
             raise ValueError(f"the first {n} rows of the cache must be idle; free the sequences that they hold first")
+
+        if n == 0 or steps == 0:
+            return [[[] for _ in range(samples)] for _ in prompts]
 
         def pick(logits):
             if temperature == 0:

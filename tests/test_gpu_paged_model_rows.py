@@ -140,3 +140,13 @@ def test_samples_leave_the_sequences_of_other_rows_alone():
     p.sample(_prompts(30), 3, 4, temperature=0)
     assert p.cache.seq_lens.tolist() == [0, 0, 0, 20] and p.cache.free_pages() == 22
     assert torch.equal(p.step(*step)[3], alone.step(*step)[3])
+
+
+def test_no_steps_no_prompts_and_counts_that_mean_nothing():
+    p = _paged()
+    assert p.sample(_prompts(30), 2, 0) == [[[], []]] and p.sample([], 2, 3) == []
+    assert [len(t) for t in p.sample(_prompts(30), 2, 1)[0]] == [1, 1]
+    for samples, steps in ((0, 3), (-1, 3), (2, -1)):
+        with pytest.raises(ValueError, match="must be positive"):
+            p.sample(_prompts(30), samples, steps)
+    assert p.cache.free_pages() == 24
