@@ -10,7 +10,9 @@
 // TypeError for dtypes, RuntimeError for devices; a step of a small model is a
 // few microseconds on the GPU, so they take their arguments by position and
 // unpack them without conversions.
+#include <c10/core/AutogradState.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/extension.h>
 
@@ -108,11 +110,24 @@ void need_cuda(const Tensor& t, const Tensor& like) {
   OC_RUNTIME(t.device() == like.device(), "tensors on different devices: ", like.device(), " and ", t.device());
 }
 
+// Whether forward-mode derivatives are being computed.
+bool forward_mode() {
+  return c10::AutogradState::get_tls_state().get_fw_grad_mode() && torch::autograd::ForwardADLevel::try_get_by_idx(0);
+}
+
+// No derivative is lost without a word: neither a backward pass nor a forward-mode one through this tensor.
+void need_constant(const Tensor& t, const char* name, bool forward) {
+  if (!t.unsafeGetTensorImpl()->autograd_meta()) return;  // has neither
+  OC_RUNTIME(!(t.requires_grad() && at::GradMode::is_enabled()), name,
+              " requires grad, and this operator has no backward pass; call it under torch.no_grad()");
+  OC_RUNTIME(!(forward && t._fw_grad(0).defined()), name,
+              " has a forward-mode derivative, and this operator does not pass it on");
+}
+
 // An input of an operator that has no backward pass.
 void need_input(const Tensor& t, const Tensor& like, const char* name) {
   need_cuda(t, like);
-  OC_RUNTIME(!(t.requires_grad() && at::GradMode::is_enabled()), name,
-              " requires grad, and this operator has no backward pass; call it under torch.no_grad()");
+  need_constant(t, name, forward_mode());
 }
 
 int float_code(const Tensor& t, const char* name) {
@@ -142,7 +157,7 @@ Tensor ints(const Tensor& t, const Tensor& like, const char* name) {
 }
 
 Tensor floats(const Tensor& t, const Tensor& like, const char* name) {
-  need_cuda(t, like);
+  need_input(t, like, name);
   OC_TYPE(t.scalar_type() == at::kFloat, name, " must be float32, got ", t.scalar_type());
   return t.contiguous();
 }
@@ -154,8 +169,8 @@ int as_int(int64_t x, const char* name) {
 
 // k_cache / v_cache (num_blocks, kv_heads, block_size, head_dim)
 void need_cache(const Tensor& k, const Tensor& v, const Tensor& like, int64_t kv_heads, int64_t head_dim) {
-  need_cuda(k, like);
-  need_cuda(v, like);
+  need_input(k, like, "k_cache");
+  need_input(v, like, "v_cache");
   OC_VALUE(k.dim() == 4 && k.sizes() == v.sizes(),
                     "k_cache and v_cache must be (num_blocks, kv_heads, block_size, head_dim) alike, got ", k.sizes(),
                     " and ", v.sizes());
@@ -488,11 +503,13 @@ struct CacheList {
     base.reserve(n);
     stride.reserve(n);
     const Tensor* first = nullptr;
+    const bool forward = forward_mode();
     for (Py_ssize_t i = 0; i < n; ++i) {
       PyObject* o = list ? PyList_GET_ITEM(caches.ptr(), i) : PyTuple_GET_ITEM(caches.ptr(), i);
       OC_TYPE(THPVariable_Check(o), "caches must be a list or tuple of tensors");
       const Tensor& c = THPVariable_Unpack(o);
       need_cuda(c, like);
+      need_constant(c, "a cache", forward);
       if (!first || c.scalar_type() != first->scalar_type() || c.sizes() != first->sizes() ||
           c.strides() != first->strides()) {
         OC_VALUE(c.dim() >= 2, "a cache must be (num_blocks, ...), got ", c.sizes());
