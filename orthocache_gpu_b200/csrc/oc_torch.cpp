@@ -124,6 +124,11 @@ void need_constant(const Tensor& t, const char* name, bool forward) {
               " has a forward-mode derivative, and this operator does not pass it on");
 }
 
+// Marks a tensor that a call writes to, as in-place operations of torch do: a backward pass that saved it fails then.
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();  // inference tensors have no version
+}
+
 // An input of an operator that has no backward pass.
 void need_input(const Tensor& t, const Tensor& like, const char* name) {
   need_cuda(t, like);
@@ -312,6 +317,10 @@ std::tuple<OptTensor, OptTensor> rotary_append(const OptTensor& q_, const OptTen
   a.num_sms = (int)num_sms;
   a.status = word(status);
   if (T > 0 && D > 0) check(oc_rotary_append_paged(&a, handle(stream)), "rotary_append_paged");
+  if (k_cache.has_value()) {
+    written(*k_cache);
+    written(*v_cache);
+  }
   return {q_out, k_out};
 }
 
@@ -493,6 +502,7 @@ std::tuple<Tensor, OptTensor> prompt(const Tensor& q_, const Tensor& k_, const T
 struct CacheList {
   std::vector<void*> base;
   std::vector<int64_t> stride;
+  std::vector<at::TensorImpl*> all;  // the tensors of the caller's list, which outlive the call
   int64_t page_bytes = 1, num_pages = 0;
 
   // a list or tuple of tensors, looked at without a conversion: a model has tens of caches, a call a few us
@@ -502,6 +512,7 @@ struct CacheList {
     const Py_ssize_t n = list ? PyList_GET_SIZE(caches.ptr()) : PyTuple_GET_SIZE(caches.ptr());
     base.reserve(n);
     stride.reserve(n);
+    all.reserve(n);
     const Tensor* first = nullptr;
     const bool forward = forward_mode();
     for (Py_ssize_t i = 0; i < n; ++i) {
@@ -525,12 +536,17 @@ struct CacheList {
         if (pages) page_bytes = bytes;
         first = &c;
       }
+      all.push_back(c.unsafeGetTensorImpl());
       base.push_back(c.data_ptr());
       stride.push_back(c.stride(0) * (int64_t)c.element_size());
     }
     if (num_pages == 0) base.clear();  // nothing to move
   }
   int count() const { return static_cast<int>(base.size()); }
+  void written() const {
+    for (at::TensorImpl* t : all)
+      if (!t->is_inference()) t->bump_version();
+  }
 };
 
 Tensor need_int32(const Tensor& t, const Tensor& like, const char* name, int64_t dim) {
@@ -557,6 +573,7 @@ void copy_pages(py::handle caches, const Tensor& src_, const Tensor& dst_, int64
   check(oc_copy_pages(c.base.data(), c.stride.data(), c.count(), c.page_bytes, c.num_pages, src.data_ptr<int32_t>(),
                       dst.data_ptr<int32_t>(), src.numel(), word(status), (int)num_sms, handle(stream)),
         "copy_pages");
+  c.written();
 }
 
 std::tuple<Tensor, Tensor, Tensor> fork_sequences(const Tensor& tables, const Tensor& lens, const Tensor& refs,
@@ -609,6 +626,9 @@ OptTensor reserve_pages(py::handle caches, const Tensor& tables, const Tensor& l
                          as_int(block_size, "block_size"), space.data_ptr(), bytes, word(status), (int)num_sms,
                          handle(stream)),
         "reserve_pages");
+  c.written();
+  written(tables);
+  written(refs);
   return return_done ? OptTensor(space.select(0, 1)) : c10::nullopt;
 }
 
@@ -630,6 +650,7 @@ std::tuple<Tensor, Tensor> compact_pages(py::handle caches, const Tensor& tables
                          as_int(tables.size(1), "max_blocks"), P, space.data_ptr(), bytes, word(status), (int)num_sms,
                          handle(stream)),
         "compact_pages");
+  c.written();
   return {t, r};
 }
 

@@ -53,3 +53,25 @@ def test_inputs_that_carry_a_derivative_are_refused(name):
     with fwd.dual_level():
         call(_inputs())
     oc.check_status()
+
+
+def test_tensors_that_are_written_to_get_a_new_version():
+    """As torch's in-place operations do it, so that a backward pass that saved the old contents fails."""
+    x = _inputs()
+    calls = _calls()
+    saved = (x["k_cache"] * torch.ones((), device="cuda", requires_grad=True)).sum()  # saves k_cache
+    for name in ("append", "reserve", "compact", "copy"):
+        before = [x[c]._version for c in ("k_cache", "v_cache")]
+        calls[name][1](x)
+        assert [x[c]._version for c in ("k_cache", "v_cache")] == [v + 1 for v in before], name
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        saved.backward()
+    table, refs = torch.full((2, 2), -1, dtype=torch.int32, device="cuda"), torch.zeros(4, dtype=torch.int32, device="cuda")
+    lens, before = torch.zeros(2, dtype=torch.int32, device="cuda"), (table._version, refs._version)
+    oc.reserve_pages([], table, lens, refs, lens + 1, 16)
+    assert (table._version, refs._version) == (before[0] + 1, before[1] + 1)
+    with torch.inference_mode():  # such tensors have no version
+        y = _inputs()
+    calls["append"][1](y)
+    calls["copy"][1](y)
+    oc.check_status()
