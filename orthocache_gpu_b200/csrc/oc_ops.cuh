@@ -15,6 +15,14 @@
 
 namespace oc {
 
+// Bound of a wait for a copy (a build option: with 0 every wait runs out), and
+// of the waits after one has run out: for the copies that are still in flight,
+// which must land before the CTA's memory is given back.
+#ifndef OC_WAIT_POLLS
+#define OC_WAIT_POLLS (1u << 22)
+#endif
+constexpr uint32_t kPolls = OC_WAIT_POLLS, kLandPolls = 1u << 22;
+
 struct fp8_t {
   uint8_t b;
 };

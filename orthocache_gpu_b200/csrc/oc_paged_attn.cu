@@ -49,7 +49,6 @@ constexpr int kLongRun = 24;     // places per CTA from which runs have a finer 
 constexpr int kTailPart = 4;     // which is one kTailPart-th of all places
 constexpr int kUnitCost = 3;     // what beginning and ending a unit costs, in tiles, when shares are equalised
 constexpr int kDirectTiles = 8;  // units of at most so many tiles get a CTA each and no joining launch
-constexpr uint32_t kPolls = 1u << 22;  // bound of a wait for a copy
 
 // ------------------------------------------------------------------ tile shape
 template <int ES, int DP, int NT>

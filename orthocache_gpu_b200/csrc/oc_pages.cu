@@ -108,7 +108,6 @@ struct Copies {
 // each warp keeps kStages pieces of up to 8 KB on their way, 192 KB an SM, and
 // spends no registers on them.  A warp takes an equal run of the pieces.
 constexpr int kCopyWarps = 6, kStages = 4, kPiece = 8192;
-constexpr uint32_t kPolls = 1u << 22;  // bound of a wait for a copy
 
 __global__ void __launch_bounds__(kCopyWarps * 32)
     copy_bulk_kernel(const __grid_constant__ Caches caches, const __grid_constant__ Copies job, Renumber table,
@@ -174,7 +173,8 @@ __global__ void __launch_bounds__(kCopyWarps * 32)
   };
   for (int i = 0; i < kStages - 1; ++i) load(begin + i);
   bool late = false;
-  for (int64_t at = begin; at < end; ++at) {
+  int64_t at = begin;
+  for (; at < end; ++at) {
     const int s = (int)((at - begin) % kStages);
     late = !mbar_wait_bounded(bar + 8 * s, (uint32_t)((at - begin) / kStages) & 1, kPolls);
     if (late) break;
@@ -188,7 +188,8 @@ __global__ void __launch_bounds__(kCopyWarps * 32)
   }
   if (late) {  // report it, and let the other copies land before the CTA's memory is reused
     raise_status(status, OC_STATUS_TIMEOUT);
-    for (int64_t at = begin; at < end && at < begin + kStages; ++at) mbar_wait_bounded(bar + 8 * (at - begin), 0, kPolls);
+    for (int64_t i = at; i < end && i < at + kStages - 1; ++i)
+      mbar_wait_bounded(bar + 8 * (uint32_t)((i - begin) % kStages), (uint32_t)((i - begin) / kStages) & 1, kLandPolls);
   }
   bulk_wait<0>();
 }

@@ -90,7 +90,6 @@ __device__ __forceinline__ Sight sight_of(const oc_prompt_args& a, const Doc& d,
 // ------------------------------------------------------------------ the tiled kernel
 constexpr int kBM = 128;       // queries of a tile; one or two tiles a CTA
 constexpr int kBN = 128;       // keys of a tile
-constexpr uint32_t kPolls = 1u << 22;  // bound of a wait
 
 template <int DP, int TILES_>
 struct Tile {

@@ -222,7 +222,6 @@ int launch(const oc_rotary_args& a, void* stream) {
 // Lane (head, column) holds its column's table entries; those, the page and
 // the position of the next tokens are read while this one is worked on.
 constexpr int kStages = 3, kStageBytes = 4096, kStreamWarps = 16;
-constexpr uint32_t kPolls = 1u << 22;  // bound of a wait for a copy
 
 // JOINED: q, k and v of a token lie side by side and make one piece.
 template <typename T, typename C, int N, bool INTER, bool JOINED>
