@@ -410,9 +410,9 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<sizeof(C), DP, NT>::PER_SM)
     for_v = s1;
   }
   uint32_t parity = 0;  // bit b: the phase of buffer b that completes next
-  auto arrived = [&](int b) {
-    const bool ok = mbar_wait_bounded(my_bar + 8 * b, parity >> b & 1, kPolls);
-    parity ^= 1u << b;
+  auto arrived = [&](int b) {  // the same answer for the whole warp
+    const bool ok = __all_sync(0xffffffffu, mbar_wait_bounded(my_bar + 8 * b, parity >> b & 1, kPolls));
+    parity ^= ok ? 1u << b : 0u;
     return ok;
   };
 
@@ -725,17 +725,21 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<sizeof(C), DP, NT>::PER_SM)
   begin_unit();
   bool from_start = cs.tile == 0;  // this CTA has the unit from its first tile
   int kb = 0;                      // buffer of the tile's keys; its values are in the next one
-  bool late = false;               // a copy did not arrive within the bound
+  unsigned owed = 0;               // a copy did not arrive within the bound: the buffers that copies are on their way to
   for (;;) {
     const int vb = kb + 1 == kBufs ? 0 : kb + 1;
-    late = !arrived(kb);
-    if (late) break;
+    if (!arrived(kb)) {  // this tile's two, and the next tile's keys
+      owed = for_v.on ? (1u << kBufs) - 1 : 1u << kb | 1u << vb;
+      break;
+    }
     scores(kb);
     __syncwarp();
     const bool more = for_v.on;
     if (more) issue(&maps.v, maps.v_role, for_v, kb);
-    late = !arrived(vb);
-    if (late) break;
+    if (!arrived(vb)) {  // this tile's values, and the next tile's two
+      owed = more ? (1u << kBufs) - 1 : 1u << vb;
+      break;
+    }
     clear_hidden(vb);
     values(vb);
     __syncwarp();
@@ -754,10 +758,11 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<sizeof(C), DP, NT>::PER_SM)
       from_start = true;
     }
   }
-  if (late) {  // report it, and let this warp's other copies land before the CTA's memory is reused
+  if (owed) {  // report it, and let this warp's copies land before the CTA's memory is reused
     raise_status(a.status, OC_STATUS_TIMEOUT);
 #pragma unroll 1
-    for (int b = 0; b < kBufs; ++b) mbar_wait_bounded(my_bar + 8 * b, parity >> b & 1, kPolls);
+    for (int b = 0; b < kBufs; ++b)
+      if (owed >> b & 1) mbar_wait_bounded(my_bar + 8 * b, parity >> b & 1, kLandPolls);
   }
 }
 

@@ -20,7 +20,11 @@ TIMEOUT = 1
 @pytest.fixture(scope="module")
 def impatient(tmp_path_factory):
     """A library of one translation unit in which no wait succeeds."""
+    done = {}
+
     def load(unit):
+        if unit in done:
+            return done[unit]
         out = str(tmp_path_factory.mktemp("late") / f"{unit}.so")
         subprocess.run([_build.nvcc(), *_build.ARCH, "-O3", "-std=c++17", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
                         "-DOC_WAIT_POLLS=0", "-shared", os.path.join(_build.CSRC, f"{unit}.cu"), "-o", out, "-lcudart"], check=True)
@@ -28,6 +32,7 @@ def impatient(tmp_path_factory):
         for name, (res, args) in _lib.SIGNATURES.items():
             if hasattr(lib, name):
                 getattr(lib, name).restype, getattr(lib, name).argtypes = res, args
+        done[unit] = lib
         return lib
     return load
 
@@ -54,3 +59,31 @@ def test_page_copies(impatient):
         oc.check_status()
         for c, b in zip(caches, before):
             assert torch.equal(c[pairs:], b[:pairs])
+
+
+@pytest.mark.parametrize("lens", [[40, 300, 0], [1, 20000]])
+def test_paged_decode(impatient, lens):
+    """Units of a CTA each, and units that are split: the launch ends, and the next one of the same GPU is right."""
+    from test_paged_decode_plan import Args
+    from serving_helpers import pages_for
+    lib = impatient("oc_paged_attn")
+    table, pages = pages_for(lens, 16, "cuda")
+    n = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    q = torch.randn(len(lens), 8, 64, device="cuda", dtype=torch.bfloat16)
+    k, v = (torch.randn(pages, 2, 16, 64, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    want = oc.paged_decode_attention(q, k, v, table, n)
+    out, status = torch.empty_like(q), torch.zeros(1, dtype=torch.int32, device="cuda")
+    a = Args(q=q.data_ptr(), k_cache=k.data_ptr(), v_cache=v.data_ptr(), out=out.data_ptr(), block_tables=table.data_ptr(),
+             seq_lens=n.data_ptr(), q_seq_stride=q.stride(0), q_head_stride=q.stride(1), out_seq_stride=out.stride(0),
+             out_head_stride=out.stride(1), kc_block_stride=k.stride(0), kc_head_stride=k.stride(1), kc_tok_stride=k.stride(2),
+             vc_block_stride=v.stride(0), vc_head_stride=v.stride(1), vc_tok_stride=v.stride(2),
+             block_table_stride=table.stride(0), num_blocks=pages, status=status.data_ptr(), scale=0.125, k_scale=1.0,
+             v_scale=1.0, num_seqs=len(lens), kv_heads=2, group=4, head_dim=64, dtype=_lib.OC_BF16, cache_dtype=_lib.OC_BF16,
+             block_size=16, max_blocks=table.shape[1], num_sms=148)
+    a.workspace_bytes = lib.oc_paged_decode_workspace_bytes(C.byref(a))
+    space = torch.empty(max(1, a.workspace_bytes), dtype=torch.uint8, device="cuda")
+    a.workspace = space.data_ptr()
+    assert lib.oc_paged_decode_attention(C.byref(a), _stream()) == 0
+    assert status.item() == TIMEOUT
+    assert torch.equal(oc.paged_decode_attention(q, k, v, table, n), want)
+    oc.check_status()
