@@ -354,7 +354,8 @@ __global__ void __launch_bounds__(kStreamWarps * 32, 1)
   int stage = 0;
   uint32_t parity = 0;
   bool late = false;
-  for (int64_t left = end - begin; left > 0; --left) {
+  int64_t left = end - begin;
+  for (; left > 0; --left) {
     if (now.page == -1 && lane == 0) raise_status(a.status, OC_STATUS_BAD_PAGE);
     const Piece p = piece_of(i);
     late = !__all_sync(0xffffffffu, mbar_wait_bounded(my_bar + 8 * stage, parity >> stage & 1, kPolls));
@@ -436,10 +437,13 @@ __global__ void __launch_bounds__(kStreamWarps * 32, 1)
       ahead = place_of(t + 2);
     }
   }
-  if (late) {  // report it, and let this warp's other copies land before the CTA's memory is reused
+  if (late) {  // report it, and let this warp's copies land before the CTA's memory is reused
     if (lane == 0) raise_status(a.status, OC_STATUS_TIMEOUT);
 #pragma unroll 1
-    for (int b = 0; b < kStages; ++b) mbar_wait_bounded(my_bar + 8 * b, parity >> b & 1, kPolls);
+    for (int i = 0; i < kStages && i < left; ++i) {
+      mbar_wait_bounded(my_bar + 8 * stage, parity >> stage & 1, kLandPolls);
+      stage = stage + 1 == kStages ? 0 : stage + 1;
+    }
   }
 }
 

@@ -87,3 +87,38 @@ def test_paged_decode(impatient, lens):
     assert status.item() == TIMEOUT
     assert torch.equal(oc.paged_decode_attention(q, k, v, table, n), want)
     oc.check_status()
+
+
+class RotaryArgs(C.Structure):
+    """oc_rotary_args of include/orthocache_b200.h."""
+
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v", "q_out", "k_out")] + \
+        [(n, C.c_int64) for n in ("q_tok_stride", "q_head_stride", "k_tok_stride", "k_head_stride", "v_tok_stride",
+                                  "v_head_stride", "qo_tok_stride", "qo_head_stride", "ko_tok_stride", "ko_head_stride", "tokens")] + \
+        [(n, C.c_void_p) for n in ("positions", "seq_ids", "cos_tab", "sin_tab")] + [("table_rows", C.c_int64)] + \
+        [(n, C.c_void_p) for n in ("k_cache", "v_cache")] + \
+        [(n, C.c_int64) for n in ("kc_block_stride", "kc_head_stride", "kc_tok_stride", "vc_block_stride", "vc_head_stride",
+                                  "vc_tok_stride")] + [("block_tables", C.c_void_p)] + \
+        [(n, C.c_int64) for n in ("block_table_stride", "num_blocks")] + [("status", C.c_void_p)] + \
+        [(n, C.c_float) for n in ("k_scale", "v_scale")] + \
+        [(n, C.c_int) for n in ("q_heads", "kv_heads", "head_dim", "rotary_dim", "dtype", "cache_dtype", "positions_64", "flags",
+                                "block_size", "max_blocks", "num_seqs", "num_sms")]
+
+
+@pytest.mark.parametrize("T, H", [(2400, 1), (2400, 40), (9000, 3)])
+def test_rotary_of_prompts(impatient, T, H):
+    """One piece a warp, and more than its ring holds."""
+    lib, status = impatient("oc_rotary"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    x = torch.randn(T, H, 128, device="cuda", dtype=torch.float16)
+    pos = torch.arange(T, device="cuda", dtype=torch.int32)
+    cos, sin = oc.rotary_tables(128, T, device="cuda")
+    want = oc.rotary_embedding(x, pos, cos, sin)
+    out = torch.full_like(x, 7.0)
+    a = RotaryArgs(q=x.data_ptr(), q_out=out.data_ptr(), q_tok_stride=x.stride(0), q_head_stride=x.stride(1),
+                   qo_tok_stride=x.stride(0), qo_head_stride=x.stride(1), tokens=T, positions=pos.data_ptr(),
+                   cos_tab=cos.data_ptr(), sin_tab=sin.data_ptr(), table_rows=T, status=status.data_ptr(), k_scale=1.0, v_scale=1.0,
+                   q_heads=H, head_dim=128, rotary_dim=128, dtype=_lib.OC_F16, num_sms=148)
+    assert lib.oc_rotary_append_paged(C.byref(a), _stream()) == 0
+    assert status.item() == TIMEOUT and bool((out == 7.0).all())
+    assert torch.equal(oc.rotary_embedding(x, pos, cos, sin), want)
+    oc.check_status()
