@@ -122,3 +122,30 @@ def test_rotary_of_prompts(impatient, T, H):
     assert status.item() == TIMEOUT and bool((out == 7.0).all())
     assert torch.equal(oc.rotary_embedding(x, pos, cos, sin), want)
     oc.check_status()
+
+
+class PromptArgs(C.Structure):
+    """oc_prompt_args of include/orthocache_b200.h."""
+
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v", "out", "lse", "slopes", "cu_q", "cu_k", "prefix_lens")] + \
+        [(n, C.c_int64) for n in ("q_tok_stride", "q_head_stride", "k_tok_stride", "k_head_stride", "v_tok_stride",
+                                  "v_head_stride", "out_tok_stride", "out_head_stride", "lse_tok_stride", "tokens", "key_tokens")] + \
+        [("status", C.c_void_p)] + [(n, C.c_float) for n in ("scale", "softcap")] + \
+        [(n, C.c_int) for n in ("docs", "kv_heads", "group", "head_dim", "dtype", "causal", "window", "num_sms")]
+
+
+@pytest.mark.parametrize("T, D", [(100, 64), (900, 64), (900, 128), (5000, 64)])
+def test_prompt_attention(impatient, T, D):
+    """Tensor memory and the SM are given back: the next launches are right."""
+    lib, status = impatient("oc_prompt_attn"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    q, k, v = (torch.randn(T, h, D, device="cuda", dtype=torch.bfloat16) for h in (4, 2, 2))
+    want, out = oc.prompt_attention(q, k, v), torch.empty_like(q)
+    a = PromptArgs(q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), out=out.data_ptr(), q_tok_stride=q.stride(0),
+                   q_head_stride=D, k_tok_stride=k.stride(0), k_head_stride=D, v_tok_stride=v.stride(0), v_head_stride=D,
+                   out_tok_stride=out.stride(0), out_head_stride=D, tokens=T, key_tokens=T, status=status.data_ptr(),
+                   scale=D ** -0.5, docs=1, kv_heads=2, group=2, head_dim=D, dtype=_lib.OC_BF16, causal=1, num_sms=148)
+    for _ in range(3):
+        assert lib.oc_prompt_attention(C.byref(a), _stream()) == 0
+    assert status.item() == TIMEOUT
+    assert torch.equal(oc.prompt_attention(q, k, v), want)
+    oc.check_status()
