@@ -936,6 +936,7 @@ bool tiled(const oc_paged_decode_args& a) {
 struct Plan {
   bool direct;
   int64_t grid, late;  // CTAs, and those of them that wait for others to leave
+  int64_t places;      // of all units at their longest, where they are split: kernels count them in 32 bits
   int nt;
 };
 
@@ -949,6 +950,7 @@ void plan_nt(const oc_paged_decode_args& a, Plan& p) {
   const int64_t useful = (units * (tiles + kUnitCost) + kMinShare - 1) / kMinShare;
   p.nt = NT;
   p.direct = tiles <= kDirectTiles;
+  p.places = p.direct ? 0 : units * (tiles + kUnitCost);
   p.late = ES > 1 && !p.direct && units * (tiles + kUnitCost) >= kLongRun * wave ? wave : 0;
   p.grid = p.direct ? units : useful < wave ? useful : wave + p.late;
 }
@@ -1044,7 +1046,7 @@ int launch_tiled(const oc_paged_decode_args& a, const Plan& p, void* stream) {
 template <typename T, typename C, int DP>
 int launch_nt(const oc_paged_decode_args& a, void* stream) {
   const Plan p = plan_of<sizeof(C), DP>(a);
-  if (p.grid > 0x7fffffff) return OC_ERR_TOO_LARGE;
+  if (p.grid > 0x7fffffff || p.places > 0x7fffffff) return OC_ERR_TOO_LARGE;
   if constexpr (DP < 256) {
     if (p.nt == 2) return launch_tiled<T, C, DP, 2>(a, p, stream);
   }

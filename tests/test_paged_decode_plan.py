@@ -42,3 +42,13 @@ def test_a_window_that_hides_nothing_does_not_change_the_plan():
     for window in (2048 * 16, 2 ** 31 - 33, 2 ** 31 - 1):
         assert lib.oc_paged_decode_workspace_bytes(C.byref(args(window=window))) == whole, window
     assert lib.oc_paged_decode_workspace_bytes(C.byref(args(window=64))) == 0  # a few tiles: no split
+
+
+def test_more_tiles_than_32_bits_count_are_refused_before_any_cuda_call():
+    """A table of 65535 sequences of up to 2^20 tokens and 64 kv heads: 2^22 units of more than 2^12 tiles."""
+    lib, at = _lib.load(), 1 << 20  # an aligned address that nothing reads
+    big = dict(num_seqs=65535, kv_heads=64, group=1, block_size=16, max_blocks=1 << 16, q=at, k_cache=at, v_cache=at, out=at,
+               block_tables=at, seq_lens=at, workspace=at, workspace_bytes=1 << 40)
+    assert lib.oc_paged_decode_attention(C.byref(args(**big)), None) == 5
+    assert lib.oc_paged_decode_attention(C.byref(args(**dict(big, dtype=_lib.OC_F16, cache_dtype=_lib.OC_F8E4M3, head_dim=64,
+                                                             max_blocks=1 << 20))), None) == 5
