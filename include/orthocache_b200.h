@@ -494,7 +494,7 @@ int oc_fork_sequences(const int32_t* table_in, int64_t table_in_stride, int32_t*
  * OC_STATUS_PAGES is set.
  * workspace: oc_reserve_workspace_bytes(num_seqs, num_pages) bytes; its second
  * int32 is 1 afterwards if the pages were reserved, else 0, for launches that
- * must not write where they were not. */
+ * must not write where they were not (num_seqs 0 launches nothing). */
 size_t oc_reserve_workspace_bytes(int num_seqs, int64_t num_pages);
 int oc_reserve_pages(void* const* caches, const int64_t* page_strides, int num_caches, int64_t page_bytes,
                      int32_t* table, int64_t table_stride, const int32_t* lens, int32_t* refs, const int32_t* wanted,

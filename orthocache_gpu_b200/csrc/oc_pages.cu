@@ -10,10 +10,10 @@
 // a dependent launch over all caches; they are bound by memory bandwidth.
 //
 // Measured on one B200, in a graph: 64 sequences of up to 900 tokens over 4096
-// pages of 16, fork 3.6 us, reserve 3.0 us without a request; fork, reserve
-// and the copies of 32 pages in each of 44 caches together 11.2 us, three
+// pages of 16, fork 3.5 us, reserve 3.2 us without a request; fork, reserve
+// and the copies of 32 pages in each of 44 caches together 11.4 us, three
 // launches that each wait for the one before.  Compaction of the same after
-// half of the sequences have ended, over 44 caches of 8 KB pages: 102 us, of
+// half of the sequences have ended, over 44 caches of 8 KB pages: 101 us, of
 // which the copies take 89 (6.2 TB/s, read and write).
 #include <cooperative_groups.h>
 

@@ -12,7 +12,7 @@
 // Measured on one B200: one token of 32 + 4 heads of 64, 2.5 us in a graph and
 // 5.9 us a call, which is the host's time; 64 tokens of 32 + 8 heads of 128,
 // 3.2 us in a graph.  8191 tokens of 32 + 8 heads of 128 in bfloat16 with an
-// 8-bit cache, 38 us (4.9 TB/s of 189 MB): instructions are issued in 61% of
+// 8-bit cache, 37 us (5.1 TB/s of 189 MB): instructions are issued in 60% of
 // the cycles, and the conversions to 8 bits take as many as the rotation.
 #include "oc_ops.cuh"
 #include "oc_ptx.cuh"
@@ -463,7 +463,8 @@ int launch_aligned(const oc_rotary_args& a, void* stream) {
   int columns;
   if (!streams<T, N, INTER>(a, columns)) return launch<T, C, N, true, INTER>(a, stream);
   constexpr int smem = kStreamWarps * kStages * kStageBytes;
-  // parts of one projection's output, small enough for one piece a token (8 + 2 heads of 128: 62 us apart, 52 joined)
+  // parts of one projection's output, small enough for one piece a token (25147 tokens of 8 + 2 heads
+  // of 128: 53 us apart, 40 joined)
   const bool joined = a.q && a.k && a.v && a.q_tok_stride == a.k_tok_stride && a.q_tok_stride == a.v_tok_stride &&
                       static_cast<const T*>(a.q) + a.q_heads * a.head_dim == a.k &&
                       static_cast<const T*>(a.k) + a.kv_heads * a.head_dim == a.v &&

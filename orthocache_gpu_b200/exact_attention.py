@@ -32,7 +32,8 @@ def paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
 
     Splits the work over the cache's length where there are few sequences; nothing synchronises with the
     host.  A length or a page outside its tables sets the device's status word (:func:`check_status`); the
-    length is clamped, and the page's keys and values count as zeros.
+    length is clamped, and the page's keys and values count as zeros.  float32, and caches that are not aligned
+    to 16 bytes or broadcast over heads, are not split and take many times as long for long sequences.
     """
     return _lib.require_binding().decode(q, k_cache, v_cache, block_tables, seq_lens, scale, softcap, alibi_slopes,
                                          window, k_scale, v_scale, return_lse)
@@ -51,6 +52,9 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     j > p - window; and every key below ``prefix_lens[d]``.  The bias is -alibi_slopes[h] * |p - j|.
     float16 and bfloat16 with head_dim a multiple of 8 up to 128; float32 up to 256.  Returns out like q,
     or (out, lse) with lse (tokens, heads) float32.
+
+    float32, and 16-bit inputs that are not aligned to 16 bytes or broadcast over heads, go row by row, which
+    takes hundreds of times as long for long prompts: make such k and v contiguous first.
     """
     return _lib.require_binding().prompt(q, k, v, cu_seqlens, cu_seqlens_k, causal, prefix_lens, window, scale, softcap,
                                          alibi_slopes, return_lse)

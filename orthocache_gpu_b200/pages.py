@@ -70,7 +70,9 @@ class PagedKVCache:
     """The paged key and value caches of every layer, with their tables.
 
     ``k[layer]`` / ``v[layer]`` are (num_pages, kv_heads, block_size, head_dim).  Rows of the tables are
-    the sequences of a batch; a row with length 0 and no pages is idle.
+    the sequences of a batch; a row with length 0 and no pages is idle.  :meth:`fork`, :meth:`free` and
+    :meth:`compact` put new tensors in the place of the tables, so a captured graph that read the old ones has
+    to be captured again; :meth:`reserve` and the appends work in place.
     """
 
     def __init__(self, layers: int, num_pages: int, kv_heads: int, head_dim: int, *, max_seqs: int, max_tokens: int,
